@@ -37,6 +37,10 @@ typedef struct CUstream_st* ir_stream_t; /* == cudaStream_t */
 #define IR_DTYPE_BF16 1
 #define IR_DTYPE_F16 2
 
+/* element formats of 8-bit K/V pools */
+#define IR_KV_E4M3 1 /* 4-bit exponent, 3-bit mantissa, largest 448 (0x7f, 0xff: NaN) */
+#define IR_KV_INT8 2 /* -127 .. 127 */
+
 /* host-side status codes */
 #define IR_OK 0
 #define IR_ERR_INVALID_ARG 1
@@ -438,6 +442,104 @@ int ir_derive_varlen_metadata(const int64_t* gather_slots, int64_t num_keys, con
                               int block_size, int max_blocks, int32_t* block_tables,
                               int32_t* context_lens, int32_t* q_start, int32_t* num_seqs,
                               int32_t* scratch, int32_t* err_flag, ir_stream_t stream);
+
+/* ---------------------------------------------------------- 8-bit K/V cache
+ *
+ * Pools of one layer as codes [num_slots, num_kv_heads, head_dim] of one byte
+ * (kv_format IR_KV_*; 16-byte aligned) with one fp32 scale per (block, kv
+ * head), k_scale / v_scale [num_blocks, num_kv_heads] contiguous: the value of
+ * an element is code * scale. Half the bytes of a 16-bit pool per token.
+ * No reference counterpart (infrared's pool is of the model's dtype,
+ * infrared/cache/paged_kv_cache.py:30-46); slots, block tables and context
+ * lengths are those of the 16-bit calls.
+ */
+
+/* Workspace bytes of ir_cache_write_q8 for this many tokens (0: none needed;
+ * no initialisation, no state between calls). */
+size_t ir_cache_write_q8_workspace_size(int64_t num_tokens, int64_t num_slots,
+                                        int block_size);
+
+/*
+ * Quantise this step's K/V rows into the pool. For every (block, kv head) the
+ * rows touch, with amax the largest finite magnitude of the rows,
+ *   scale = max(scale, smallest power of two s >= 2^-126 with
+ *                      amax <= 448 s (e4m3) or 127 s (int8)),
+ * the codes of the block's other rows are rescaled if it grew, and the new
+ * rows become round(x / scale), ties to even. A write that holds a block's
+ * first row (slot % block_size == 0) begins the block: its old scale does not
+ * count and rows that the call does not write are no longer defined. So a
+ * block filled in order, by one call or token by token, ends with the scale of
+ * its own rows. An element that is not finite becomes NaN: in e4m3 its own
+ * code, in int8 the scale of its (block, kv head) until the block is begun
+ * again. A negative slot skips the row; a slot >= num_slots is skipped and
+ * flagged IR_DEVERR_SLOT; of two rows for one slot the later one counts. The
+ * result does not depend on the order of the other rows.
+ * k, v: [num_tokens, num_kv_heads, head_dim] of dtype with row strides in
+ * elements; head_dim 64 or 128; block_size up to 1024.
+ */
+int ir_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                      void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                      const int64_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+                      int head_dim, int block_size, int64_t num_slots, int dtype,
+                      int kv_format, void* workspace, size_t workspace_bytes,
+                      int32_t* err_flag, ir_stream_t stream);
+
+/*
+ * Read rows back by slot: out[i, h, :] = code * scale, rounded once to dtype
+ * (finite values beyond its range saturate); out [num_rows, num_kv_heads,
+ * head_dim] contiguous. A slot outside [0, num_slots) gives a zero row and sets
+ * IR_DEVERR_SLOT.
+ */
+int ir_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
+                       int64_t num_rows, int num_kv_heads, int head_dim, int block_size,
+                       int64_t num_slots, int dtype, int kv_format, int32_t* err_flag,
+                       ir_stream_t stream);
+
+/* ir_paged_decode over an 8-bit pool: shape->dtype is the type of q and out,
+ * shape->flags must be 0. Workspace and plan of the same shape come from the
+ * two calls below (path 2: TMA + mma kernel for 16-bit q, block_size 8 or a
+ * multiple of 16; path 1: CUDA cores for everything else). Scores, softmax and
+ * sums are fp32; scales may have any value. */
+size_t ir_paged_decode_q8_workspace_size(const ir_decode_shape* shape, int kv_format);
+int ir_paged_decode_q8_plan(const ir_decode_shape* shape, int kv_format, int* path,
+                            int* ctas_per_kv_head);
+int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                       const float* k_scale, const float* v_scale, int kv_format,
+                       const int32_t* block_tables, const int32_t* context_lens,
+                       const ir_decode_shape* shape, void* workspace, size_t workspace_bytes,
+                       int32_t* err_flag, ir_stream_t stream);
+
+/* ir_paged_prefill over an 8-bit pool. The blocks of the sequences' histories
+ * are expanded once into a pool of shape->dtype in the workspace (two launches
+ * in all), which the prefill kernel then attends over: a block's conversion is
+ * paid once, not once per 128 query rows and head. In bf16 and fp32 the
+ * expanded values are exact for power-of-two scales. The workspace holds one
+ * layer's pool of shape->dtype and can serve every layer. */
+size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape);
+int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                        const float* k_scale, const float* v_scale, int kv_format,
+                        const int32_t* block_tables, const int32_t* context_lens,
+                        const int32_t* q_start, const ir_prefill_shape* shape, void* workspace,
+                        size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream);
+
+/*
+ * RMS norm of every query and key head over its head_dim elements, and the
+ * rotary embedding, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * w,  out = y * cos + rotate_half(y) * sin
+ * in fp32, rounded once. q [num_tokens, num_heads, head_dim] and k [num_tokens,
+ * num_kv_heads, head_dim] with token strides q_stride / k_stride (elements;
+ * views of one QKV projection may be given), q_out / k_out alike (they may be
+ * q and k themselves, but not other overlapping memory); w_q / w_k [head_dim]
+ * of dtype or null (weight one); rope_cos / rope_sin fp32 rows [num_tokens,
+ * head_dim] with rope_stride, as infrared's RotaryEmbedding returns them
+ * (infrared/model/layers.py:121-136; rotate_half :72-77). head_dim 64 or 128.
+ */
+int ir_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_stride,
+                    int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride,
+                    const void* w_q, const void* w_k, const float* rope_cos,
+                    const float* rope_sin, int64_t rope_stride, float eps, int64_t num_tokens,
+                    int num_heads, int num_kv_heads, int head_dim, int dtype,
+                    ir_stream_t stream);
 
 /* ---------------------------------------------------------- peer exchange
  *

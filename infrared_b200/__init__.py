@@ -14,7 +14,12 @@ Three hand-written sm_100a CUDA paths behind a C ABI
 * ``paged_decode_lse`` + ``lse_merge`` — partials of a KV range and their
   combination, used to spread one long context over several GPUs;
 * ``paged_prefill`` — causal attention of packed query rows (prefill with a
-  cached prefix, mixed prefill + decode frames) on the tcgen05 tensor cores.
+  cached prefix, mixed prefill + decode frames) on the tcgen05 tensor cores;
+* ``cache_write_q8`` / ``cache_gather_q8`` / ``paged_decode_q8`` /
+  ``paged_prefill_q8`` — the same over a cache of 8-bit codes (e4m3 or int8)
+  with one scale per block and kv head, quantised as it is written;
+* ``qk_norm_rope`` — RMS norm of every query and key head with the rotary
+  embedding in the same pass.
 
 ``PagedKVPool``, ``PagedContext`` and ``paged_attention`` keep the
 reference engine's interface; ``shim.install()`` routes infrared's own
@@ -23,15 +28,18 @@ decode calls here; ``dist`` shards the work over the GPUs of one node.
 
 from ._lib import InfraredB200Error, UnsupportedShape
 from .attention import paged_attention
-from .ops import (DeviceError, cache_gather, cache_write, check_device_errors,
-                  derive_block_metadata, kv_proj_rope_write, lse_merge, paged_decode,
-                  paged_decode_lse, paged_decode_rope, paged_decode_rope_write,
-                  paged_decode_write, paged_prefill)
+from .ops import (DeviceError, cache_gather, cache_gather_q8, cache_write, cache_write_q8,
+                  check_device_errors, derive_block_metadata, kv_proj_rope_write, lse_merge,
+                  paged_decode, paged_decode_lse, paged_decode_q8, paged_decode_rope,
+                  paged_decode_rope_write, paged_decode_write, paged_prefill, paged_prefill_q8,
+                  qk_norm_rope)
 from .paged_kv_cache import PagedContext, PagedKVPool
 
 __all__ = [
     "DeviceError", "InfraredB200Error", "PagedContext", "PagedKVPool", "UnsupportedShape",
-    "cache_gather", "cache_write", "check_device_errors", "derive_block_metadata",
-    "kv_proj_rope_write", "lse_merge", "paged_attention", "paged_decode", "paged_decode_lse",
-    "paged_decode_rope", "paged_decode_rope_write", "paged_decode_write", "paged_prefill",
+    "cache_gather", "cache_gather_q8", "cache_write", "cache_write_q8", "check_device_errors",
+    "derive_block_metadata", "kv_proj_rope_write", "lse_merge", "paged_attention",
+    "paged_decode", "paged_decode_lse", "paged_decode_q8", "paged_decode_rope",
+    "paged_decode_rope_write", "paged_decode_write", "paged_prefill", "paged_prefill_q8",
+    "qk_norm_rope",
 ]

@@ -13,6 +13,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,7 +24,7 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "libinfrared_b200.so"
 
 SOURCES = ["capi.cu", "cache_ops.cu", "decode_generic.cu", "decode_tma.cu", "prefill_tc.cu",
-           "peer_exchange.cu", "kv_proj.cu"]
+           "peer_exchange.cu", "kv_proj.cu", "cache_q8.cu", "decode_q8.cu", "qk_norm_rope.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -54,18 +56,24 @@ def build(force: bool = False, verbose: bool = False, out: Path | None = None,
     dst = Path(out) if out is not None else LIB
     if out is None and not defines and not force and up_to_date():
         return LIB
-    cmd = [
-        nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo",
-        "-Xcompiler", "-fPIC,-O3", "-shared", "-cudart", "static",
-        "--expt-relaxed-constexpr", "-I", str(INCLUDE),
-        *[f"-D{d}" for d in defines],
-        "-o", str(dst) + ".tmp",
-        *[str(CSRC / s) for s in SOURCES],
-    ]
+    flags = ["-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC,-O3",
+             "--expt-relaxed-constexpr", "-I", str(INCLUDE), *[f"-D{d}" for d in defines]]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True, cwd=str(CSRC))
+        flags.insert(0, "-Xptxas=-v")
+    # the sources are independent: compile them side by side, then link
+    with tempfile.TemporaryDirectory() as tmp:
+        def compile_one(src: str) -> str:
+            obj = str(Path(tmp) / (src + ".o"))
+            cmd = [nvcc(), *flags, "-c", "-o", obj, str(CSRC / src)]
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            subprocess.run(cmd, check=True, cwd=str(CSRC))
+            return obj
+
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            objects = list(pool.map(compile_one, SOURCES))
+        subprocess.run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-Xcompiler", "-fPIC",
+                        "-o", str(dst) + ".tmp", *objects], check=True)
     os.replace(str(dst) + ".tmp", dst)
     return dst
 

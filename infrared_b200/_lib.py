@@ -20,6 +20,7 @@ LIB_PATH = Path(os.environ.get("INFRARED_B200_LIB") or
                 Path(__file__).resolve().with_name("libinfrared_b200.so"))
 
 IR_DTYPE_F32, IR_DTYPE_BF16, IR_DTYPE_F16 = 0, 1, 2
+IR_KV_E4M3, IR_KV_INT8 = 1, 2
 IR_OK, IR_ERR_INVALID_ARG, IR_ERR_UNSUPPORTED, IR_ERR_CUDA, IR_ERR_WORKSPACE = range(5)
 IR_DECODE_DYNAMIC_TAIL = 1   # ir_decode_shape.flags (the workspace zero-filled)
 IR_DECODE_INLINE_MERGE = 2
@@ -151,6 +152,27 @@ _SIGNATURES = {
                                     c_size_t, c_void_p, c_void_p]),
     "ir_lse_merge": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
                              c_int, c_int, c_int, c_int, c_void_p]),
+    "ir_cache_write_q8_workspace_size": (c_size_t, [c_int64, c_int64, c_int]),
+    "ir_cache_write_q8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                  c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p,
+                                  c_void_p]),
+    "ir_cache_gather_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                   c_int, c_int, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "ir_paged_decode_q8_workspace_size": (c_size_t, [POINTER(DecodeShape), c_int]),
+    "ir_paged_decode_q8_plan": (c_int, [POINTER(DecodeShape), c_int, POINTER(c_int),
+                                        POINTER(c_int)]),
+    "ir_paged_decode_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_int, c_void_p, c_void_p, POINTER(DecodeShape), c_void_p,
+                                   c_size_t, c_void_p, c_void_p]),
+    "ir_paged_prefill_q8_workspace_size": (c_size_t, [POINTER(PrefillShape)]),
+    "ir_paged_prefill_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_int, c_void_p, c_void_p, c_void_p, POINTER(PrefillShape),
+                                    c_void_p, c_size_t, c_void_p, c_void_p]),
+    "ir_qk_norm_rope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_int64, c_float, c_int64, c_int, c_int, c_int, c_int,
+                                c_void_p]),
     "ir_paged_decode_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p, POINTER(DecodeShape), c_void_p,
                                         c_void_p]),

@@ -74,32 +74,39 @@ int sm_count_now(int) {
 }
 
 // key encoding for the occupancy cache:
-// path(2 bits) dtype(2) D==128(1) bs8(1) log2(head group)(2)
-int occ_key(int path, const ir_decode_shape* s) {
+// path(2 bits) dtype(2) D==128(1) bs8(1) log2(head group)(2) 8-bit format(2)
+int occ_key(int path, const ir_decode_shape* s, int fmt) {
   const int hg = path == 2 ? irb::tma_head_group(s->num_kv_heads) : 1;
   const int lg = hg == 8 ? 3 : hg == 4 ? 2 : hg == 2 ? 1 : 0;
   return path | (s->dtype << 2) | ((s->head_dim == 128) << 4) |
-         ((s->block_size == 8) << 5) | (lg << 6);
+         ((s->block_size == 8) << 5) | (lg << 6) | (fmt << 8);
 }
 
 int occ_compute(int key) {
   const int path = key & 3, dtype = (key >> 2) & 3, d128 = (key >> 4) & 1,
-            bs8 = (key >> 5) & 1, hg = 1 << ((key >> 6) & 3);
+            bs8 = (key >> 5) & 1, hg = 1 << ((key >> 6) & 3), fmt = (key >> 8) & 3;
   const int D = d128 ? 128 : 64;
   if (path == 2) return irb::decode_tma_occupancy(dtype, D, hg, bs8 ? 8 : 16);
-  return irb::decode_generic_occupancy(dtype, D);
+  return irb::decode_generic_occupancy(dtype, D, fmt);
+}
+
+// kv heads that one CTA of the TMA kernels covers (fmt: 8-bit pools).
+int head_group(const ir_decode_shape* s, int fmt) {
+  return fmt ? irb::q8_head_group(s->num_kv_heads, s->num_heads / s->num_kv_heads)
+             : irb::tma_head_group(s->num_kv_heads);
 }
 
 // CTAs per kv head (generic) or per head group (TMA) for this path.
-int ctas_per_group(int path, const ir_decode_shape* s, int* out) {
+int ctas_per_group(int path, const ir_decode_shape* s, int* out, int fmt = 0) {
   int sms = 1, occ = 1;
   int e = cached(-1, sm_count_now, 0, &sms);
   if (e) return e;
-  const int key = occ_key(path, s);
-  e = cached(key, occ_compute, key, &occ);
-  if (e) return e;
-  const int groups = path == 2 ? s->num_kv_heads / irb::tma_head_group(s->num_kv_heads)
-                               : s->num_kv_heads;
+  if (!(path == 2 && fmt)) {  // (the 8-bit TMA kernel fills an SM's shared memory: one CTA)
+    const int key = occ_key(path, s, fmt);
+    e = cached(key, occ_compute, key, &occ);
+    if (e) return e;
+  }
+  const int groups = path == 2 ? s->num_kv_heads / head_group(s, fmt) : s->num_kv_heads;
   int G = (sms * occ) / groups;
   *out = G < 1 ? 1 : (G > 65535 ? 65535 : G);
   return 0;
@@ -193,6 +200,26 @@ bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int64_t col
   return r == CUDA_SUCCESS;
 }
 
+// An 8-bit pool [num_slots, Hkv, D] as a 3-D (D bytes, slots, heads) map: one
+// copy moves the rows of a block for a head group, one [rows x D] region per
+// head under a swizzle as wide as the row.
+bool make_pool_map_q8(CUtensorMap* map, const void* pool, int64_t num_slots, int hkv, int d,
+                      int box_rows, int head_group) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(num_slots),
+                              static_cast<cuuint64_t>(hkv)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(hkv) * d, static_cast<cuuint64_t>(d)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(d), static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(head_group)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pool), dims, strides,
+                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // ------------------------------------------------------------ planning
 
 struct Plan {
@@ -252,22 +279,32 @@ bool tma_eligible(const ir_decode_shape* s) {
          s->num_slots <= INT32_MAX && (s->q_stride % 2) == 0;
 }
 
-int make_plan(const ir_decode_shape* s, Plan* p) {
+// The 8-bit TMA kernel takes groups of up to 16 (two sets of 8 query heads).
+bool q8_eligible(const ir_decode_shape* s) {
+  return (s->dtype == IR_DTYPE_BF16 || s->dtype == IR_DTYPE_F16) &&
+         (s->block_size == 8 || s->block_size % 16 == 0) && s->num_slots <= INT32_MAX;
+}
+
+bool kv_format_ok(int fmt) { return fmt == IR_KV_E4M3 || fmt == IR_KV_INT8; }
+
+int make_plan(const ir_decode_shape* s, Plan* p, int fmt = 0) {
   int rc = check_shape(s);
   if (rc) return rc;
-  int path = tma_eligible(s) ? 2 : 1;
+  if (fmt && s->flags)
+    return fail(IR_ERR_INVALID_ARG, "flags must be 0 for an 8-bit pool");
+  int path = (fmt ? q8_eligible(s) : tma_eligible(s)) ? 2 : 1;
   if (g_forced_path == 1) path = 1;
   if (g_forced_path == 2) {
     if (path != 2)
       return fail(IR_ERR_UNSUPPORTED, "TMA path forced but shape not eligible");
   }
   int G = 1;
-  int e = ctas_per_group(path, s, &G);
+  int e = ctas_per_group(path, s, &G, fmt);
   if (e) return cuda_status(e, "cudaGetDevice");
   p->path = path;
   p->G = G;
   const int64_t B = s->batch, H = s->num_heads, D = s->head_dim;
-  const int groups = path == 2 ? s->num_kv_heads / irb::tma_head_group(s->num_kv_heads) : 0;
+  const int groups = path == 2 ? s->num_kv_heads / head_group(s, fmt) : 0;
   const bool hdr = path == 2 && static_cast<size_t>(groups) * 8 <= kCtrBytes;
   p->dyn = (s->flags & IR_DECODE_DYNAMIC_TAIL) && hdr;
   p->inl = (s->flags & IR_DECODE_INLINE_MERGE) && hdr &&
@@ -293,14 +330,17 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
                 const int32_t* context_lens, const ir_decode_shape* s,
                 void* workspace, size_t workspace_bytes, int32_t* err,
                 cudaStream_t stream, const float* rope_cos = nullptr,
-                const float* rope_sin = nullptr, int64_t rope_stride = 0) {
+                const float* rope_sin = nullptr, int64_t rope_stride = 0, int fmt = 0,
+                const float* k_scale = nullptr, const float* v_scale = nullptr) {
   Plan plan;
-  int rc = make_plan(s, &plan);
+  int rc = make_plan(s, &plan, fmt);
   if (rc) return rc;
   if (s->batch == 0) return IR_OK;
   if (!q || !k_pool || !v_pool || !context_lens ||
       (s->max_blocks > 0 && !block_tables))
     return fail(IR_ERR_INVALID_ARG, "null input pointer");
+  if (fmt && (!k_scale || !v_scale || !aligned(k_pool, 16) || !aligned(v_pool, 16)))
+    return fail(IR_ERR_INVALID_ARG, "8-bit pools need scales and 16-byte alignment");
   if (mode == Mode::kLse ? (!lse_o || !lse_out) : !out)
     return fail(IR_ERR_INVALID_ARG, "null output pointer");
   if (mode == Mode::kWrite && (!k_new || !v_new || !slot_mapping))
@@ -335,7 +375,7 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
       // the generic path may want a different CTA count; never exceed the
       // count the workspace was sized for
       int G = 1;
-      ctas_per_group(1, s, &G);
+      ctas_per_group(1, s, &G, fmt);
       plan.G = G > plan.G ? plan.G : G;
     }
   }
@@ -381,9 +421,19 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
   a.rope_sin = rope_sin;
   a.rope_stride = rope_stride;
   a.err = err;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
 
   int e;
-  if (plan.path == 2) {
+  if (plan.path == 2 && fmt) {
+    CUtensorMap tmk, tmv;
+    const int rows = s->block_size == 8 ? 8 : 16;
+    const int hg = head_group(s, fmt);
+    if (!make_pool_map_q8(&tmk, k_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg) ||
+        !make_pool_map_q8(&tmv, v_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg))
+      return fail(IR_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    e = irb::launch_decode_q8(tmk, tmv, a, s->dtype, fmt, stream);
+  } else if (plan.path == 2) {
     CUtensorMap tmk, tmv;
     const int rows = s->block_size == 8 ? 8 : 16;
     const int hg = irb::tma_head_group(s->num_kv_heads);
@@ -408,7 +458,7 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
     }
     e = irb::launch_decode_tma(tmk, tmv, a, s->dtype, one_box, stall, stream);
   } else {
-    e = irb::launch_decode_generic(a, s->dtype, stream);
+    e = irb::launch_decode_generic(a, s->dtype, fmt, stream);
   }
   if (e) return cuda_status(e, "decode kernel launch");
   e = irb::launch_split_merge(a, s->dtype, stream);
@@ -570,6 +620,26 @@ int noalloc_scratch(void** out) {
   g_noalloc_ptr[dev] = {ctx != 0 ? ctx : current_context_id(), p};
   *out = p;
   return IR_OK;
+}
+
+// Sizes that the 8-bit cache's row calls share.
+int check_q8_rows(int64_t n, int hkv, int d, int bs, int64_t num_slots, int dtype, int fmt) {
+  if (elem_bytes(dtype) == 0) return fail(IR_ERR_INVALID_ARG, "bad dtype");
+  if (!kv_format_ok(fmt)) return fail(IR_ERR_INVALID_ARG, "unknown kv_format");
+  if (n < 0 || hkv <= 0 || bs <= 0 || num_slots < bs || num_slots % bs != 0)
+    return fail(IR_ERR_INVALID_ARG, "bad sizes (num_slots is a positive multiple of block_size)");
+  if (d != 64 && d != 128) return fail(IR_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (hkv > 4096) return fail(IR_ERR_UNSUPPORTED, "more than 4096 kv heads");
+  if (n > INT32_MAX || num_slots / bs >= INT32_MAX ||
+      n * (static_cast<int64_t>(hkv) * d / 16) > (int64_t{1} << 38))
+    return fail(IR_ERR_UNSUPPORTED, "too many rows or blocks");
+  return IR_OK;
+}
+
+// Bytes of one side of the expanded pool of ir_paged_prefill_q8.
+size_t expanded_pool_bytes(const ir_prefill_shape* s) {
+  return align256(static_cast<size_t>(s->num_slots) * s->num_kv_heads * s->head_dim *
+                  elem_bytes(s->dtype));
 }
 
 }  // namespace
@@ -1034,6 +1104,188 @@ int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v
   return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr, 0,
                      nullptr, row_bt, row_ctx, &d, ws + tb + cb, workspace_bytes - tb - cb,
                      err_flag, st);
+}
+
+// ---------------------------------------------------------------- 8-bit cache
+
+size_t ir_cache_write_q8_workspace_size(int64_t num_tokens, int64_t num_slots, int block_size) {
+  if (num_tokens <= 0 || num_slots <= 0 || block_size <= 0) return 0;
+  return irb::cache_write_q8_workspace(num_tokens, num_slots / block_size);
+}
+
+int ir_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                      void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                      const int64_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+                      int head_dim, int block_size, int64_t num_slots, int dtype,
+                      int kv_format, void* workspace, size_t workspace_bytes,
+                      int32_t* err_flag, ir_stream_t stream) {
+  int rc = check_q8_rows(num_tokens, num_kv_heads, head_dim, block_size, num_slots, dtype,
+                         kv_format);
+  if (rc) return rc;
+  if (block_size > 1024) return fail(IR_ERR_UNSUPPORTED, "block_size larger than 1024");
+  if (num_tokens == 0) return IR_OK;
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (k_stride < row || v_stride < row)
+    return fail(IR_ERR_INVALID_ARG, "token stride < Hkv*D");
+  if (!k || !v || !k_pool || !v_pool || !k_scale || !v_scale || !slot_mapping)
+    return fail(IR_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
+    return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
+  const size_t need = irb::cache_write_q8_workspace(num_tokens, num_slots / block_size);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(IR_ERR_WORKSPACE, "workspace smaller than ir_cache_write_q8_workspace_size");
+  if (need && !aligned(workspace, 256))
+    return fail(IR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  int sms = 1;
+  const int e = cached(-1, sm_count_now, 0, &sms);
+  if (e) return cuda_status(e, "device query");
+  return cuda_status(irb::launch_cache_write_q8(k, v, k_stride, v_stride, k_pool, v_pool, k_scale,
+                                                v_scale, slot_mapping, num_tokens, num_kv_heads,
+                                                head_dim, block_size, num_slots, dtype, kv_format,
+                                                workspace, sms, err_flag,
+                                                static_cast<cudaStream_t>(stream)),
+                     "8-bit cache write launch");
+}
+
+int ir_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
+                       int64_t num_rows, int num_kv_heads, int head_dim, int block_size,
+                       int64_t num_slots, int dtype, int kv_format, int32_t* err_flag,
+                       ir_stream_t stream) {
+  int rc = check_q8_rows(num_rows, num_kv_heads, head_dim, block_size, num_slots, dtype,
+                         kv_format);
+  if (rc) return rc;
+  if (num_rows == 0) return IR_OK;
+  if (!out || !pool || !scale || !slots) return fail(IR_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(pool, 16)) return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
+  return cuda_status(irb::launch_cache_gather_q8(out, pool, scale, slots, num_rows, num_kv_heads,
+                                                 head_dim, block_size, num_slots, dtype,
+                                                 kv_format, err_flag,
+                                                 static_cast<cudaStream_t>(stream)),
+                     "8-bit cache gather launch");
+}
+
+size_t ir_paged_decode_q8_workspace_size(const ir_decode_shape* shape, int kv_format) {
+  Plan p;
+  if (!kv_format_ok(kv_format) || make_plan(shape, &p, kv_format)) return 0;
+  return p.bytes;
+}
+
+int ir_paged_decode_q8_plan(const ir_decode_shape* shape, int kv_format, int* path,
+                            int* ctas_per_kv_head) {
+  if (!kv_format_ok(kv_format)) return fail(IR_ERR_INVALID_ARG, "unknown kv_format");
+  Plan p;
+  int rc = make_plan(shape, &p, kv_format);
+  if (rc) return rc;
+  if (path) *path = p.path;
+  if (ctas_per_kv_head) *ctas_per_kv_head = p.G;
+  return IR_OK;
+}
+
+int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                       const float* k_scale, const float* v_scale, int kv_format,
+                       const int32_t* block_tables, const int32_t* context_lens,
+                       const ir_decode_shape* shape, void* workspace, size_t workspace_bytes,
+                       int32_t* err_flag, ir_stream_t stream) {
+  if (!kv_format_ok(kv_format)) return fail(IR_ERR_INVALID_ARG, "unknown kv_format");
+  return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr, 0,
+                     nullptr, block_tables, context_lens, shape, workspace, workspace_bytes,
+                     err_flag, stream, nullptr, nullptr, 0, kv_format, k_scale, v_scale);
+}
+
+size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape) {
+  if (check_prefill_shape(shape)) return 0;
+  return 2 * expanded_pool_bytes(shape) + align256(ir_paged_prefill_workspace_size(shape));
+}
+
+int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                        const float* k_scale, const float* v_scale, int kv_format,
+                        const int32_t* block_tables, const int32_t* context_lens,
+                        const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
+                        size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream) {
+  if (!kv_format_ok(kv_format)) return fail(IR_ERR_INVALID_ARG, "unknown kv_format");
+  int rc = check_prefill_shape(s);
+  if (rc) return rc;
+  if (s->num_seqs == 0 || s->total_q == 0) return IR_OK;
+  if (s->num_slots < s->block_size || s->num_slots % s->block_size != 0)
+    return fail(IR_ERR_INVALID_ARG, "num_slots must be a positive multiple of block_size");
+  if (!out || !q || !k_pool || !v_pool || !k_scale || !v_scale || !context_lens || !q_start ||
+      (s->max_blocks > 0 && !block_tables))
+    return fail(IR_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
+    return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
+  if (!workspace || workspace_bytes < ir_paged_prefill_q8_workspace_size(s))
+    return fail(IR_ERR_WORKSPACE, "workspace smaller than ir_paged_prefill_q8_workspace_size");
+  if (!aligned(workspace, 256))
+    return fail(IR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  const size_t pool = expanded_pool_bytes(s);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int e = irb::launch_expand_blocks(ws, ws + pool, k_pool, v_pool, k_scale, v_scale,
+                                          block_tables, s->bt_stride, context_lens, s->num_seqs,
+                                          s->max_blocks, s->num_slots / s->block_size,
+                                          s->num_kv_heads, s->head_dim, s->block_size, s->dtype,
+                                          kv_format, static_cast<cudaStream_t>(stream));
+  if (e) return cuda_status(e, "8-bit block expansion launch");
+  return ir_paged_prefill(out, q, ws, ws + pool, block_tables, context_lens, q_start, s,
+                          ws + 2 * pool, workspace_bytes - 2 * pool, err_flag, stream);
+}
+
+// ---------------------------------------------------------------- q/k norm + rotation
+
+int ir_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_stride,
+                    int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride,
+                    const void* w_q, const void* w_k, const float* rope_cos,
+                    const float* rope_sin, int64_t rope_stride, float eps, int64_t num_tokens,
+                    int num_heads, int num_kv_heads, int head_dim, int dtype,
+                    ir_stream_t stream) {
+  const int eb = elem_bytes(dtype);
+  if (eb == 0) return fail(IR_ERR_INVALID_ARG, "bad dtype");
+  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0)
+    return fail(IR_ERR_INVALID_ARG, "bad sizes");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(IR_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (num_heads > 4096 || num_kv_heads > 4096)
+    return fail(IR_ERR_UNSUPPORTED, "more than 4096 heads");
+  if (!(eps >= 0.f)) return fail(IR_ERR_INVALID_ARG, "eps must not be negative");
+  if (num_tokens == 0) return IR_OK;
+  const int64_t qrow = static_cast<int64_t>(num_heads) * head_dim;
+  const int64_t krow = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (q_stride < qrow || q_out_stride < qrow || k_stride < krow || k_out_stride < krow ||
+      rope_stride < head_dim)
+    return fail(IR_ERR_INVALID_ARG, "token stride smaller than the row");
+  if (!q || !k || !q_out || !k_out || !rope_cos || !rope_sin)
+    return fail(IR_ERR_INVALID_ARG, "null pointer");
+  if (num_tokens > (int64_t{1} << 34)) return fail(IR_ERR_UNSUPPORTED, "grid too large");
+  irb::NormRopeArgs a{};
+  a.q = q;
+  a.k = k;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.qo_stride = q_out_stride;
+  a.ko_stride = k_out_stride;
+  a.w_q = w_q;
+  a.w_k = w_k;
+  a.cos = rope_cos;
+  a.sin = rope_sin;
+  a.rope_stride = rope_stride;
+  a.n = num_tokens;
+  a.H = num_heads;
+  a.Hkv = num_kv_heads;
+  a.D = head_dim;
+  a.eps = eps;
+  // rows in vectors of 4 elements where every row starts on one
+  const size_t va = 4 * static_cast<size_t>(eb);
+  const int vec = aligned(q, va) && aligned(k, va) && aligned(q_out, va) && aligned(k_out, va) &&
+                  aligned(w_q, va) && aligned(w_k, va) && aligned(rope_cos, 16) &&
+                  aligned(rope_sin, 16) && q_stride % 4 == 0 && k_stride % 4 == 0 &&
+                  q_out_stride % 4 == 0 && k_out_stride % 4 == 0 && rope_stride % 4 == 0;
+  int sms = 1;
+  const int e = cached(-1, sm_count_now, 0, &sms);
+  if (e) return cuda_status(e, "device query");
+  return cuda_status(irb::launch_qk_norm_rope(a, dtype, vec, sms,
+                                              static_cast<cudaStream_t>(stream)),
+                     "q/k norm and rotation launch");
 }
 
 // ---------------------------------------------------------------- peer exchange

@@ -76,6 +76,9 @@ struct DecodeArgs {
   const float* rope_sin;
   int64_t rope_stride;
   int32_t* err;
+  // 8-bit pools: fp32 scales [num_blocks, Hkv] (null: pools of the dtype)
+  const float* k_scale;
+  const float* v_scale;
 };
 
 __device__ __forceinline__ int clamp_ctx(int c, const DecodeArgs& a) {

@@ -10,8 +10,13 @@
 // computes the 16 x group scores with fp32 dot products, updates the
 // per-head online softmax (exp2 with the scale folded into log2 units) and
 // accumulates P.V with each thread owning one head-dim column.
+//
+// Pools of 8-bit codes (C = e4m3_t / int8_t, quant.cuh) go the same way: a
+// chunk holds 16 codes, and its block's scale is multiplied in when the chunk
+// is stored in shared memory as fp32.
 #include "decode_common.cuh"
 #include "kernels.h"
+#include "quant.cuh"
 
 namespace irb {
 
@@ -20,9 +25,11 @@ namespace {
 constexpr int kGenThreads = 128;
 constexpr int kMaxGroup = 16;
 
-template <typename T, int D>
+// T: type of q and out; C: element of the pools (T itself, or a code type).
+template <typename T, int D, typename C = T>
 __global__ void __launch_bounds__(kGenThreads)
     decode_generic_kernel(const DecodeArgs a) {
+  constexpr bool kQ8 = !std::is_same<T, C>::value;
   constexpr int HPT = kGenThreads / D;            // head groups per column
   constexpr int NH = (kMaxGroup + HPT - 1) / HPT;  // heads per thread
   // rows of K padded to D + 4 floats: 16-byte aligned for the vector reads
@@ -44,20 +51,21 @@ __global__ void __launch_bounds__(kGenThreads)
   if (start >= end) return;
 
   const int d = tid % D, hg = tid / D;
-  const T* kpool = reinterpret_cast<const T*>(a.k_pool);
-  const T* vpool = reinterpret_cast<const T*>(a.v_pool);
+  const C* kpool = reinterpret_cast<const C*>(a.k_pool);
+  const C* vpool = reinterpret_cast<const C*>(a.v_pool);
   // K and V rows move in 16-byte chunks: thread tid owns chunks tid,
   // tid + 128, ... of each tile side, and the next tile's chunks are loaded
   // into registers before the current tile is computed, so that the loads
   // overlap the math. Pools that are not 16-byte aligned (the host sends
   // those here too) are read element by element into the same chunks.
-  constexpr int EPC = 16 / static_cast<int>(sizeof(T));  // elements per chunk
+  constexpr int EPC = 16 / static_cast<int>(sizeof(C));  // elements per chunk
   constexpr int CPR = D / EPC;                            // chunks per row
   constexpr int NCH = kTile * CPR;                        // chunks per tile side
   constexpr int CPT = (NCH + kGenThreads - 1) / kGenThreads;
   const bool vec = ((reinterpret_cast<uintptr_t>(kpool) |
                      reinterpret_cast<uintptr_t>(vpool)) & 15) == 0;
   uint4 kr[CPT], vr[CPT];
+  float ksc[CPT], vsc[CPT];  // scales of the chunks' blocks (8-bit pools)
   // the sequence (tile prefix pb, nb tiles) holding a tile
   struct Cursor {
     int b;
@@ -81,6 +89,7 @@ __global__ void __launch_bounds__(kGenThreads)
     for (int k = 0; k < CPT; ++k) {
       kr[k] = make_uint4(0, 0, 0, 0);
       vr[k] = make_uint4(0, 0, 0, 0);
+      if constexpr (kQ8) ksc[k] = vsc[k] = 0.f;
       const int i = tid + k * kGenThreads;
       if (i >= NCH) continue;
       const int r = i / CPR, cc = i % CPR;
@@ -90,12 +99,16 @@ __global__ void __launch_bounds__(kGenThreads)
       if (id >= 0 && id < a.num_blocks) {
         const int64_t row = static_cast<int64_t>(id) * a.bs + pos % a.bs;
         const int64_t off = (row * a.Hkv + kvh) * D + cc * EPC;
+        if constexpr (kQ8) {
+          ksc[k] = a.k_scale[static_cast<int64_t>(id) * a.Hkv + kvh];
+          vsc[k] = a.v_scale[static_cast<int64_t>(id) * a.Hkv + kvh];
+        }
         if (vec) {
           kr[k] = *reinterpret_cast<const uint4*>(kpool + off);
           vr[k] = *reinterpret_cast<const uint4*>(vpool + off);
         } else {
-          T* kt = reinterpret_cast<T*>(&kr[k]);
-          T* vt = reinterpret_cast<T*>(&vr[k]);
+          C* kt = reinterpret_cast<C*>(&kr[k]);
+          C* vt = reinterpret_cast<C*>(&vr[k]);
 #pragma unroll
           for (int e = 0; e < EPC; ++e) {
             kt[e] = kpool[off + e];
@@ -118,6 +131,16 @@ __global__ void __launch_bounds__(kGenThreads)
       const int i = tid + k * kGenThreads;
       if (i >= NCH) continue;
       const int r = i / CPR, cc = i % CPR;
+      if constexpr (kQ8) {
+        const C* kc = reinterpret_cast<const C*>(&kr[k]);
+        const C* vc = reinterpret_cast<const C*>(&vr[k]);
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) {
+          k_s[r][cc * EPC + e] = DT<C>::to_f(kc[e]) * ksc[k];
+          v_s[r][cc * EPC + e] = DT<C>::to_f(vc[e]) * vsc[k];
+        }
+        continue;
+      }
       T* kt = reinterpret_cast<T*>(&kr[k]);
       T* vt = reinterpret_cast<T*>(&vr[k]);
       const int pos = tok0 + r;
@@ -145,8 +168,8 @@ __global__ void __launch_bounds__(kGenThreads)
           const int64_t dst = (sw * a.Hkv + kvh) * D + cc * EPC;
 #pragma unroll
           for (int e = 0; e < EPC; ++e) {
-            const_cast<T*>(kpool)[dst + e] = kt[e];
-            const_cast<T*>(vpool)[dst + e] = vt[e];
+            const_cast<T*>(reinterpret_cast<const T*>(kpool))[dst + e] = kt[e];
+            const_cast<T*>(reinterpret_cast<const T*>(vpool))[dst + e] = vt[e];
           }
         } else if (cc == 0 && sw >= a.num_slots) {
           set_err(a.err, IR_DEVERR_SLOT);
@@ -258,7 +281,8 @@ __global__ void __launch_bounds__(kGenThreads)
         const int n = hg + k * HPT;
         if (n < a.n_rep) {
           const float M = m_s[n], Lsum = l_s[n];
-          const bool empty = (M == -INFINITY);
+          // (a row whose scores are all NaN is not empty: l is NaN)
+          const bool empty = (M == -INFINITY) && (!kQ8 || Lsum == 0.f);
           const float val = empty ? 0.f : acc[k] / Lsum;
           const float lse2 = empty ? -INFINITY : M + log2f(Lsum);
           write_segment_value<T>(a, kvh, g, b, whole, n, d, val, lse2);
@@ -425,41 +449,55 @@ __global__ void lse_merge_kernel(T* out, int64_t out_stride, const float* o_part
   }
 }
 
-template <typename T>
-int launch_generic_t(const DecodeArgs& a, cudaStream_t s) {
+template <typename T, typename C>
+int launch_generic_c(const DecodeArgs& a, cudaStream_t s) {
   dim3 grid(a.Hkv, a.G);
   if (a.D == 128)
-    decode_generic_kernel<T, 128><<<grid, kGenThreads, 0, s>>>(a);
+    decode_generic_kernel<T, 128, C><<<grid, kGenThreads, 0, s>>>(a);
   else
-    decode_generic_kernel<T, 64><<<grid, kGenThreads, 0, s>>>(a);
+    decode_generic_kernel<T, 64, C><<<grid, kGenThreads, 0, s>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T>
-int occupancy_generic_t(int D) {
+int launch_generic_t(const DecodeArgs& a, int fmt, cudaStream_t s) {
+  if (fmt == IR_KV_E4M3) return launch_generic_c<T, e4m3_t>(a, s);
+  if (fmt == IR_KV_INT8) return launch_generic_c<T, int8_t>(a, s);
+  return launch_generic_c<T, T>(a, s);
+}
+
+template <typename T, typename C>
+int occupancy_generic_c(int D) {
   int n = 0;
   cudaError_t e = D == 128 ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                                 &n, decode_generic_kernel<T, 128>, kGenThreads, 0)
+                                 &n, decode_generic_kernel<T, 128, C>, kGenThreads, 0)
                            : cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                                 &n, decode_generic_kernel<T, 64>, kGenThreads, 0);
+                                 &n, decode_generic_kernel<T, 64, C>, kGenThreads, 0);
   return (e == cudaSuccess && n > 0) ? n : 1;
+}
+
+template <typename T>
+int occupancy_generic_t(int D, int fmt) {
+  if (fmt == IR_KV_E4M3) return occupancy_generic_c<T, e4m3_t>(D);
+  if (fmt == IR_KV_INT8) return occupancy_generic_c<T, int8_t>(D);
+  return occupancy_generic_c<T, T>(D);
 }
 
 }  // namespace
 
-int launch_decode_generic(const DecodeArgs& a, int dtype, cudaStream_t s) {
+int launch_decode_generic(const DecodeArgs& a, int dtype, int fmt, cudaStream_t s) {
   switch (dtype) {
-    case IR_DTYPE_F32: return launch_generic_t<float>(a, s);
-    case IR_DTYPE_BF16: return launch_generic_t<__nv_bfloat16>(a, s);
-    default: return launch_generic_t<__half>(a, s);
+    case IR_DTYPE_F32: return launch_generic_t<float>(a, fmt, s);
+    case IR_DTYPE_BF16: return launch_generic_t<__nv_bfloat16>(a, fmt, s);
+    default: return launch_generic_t<__half>(a, fmt, s);
   }
 }
 
-int decode_generic_occupancy(int dtype, int D) {
+int decode_generic_occupancy(int dtype, int D, int fmt) {
   switch (dtype) {
-    case IR_DTYPE_F32: return occupancy_generic_t<float>(D);
-    case IR_DTYPE_BF16: return occupancy_generic_t<__nv_bfloat16>(D);
-    default: return occupancy_generic_t<__half>(D);
+    case IR_DTYPE_F32: return occupancy_generic_t<float>(D, fmt);
+    case IR_DTYPE_BF16: return occupancy_generic_t<__nv_bfloat16>(D, fmt);
+    default: return occupancy_generic_t<__half>(D, fmt);
   }
 }
 

@@ -82,9 +82,55 @@ int launch_decode_tma(const CUtensorMap& tmk, const CUtensorMap& tmv,
                       cudaStream_t stream);
 int decode_tma_occupancy(int dtype, int D, int Hkv, int bs);
 
-// decode_generic.cu: any dtype, D in {64, 128}, group <= 16, any block size
-int launch_decode_generic(const DecodeArgs& a, int dtype, cudaStream_t stream);
-int decode_generic_occupancy(int dtype, int D);
+// decode_generic.cu: any dtype, D in {64, 128}, group <= 16, any block size;
+// fmt: 0 pools of the dtype, IR_KV_* pools of 8-bit codes
+int launch_decode_generic(const DecodeArgs& a, int dtype, int fmt, cudaStream_t stream);
+int decode_generic_occupancy(int dtype, int D, int fmt);
+
+// decode_q8.cu: 8-bit pools, 16-bit q, D in {64, 128}, group <= 16, bs == 8 or
+// bs % 16 == 0. One CTA (per SM) covers q8_head_group(Hkv, group) kv heads; the
+// maps view a pool as (D bytes, slots, Hkv) with boxes {D, min(bs, 16), head
+// group} and a swizzle as wide as the row.
+int q8_head_group(int num_kv_heads, int n_rep);
+int launch_decode_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, const DecodeArgs& a,
+                     int dtype, int fmt, cudaStream_t stream);
+
+// cache_q8.cu: the 8-bit cache. Workspace bytes of a write of n tokens (0: none).
+size_t cache_write_q8_workspace(int64_t n, int64_t num_blocks);
+int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                          void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                          const int64_t* slots, int64_t n, int Hkv, int D, int bs,
+                          int64_t num_slots, int dtype, int fmt, void* ws, int sms, int32_t* err,
+                          cudaStream_t stream);
+int launch_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
+                           int64_t n, int Hkv, int D, int bs, int64_t num_slots, int dtype,
+                           int fmt, int32_t* err, cudaStream_t stream);
+// Every block that a sequence's history covers, as rows of dtype at the same
+// place of the output pools.
+int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
+                         const float* k_scale, const float* v_scale, const int32_t* bt,
+                         int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
+                         int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
+                         cudaStream_t stream);
+
+// qk_norm_rope.cu
+struct NormRopeArgs {
+  const void* q;  // [n, H, D] rows with q_stride
+  const void* k;  // [n, Hkv, D]
+  void* q_out;
+  void* k_out;
+  int64_t q_stride, k_stride, qo_stride, ko_stride;
+  const void* w_q;  // [D] of the dtype, or null (no weight)
+  const void* w_k;
+  const float* cos;  // [n, D] rows with rope_stride
+  const float* sin;
+  int64_t rope_stride;
+  int64_t n;
+  int H, Hkv, D;
+  int hpg;  // heads per lane group (set by the launcher)
+  float eps;
+};
+int launch_qk_norm_rope(const NormRopeArgs& a, int dtype, int vec, int sms, cudaStream_t s);
 
 // merges (decode_generic.cu): the pieces of sequences split across CTAs
 // (programmatic dependent launch behind the decode kernel), and partials of

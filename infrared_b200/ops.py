@@ -26,6 +26,12 @@ _DTYPES = {
     torch.float16: _lib.IR_DTYPE_F16,
 }
 
+# element types of 8-bit pools
+_KV_FORMATS = {
+    torch.float8_e4m3fn: _lib.IR_KV_E4M3,
+    torch.int8: _lib.IR_KV_INT8,
+}
+
 
 class DeviceError(RuntimeError):
     """Errors a kernel recorded on the device (see ``IR_DEVERR_*``)."""
@@ -755,3 +761,256 @@ def derive_varlen_metadata(gather_slots: torch.Tensor, mask: torch.Tensor, block
         nseq.data_ptr(), scratch.data_ptr(), error_flag(dev).data_ptr(), _stream(dev)))
     s = int(nseq.item())
     return bt[:s], ctx[:s], q_start[:s + 1]
+
+
+# --- 8-bit K/V cache ----------------------------------------------------------
+
+
+def kv_format(dtype: torch.dtype) -> int:
+    """``IR_KV_*`` of an 8-bit pool's dtype."""
+    try:
+        return _KV_FORMATS[dtype]
+    except KeyError:
+        raise _lib.UnsupportedShape(
+            _lib.IR_ERR_UNSUPPORTED, f"8-bit pools are float8_e4m3fn or int8, not {dtype}")
+
+
+def _row_stride(t: torch.Tensor, row: int) -> int:
+    """Stride between t's rows of ``row`` elements (one row or none: any stride
+    that the tensor reports stands for nothing, so the row itself)."""
+    return t.stride(0) if t.shape[0] > 1 else row
+
+
+def _check_pool_q8(pool: torch.Tensor, scale: torch.Tensor, block_size: int, name: str) -> int:
+    """Checks one side of an 8-bit cache; its format."""
+    fmt = kv_format(pool.dtype)
+    _check_pool(pool, name)
+    if block_size <= 0 or pool.shape[0] % block_size:
+        raise ValueError(f"{name} must hold whole blocks of block_size rows")
+    if scale.dtype != torch.float32 or not scale.is_contiguous() or \
+            tuple(scale.shape) != (pool.shape[0] // block_size, pool.shape[1]):
+        raise ValueError(f"the scale of {name} must be contiguous fp32 [num_blocks, Hkv]")
+    if scale.device != pool.device:
+        raise ValueError("all tensors must be on the same device")
+    return fmt
+
+
+def _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size) -> int:
+    fmt = _check_pool_q8(k_pool, k_scale, block_size, "k_pool")
+    if _check_pool_q8(v_pool, v_scale, block_size, "v_pool") != fmt or \
+            v_pool.shape != k_pool.shape or v_pool.device != k_pool.device:
+        raise ValueError("k_pool and v_pool differ")
+    return fmt
+
+
+@_on_tensor_device
+def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
+                   v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                   slot_mapping: torch.Tensor, block_size: int) -> None:
+    """Quantise ``k, v [N, Hkv, D]`` into one layer's 8-bit pools at ``slot_mapping``.
+
+    The pools are ``[num_slots, Hkv, D]`` codes (``float8_e4m3fn`` or
+    ``int8``), the scales fp32 ``[num_blocks, Hkv]``: a row's value is
+    code * scale. Every touched (block, head) keeps the larger of its scale and
+    the smallest power of two that holds the new rows; codes of other rows are
+    rescaled when it grows; a write that holds a block's first row begins the
+    block afresh (``ir_cache_write_q8``). Negative slots skip their rows.
+    """
+    dev = _dev_index(k_pool)
+    fmt = _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size)
+    n = slot_mapping.numel()
+    hkv, d = k_pool.shape[1], k_pool.shape[2]
+    k = k.reshape(n, hkv, d)
+    v = v.reshape(n, hkv, d)
+    for t, nm in ((k, "k"), (v, "v")):
+        if t.dtype != k.dtype or t.device != k_pool.device:
+            raise ValueError(f"{nm} must match k's dtype and the pool's device")
+        if n and (t.stride(2) != 1 or t.stride(1) != d):
+            raise ValueError(f"{nm} rows must be [Hkv, D] contiguous")
+    slots = slot_mapping.reshape(-1)
+    if slots.dtype != torch.int64 or not slots.is_contiguous() or slots.device != k_pool.device:
+        raise ValueError("slot_mapping must be a contiguous int64 tensor on the pool's device")
+    code = dtype_code(k.dtype)
+    if n == 0:
+        return
+    lib = _lib.load()
+    nbytes = lib.ir_cache_write_q8_workspace_size(n, k_pool.shape[0], block_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=k_pool.device) if nbytes else None
+    check(lib.ir_cache_write_q8(
+        k.data_ptr(), v.data_ptr(), _row_stride(k, hkv * d), _row_stride(v, hkv * d),
+        k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), n, hkv, d,
+        block_size, k_pool.shape[0], code, fmt, _ptr(ws), nbytes, error_flag(dev).data_ptr(),
+        _stream(dev)))
+
+
+@_on_tensor_device
+def cache_gather_q8(pool: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor,
+                    block_size: int, dtype: torch.dtype) -> torch.Tensor:
+    """Rows of an 8-bit pool as values of ``dtype``: a 1-D or 2-D int64 slot tensor
+    -> ``[*slots.shape, Hkv, D]`` (finite values beyond the dtype saturate)."""
+    dev = _dev_index(pool)
+    fmt = _check_pool_q8(pool, scale, block_size, "pool")
+    flat = slots.reshape(-1)
+    if flat.dtype != torch.int64 or flat.device != pool.device:
+        raise ValueError("slots must be int64 on the pool's device")
+    flat = flat.contiguous()
+    code = dtype_code(dtype)
+    out = torch.empty((*slots.shape, pool.shape[1], pool.shape[2]), dtype=dtype,
+                      device=pool.device)
+    if flat.numel():
+        check(_lib.load().ir_cache_gather_q8(
+            out.data_ptr(), pool.data_ptr(), scale.data_ptr(), flat.data_ptr(), flat.numel(),
+            pool.shape[1], pool.shape[2], block_size, pool.shape[0], code, fmt,
+            error_flag(dev).data_ptr(), _stream(dev)))
+    return out
+
+
+def _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, block_size):
+    _dev_index(q)
+    fmt = _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size)
+    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError("q must be [rows, H, D] with [H, D] contiguous rows")
+    if k_pool.shape[2] != q.shape[2]:
+        raise ValueError("head_dim of q and pools differ")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or \
+            (block_tables.numel() and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [B, max_blocks] with unit column stride")
+    if context_lens.dtype != torch.int32 or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous int32 [B]")
+    for t in (k_pool, block_tables, context_lens):
+        if t.device != q.device:
+            raise ValueError("all tensors must be on the same device")
+    return fmt
+
+
+def _scratch(ws: torch.Tensor | None, nbytes: int, device) -> torch.Tensor:
+    """The caller's workspace, or one of this call alone: it needs no initial
+    state, and PyTorch's allocator orders its reuse on the current stream and
+    inside a graph capture, so calls on other streams and replayed graphs
+    never share it."""
+    if ws is None:
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    if ws.numel() * ws.element_size() < nbytes or ws.device != device or not ws.is_contiguous():
+        raise ValueError(f"workspace must be {nbytes} contiguous bytes on q's device")
+    return ws
+
+
+def _check_out(out, q):
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
+            out.stride(1) != q.shape[2] or out.device != q.device:
+        raise ValueError("out must be of q's shape, dtype and device with [H, D] contiguous rows")
+
+
+def decode_plan_q8(q, k_pool, block_tables, block_size, scale=1.0):
+    """``(path, ctas_per_kv_head, workspace_bytes)`` of :func:`paged_decode_q8`."""
+    s = _shape(q, k_pool, block_tables, block_size, scale, q.shape[1] * q.shape[2])
+    fmt = kv_format(k_pool.dtype)
+    lib = _lib.load()
+    path, g = _lib.c_int(), _lib.c_int()
+    check(lib.ir_paged_decode_q8_plan(s, fmt, path, g))
+    return path.value, g.value, lib.ir_paged_decode_q8_workspace_size(s, fmt)
+
+
+@_on_tensor_device
+def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                    k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                    context_lens: torch.Tensor, scale: float, block_size: int,
+                    out: torch.Tensor | None = None,
+                    ws: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_decode` over an 8-bit cache (:func:`cache_write_q8`):
+    ``q [B, H, D]`` (any dtype of the framework) -> ``[B, H, D]``."""
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens,
+                           block_size)
+    if block_tables.shape[0] != q.shape[0] or context_lens.numel() != q.shape[0]:
+        raise ValueError("batch sizes of q, block_tables and context_lens differ")
+    _check_out(out, q)
+    dev = _dev_index(q)
+    lib = _lib.load()
+    row = q.shape[1] * q.shape[2]
+    s = _shape(q, k_pool, block_tables, block_size, scale, _row_stride(out, row))
+    s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
+    nbytes = lib.ir_paged_decode_q8_workspace_size(s, fmt)
+    if nbytes == 0:
+        check(lib.ir_paged_decode_q8_plan(s, fmt, None, None))
+    ws = _scratch(ws, nbytes, q.device)
+    check(lib.ir_paged_decode_q8(
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), fmt, block_tables.data_ptr(), context_lens.data_ptr(), s,
+        ws.data_ptr(), ws.numel() * ws.element_size(), error_flag(dev).data_ptr(), _stream(dev)))
+    return out
+
+
+@_on_tensor_device
+def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, q_start: torch.Tensor, scale: float,
+                     block_size: int, out: torch.Tensor | None = None,
+                     ws: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_prefill` over an 8-bit cache (:func:`cache_write_q8`). Its
+    workspace holds one layer's pool in q's dtype (``ir_paged_prefill_q8``)."""
+    fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens,
+                           block_size)
+    if q_start.dtype != torch.int32 or not q_start.is_contiguous() or q_start.device != q.device:
+        raise ValueError("q_start must be a contiguous int32 tensor on q's device")
+    nseq = q_start.numel() - 1
+    if nseq < 0 or block_tables.shape[0] != nseq or context_lens.numel() != nseq:
+        raise ValueError("q_start must have one more entry than block_tables / context_lens")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _check_out(out, q)
+    dev = _dev_index(q)
+    row = q.shape[1] * q.shape[2]
+    s = _prefill_shape(q, k_pool, block_tables, q_start, block_size, scale,
+                       _row_stride(out, row))
+    s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
+    lib = _lib.load()
+    nbytes = lib.ir_paged_prefill_q8_workspace_size(s)
+    ws = _scratch(ws, nbytes, q.device)
+    check(lib.ir_paged_prefill_q8(
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), fmt, block_tables.data_ptr(), context_lens.data_ptr(),
+        q_start.data_ptr(), s, ws.data_ptr(), ws.numel() * ws.element_size(),
+        error_flag(dev).data_ptr(), _stream(dev)))
+    return out
+
+
+# --- q/k norm with rotation ---------------------------------------------------
+
+
+@_on_tensor_device
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, w_q: torch.Tensor | None,
+                 w_k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, eps: float,
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """RMS norm of every head of ``q [N, H, D]`` and ``k [N, Hkv, D]`` over D, times
+    ``w_q`` / ``w_k [D]`` (None: one), and the rotary embedding with fp32
+    ``cos`` / ``sin [N, D]``, in one kernel; returns ``(q_out, k_out)``.
+
+    Computed in fp32 and rounded once. ``q`` and ``k`` may be row views of one
+    QKV projection; ``q_out`` / ``k_out`` may be ``q`` / ``k`` themselves.
+    """
+    dev = _dev_index(q)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("q must be [N, H, D] and k [N, Hkv, D]")
+    n, h, d = q.shape
+    hkv = k.shape[1]
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    for name, t, like in (("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)):
+        if t.dtype != q.dtype or t.device != q.device or t.shape != like.shape:
+            raise ValueError(f"{name} must match q's dtype and device and its input's shape")
+        if t.stride(2) != 1 or t.stride(1) != d:
+            raise ValueError(f"{name} rows must be [heads, D] contiguous")
+    for name, t in (("w_q", w_q), ("w_k", w_k)):
+        if t is not None and (t.numel() != d or t.dtype != q.dtype or not t.is_contiguous()
+                              or t.device != q.device):
+            raise ValueError(f"{name} must be a contiguous [D] weight of q's dtype")
+    cos, sin = _rope_rows(cos, sin, n, d, q.device)
+    check(_lib.load().ir_qk_norm_rope(
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), _row_stride(q, h * d),
+        _row_stride(k, hkv * d), _row_stride(q_out, h * d), _row_stride(k_out, hkv * d),
+        _ptr(w_q), _ptr(w_k), cos.data_ptr(), sin.data_ptr(), _row_stride(cos, d), float(eps), n, h, hkv, d, dtype_code(q.dtype), _stream(dev)))
+    return q_out, k_out

@@ -1,0 +1,564 @@
+"""8-bit K/V cache and its attention on the GPU against the fp64 restatement.
+
+Codes, scales and rows read back are exact (a power-of-two scale divides
+exactly, so a code has one rounding, the same everywhere). Attention is held
+to bounds counted from the roundings of each kernel, row by row:
+
+* a score is a sum of D products accumulated in fp32: at most D steps of
+  2^-23 (a tensor core may truncate) of sum_d |q_d k_d|, plus a few roundings
+  of the score itself (scaling, exponent's argument);
+* a relative error e of every weight moves the output by at most 2 e times
+  sum_j p_j |v_j| (numerator and denominator);
+* weights rounded to fp16 (16-bit q): 2^-11 each, 2^-24 of 2^-7 below the
+  normal range; sums over T tokens in fp32: T steps of 2^-23 at most;
+* the exponential instruction: 2^-22;
+* the output rounding: half a unit of the output type.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import infrared_b200 as irb
+from infrared_b200 import ops
+from infrared_b200 import workloads as wl
+from oracle import kv_q8_np as q8
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+
+DEV = "cuda"
+FMT = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+@pytest.fixture(autouse=True)
+def _clean_errors():
+    ops.error_flag().zero_()
+    yield
+    ops.check_device_errors()
+
+
+def dev(x, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(x)).to(DEV)
+    return t if dtype is None else t.to(dtype)
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def codes_to(codes, fmt):
+    return dev(codes.astype(np.float32)).to(FMT[fmt])
+
+
+def make_pool(rng, nb, bs, hkv, d, fmt, spread=1.0):
+    """Codes and scales of a random pool, one (block, head) quantised at a time."""
+    codes, scale = np.zeros((nb * bs, hkv, d)), np.zeros((nb, hkv))
+    rows = rng.normal(size=(nb * bs, hkv, d)) * spread * \
+        np.exp(rng.normal(size=(nb, 1, hkv, 1)) * np.ones((nb, bs, hkv, 1))).reshape(nb * bs, hkv, 1)
+    q8.write(codes, scale, rows, range(nb * bs), bs, fmt)
+    return codes, scale
+
+
+# ---------------------------------------------------------------- cache write
+
+
+def _write_case(rng, n, hkv, d, bs, nb, fmt, dtype, order="mixed"):
+    codes, scale = make_pool(rng, nb, bs, hkv, d, fmt, 0.2)
+    rows = [dev(rng.normal(size=(n, hkv, d)) * np.exp(rng.normal(size=(n, hkv, 1)))).to(dtype)
+            for _ in range(2)]
+    slots = rng.permutation(nb * bs)[:n]
+    if order == "runs":
+        slots = np.sort(slots)
+    return codes, scale, rows, slots
+
+
+def _check_write(codes, scale, rows, slots, bs, fmt, neg=()):
+    slots = np.array(slots, np.int64)
+    slots[list(neg)] = -1
+    kp, vp = codes_to(codes, fmt), codes_to(codes, fmt)
+    ks, vs = dev(scale.astype(np.float32)), dev(scale.astype(np.float32))
+    irb.cache_write_q8(rows[0], rows[1], kp, vp, ks, vs, dev(slots), bs)
+    for pool, sc, x in ((kp, ks, rows[0]), (vp, vs, rows[1])):
+        want, ws = codes.copy(), scale.copy()
+        q8.write(want, ws, host(x), slots, bs, fmt)
+        np.testing.assert_array_equal(host(sc), ws)
+        np.testing.assert_array_equal(host(pool), want)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,hkv,d,bs,nb", [
+    (1, 1, 64, 16, 3), (1, 4, 128, 1, 5), (5, 2, 64, 5, 4), (64, 4, 128, 16, 80),
+    (333, 2, 64, 16, 40), (100, 8, 128, 8, 60), (70, 3, 128, 64, 4), (40, 1, 128, 1024, 1),
+])
+def test_write(n, hkv, d, bs, nb, dtype, fmt):
+    rng = np.random.default_rng(n * 7 + d + bs)
+    _check_write(*_write_case(rng, n, hkv, d, bs, nb, fmt, dtype), bs, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+@pytest.mark.parametrize("n,hkv,d,bs,nb", [
+    (1024, 2, 64, 16, 100), (1025, 2, 64, 16, 100), (3000, 1, 128, 16, 200), (2500, 2, 64, 12, 250),
+    (1500, 1, 64, 1, 1600), (1030, 2, 64, 256, 5),
+])
+def test_write_many_tokens(n, hkv, d, bs, nb, order, fmt):
+    rng = np.random.default_rng(n + bs)
+    case = _write_case(rng, n, hkv, d, bs, nb, fmt, torch.bfloat16, order)
+    _check_write(*case, bs, fmt, neg=(0, 17, n - 1))
+
+
+@pytest.mark.parametrize("n", [40, 1100])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_write_same_slot_twice_keeps_the_last_row(fmt, n):
+    rng = np.random.default_rng(n)
+    codes, scale, rows, slots = _write_case(rng, n, 2, 64, 16, 80, fmt, torch.float16)
+    slots[n // 2:] = slots[:n - n // 2]
+    _check_write(codes, scale, rows, slots, 16, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_write_step_by_step_equals_the_restatement(fmt):
+    """A prompt, then tokens that raise the tail block's scale, on row views of
+    one projection output."""
+    rng = np.random.default_rng(8)
+    hkv, d, bs, nb = 2, 64, 16, 4
+    codes, scale = make_pool(rng, nb, bs, hkv, d, fmt)
+    kp, vp = codes_to(codes, fmt), codes_to(codes, fmt)
+    ks, vs = dev(scale.astype(np.float32)), dev(scale.astype(np.float32))
+    wk, wv, sk, sv = codes.copy(), codes.copy(), scale.copy(), scale.copy()
+    table, pos = [2, 0, 3], 0
+    for n, size in ((19, 1.0), (1, 0.5), (1, 3.0), (1, 40.0), (9, 0.1), (3, 9.0), (1, 1e-3)):
+        x = dev(rng.normal(size=(n, 3 * hkv * d)) * size).to(torch.bfloat16)
+        k, v = x[:, hkv * d:2 * hkv * d], x[:, 2 * hkv * d:]
+        p = np.arange(pos, pos + n)
+        slots = np.array(table)[p // bs] * bs + p % bs
+        irb.cache_write_q8(k.view(n, hkv, d), v.view(n, hkv, d), kp, vp, ks, vs, dev(slots), bs)
+        q8.write(wk, sk, host(k).reshape(n, hkv, d), slots, bs, fmt)
+        q8.write(wv, sv, host(v).reshape(n, hkv, d), slots, bs, fmt)
+        pos += n
+    for got, want in ((kp, wk), (vp, wv), (ks, sk), (vs, sv)):
+        np.testing.assert_array_equal(host(got), want)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_write_unaligned_rows(offset):
+    rng = np.random.default_rng(5)
+    n, hkv, d, bs = 20, 2, 64, 16
+    codes, scale, _, slots = _write_case(rng, n, hkv, d, bs, 4, "e4m3", torch.bfloat16)
+    rows = []
+    for _ in range(2):
+        flat = dev(rng.normal(size=n * (hkv * d + 5) + 8)).to(torch.bfloat16)
+        rows.append(flat[offset:].as_strided((n, hkv, d), (hkv * d + 5, d, 1),
+                                             flat.storage_offset() + offset))
+    _check_write(codes, scale, rows, slots, bs, "e4m3")
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_write_values_that_are_not_finite(fmt):
+    rng = np.random.default_rng(6)
+    codes, scale, rows, _ = _write_case(rng, 6, 2, 64, 16, 3, fmt, torch.float32)
+    rows[0][1, 0, 5] = float("nan")
+    rows[0][2, 1, 7] = float("inf")
+    rows[1][3, 0, 0] = float("-inf")
+    rows[1][4] = 0.0
+    rows[1][5] = 1e-42
+    slots = np.array([16, 17, 18, 35, 36, 37])
+    _check_write(codes, scale, rows, slots, 16, fmt)
+    # a NaN scale of an int8 block stays until the block is begun again
+    scale[2, 0] = np.nan if fmt == "int8" else scale[2, 0]
+    _check_write(codes, scale, rows, np.array([33, 34, 35, 36, 37, 38]), 16, fmt)
+    _check_write(codes, scale, rows, np.array([33, 34, 32, 36, 37, 38]), 16, fmt)
+
+
+@pytest.mark.parametrize("n", [5, 1200])
+def test_write_slot_outside_the_pool_is_flagged_and_skipped(n):
+    rng = np.random.default_rng(9)
+    codes, scale, rows, slots = _write_case(rng, n, 1, 64, 16, 90, "e4m3", torch.bfloat16)
+    bad = slots.copy()
+    bad[3] = 90 * 16
+    kp, vp = codes_to(codes, "e4m3"), codes_to(codes, "e4m3")
+    ks, vs = dev(scale.astype(np.float32)), dev(scale.astype(np.float32))
+    irb.cache_write_q8(rows[0], rows[1], kp, vp, ks, vs, dev(bad.astype(np.int64)), 16)
+    with pytest.raises(irb.DeviceError, match="SLOT"):
+        irb.check_device_errors()
+    want, ws = codes.copy(), scale.copy()
+    bad[3] = -1
+    q8.write(want, ws, host(rows[0]), bad, 16, "e4m3")
+    np.testing.assert_array_equal(host(kp), want)
+    np.testing.assert_array_equal(host(ks), ws)
+
+
+# ---------------------------------------------------------------- gather
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gather(fmt, dtype):
+    rng = np.random.default_rng(1)
+    for hkv, d, bs, nb in ((2, 64, 16, 20), (4, 128, 5, 9), (1, 64, 1, 7)):
+        codes, scale = make_pool(rng, nb, bs, hkv, d, fmt)
+        scale[0] = 2.0 ** 12   # values beyond fp16 saturate
+        slots = rng.integers(0, nb * bs, size=(3, 11))
+        got = irb.cache_gather_q8(codes_to(codes, fmt), dev(scale.astype(np.float32)), dev(slots),
+                                  bs, dtype)
+        assert got.shape == (3, 11, hkv, d) and got.dtype == dtype
+        top = torch.finfo(dtype).max
+        want = torch.from_numpy(q8.values(codes, scale, bs)[slots]).clamp(-top, top).to(dtype)
+        assert torch.equal(got.cpu(), want)
+        assert irb.cache_gather_q8(codes_to(codes, fmt), dev(scale.astype(np.float32)),
+                                   dev(slots[:0]), bs, dtype).numel() == 0
+
+
+def test_gather_bad_slots_give_zero_rows():
+    rng = np.random.default_rng(1)
+    codes, scale = make_pool(rng, 3, 16, 2, 64, "e4m3")
+    got = irb.cache_gather_q8(codes_to(codes, "e4m3"), dev(scale.astype(np.float32)),
+                              dev(np.array([-1, 5, 48])), 16, torch.float32)
+    with pytest.raises(irb.DeviceError, match="SLOT"):
+        irb.check_device_errors()
+    assert not got[0].any() and not got[2].any()
+    np.testing.assert_array_equal(host(got[1]), q8.values(codes, scale, 16)[5])
+
+
+# ---------------------------------------------------------------- attention
+
+
+def attend_tolerance(out, weighted, size, n, d, dtype, low_p):
+    """The bound of the module's header for one row."""
+    e = (d + 8) * 2.0 ** -23 * size + 2.0 ** -21 + n * 2.0 ** -23
+    if low_p:
+        e = e + 2.0 ** -11
+    tail = n * 2.0 ** -31 * np.abs(weighted).max() if low_p else 0.0
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    return 2 * e[:, None] * weighted + tail + half * np.abs(out) * (1 + 2.0 ** -6) + tiny
+
+
+def check_decode(w, fmt, dtype, path=None, seed=0, q=None, spread=1.0, out=None):
+    rng = np.random.default_rng(seed)
+    kc, ks = make_pool(rng, w.num_blocks, w.block_size, w.num_kv_heads, w.head_dim, fmt, spread)
+    vc, vs = make_pool(rng, w.num_blocks, w.block_size, w.num_kv_heads, w.head_dim, fmt)
+    if q is None:
+        q = dev(rng.normal(size=(w.batch, w.num_heads, w.head_dim))).to(dtype)
+    bt, ctx = dev(w.block_tables), dev(w.context_lens)
+    kp, vp = codes_to(kc, fmt), codes_to(vc, fmt)
+    if path is not None:
+        assert ops.decode_plan_q8(q, kp, bt, w.block_size)[0] == path
+    got = irb.paged_decode_q8(q, kp, vp, dev(ks.astype(np.float32)), dev(vs.astype(np.float32)),
+                              bt, ctx, w.scale, w.block_size, out=out)
+    kv, vv = q8.values(kc, ks, w.block_size), q8.values(vc, vs, w.block_size)
+    g, qh = host(got), host(q)
+    for i in range(w.batch):
+        n = int(w.context_lens[i])
+        want, weighted, size = q8.attend(
+            qh[i], q8.history(kv, w.block_tables[i], n, w.block_size),
+            q8.history(vv, w.block_tables[i], n, w.block_size), w.scale)
+        tol = attend_tolerance(want, weighted, size, n, w.head_dim, dtype, path == 2)
+        err = np.abs(g[i] - want)
+        assert (err <= tol).all(), (i, n, float((err - tol).max()), float(err.max()))
+    return got
+
+
+GEOM = [  # H, Hkv, D, block size, path of 16-bit q
+    (28, 4, 128, 16, 2), (14, 2, 64, 16, 2), (8, 8, 128, 32, 2), (16, 8, 64, 48, 2),
+    (8, 1, 128, 16, 2), (3, 3, 64, 16, 2), (11, 1, 128, 16, 2), (32, 2, 64, 16, 2),
+    (44, 4, 128, 64, 2), (28, 4, 128, 8, 2), (14, 2, 64, 8, 2), (12, 1, 64, 8, 2),
+    (128, 8, 128, 16, 2), (6, 6, 128, 8, 2), (28, 4, 128, 12, 1), (14, 2, 64, 5, 1),
+    (4, 2, 64, 1, 1),
+]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("geom", GEOM)
+def test_decode_bf16(geom, fmt):
+    h, hkv, d, bs, path = geom
+    w = wl.custom(h + bs, 7, h, hkv, d, bs, 0, 150)
+    w.context_lens[:4] = [0, 1, 150, 17]
+    check_decode(w, fmt, torch.bfloat16, path)
+
+
+def _with_lengths(seed, lens, h, hkv, d, bs):
+    """A workload of exactly these context lengths."""
+    rng = np.random.default_rng(seed)
+    ctx = np.array(lens, np.int32)
+    nb = int(((ctx.astype(np.int64) + bs - 1) // bs).sum()) + 3
+    bt, _ = wl.assign_blocks(rng, ctx, bs, nb)
+    return wl.Workload("lens", len(lens), h, hkv, d, bs, nb, "bfloat16", d ** -0.5, 1.0, ctx, bt,
+                       wl.tail_slots(bt, ctx, bs))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("geom", [GEOM[0], GEOM[1], GEOM[6], GEOM[9], GEOM[15]])
+def test_decode_other_types(geom, dtype, fmt):
+    h, hkv, d, bs, path = geom
+    w = _with_lengths(3, [1, 16, 0, 33, 129, 8], h, hkv, d, bs)
+    check_decode(w, fmt, dtype, path if dtype == torch.float16 else 1, spread=3.0)
+
+
+@pytest.mark.parametrize("lens", [
+    [1], [0], [0, 0, 0], [5000], [2047, 2048, 2049], [15, 16, 17, 31, 32, 33] * 4,
+    [1] * 300, [7, 0] * 150, [1500, 3, 0, 800] * 5,
+])
+def test_decode_lengths(lens):
+    """One sequence over all SMs, many short ones in one CTA, empty rows between."""
+    h, hkv, d = (28, 4, 128) if sum(lens) < 3000 else (8, 2, 64)
+    check_decode(_with_lengths(len(lens), lens, h, hkv, d, 16), "e4m3", torch.bfloat16, 2)
+
+
+@pytest.mark.parametrize("hkv", [1, 2, 4, 8])
+@pytest.mark.parametrize("rep", [1, 8, 9, 16])
+def test_decode_head_groups(hkv, rep):
+    w = _with_lengths(hkv, [300, 1, 77, 200], hkv * rep, hkv, 128, 16)
+    check_decode(w, "int8", torch.bfloat16, 2)
+
+
+def test_decode_strided_and_unaligned_rows():
+    w = _with_lengths(2, [40, 100, 3], 14, 2, 64, 16)
+    rng = np.random.default_rng(4)
+    flat = dev(rng.normal(size=3 * 2000 + 16)).to(torch.bfloat16)
+    for off, stride in ((0, 2000), (1, 901), (4, 1000), (0, 904)):
+        q = flat[off:].as_strided((3, 14, 64), (stride, 64, 1), off)
+        check_decode(w, "e4m3", torch.bfloat16, 2, q=q)
+    out = torch.full((3, 14 * 64 + 8), 9.0, dtype=torch.bfloat16, device=DEV)
+    check_decode(w, "e4m3", torch.bfloat16, 2, out=out[:, :14 * 64].view(3, 14, 64))
+    assert (out[:, 14 * 64:] == 9.0).all()
+    # rows of out that do not start on 16 bytes take the CUDA-core kernel
+    odd = torch.empty(3 * (14 * 64 + 1), dtype=torch.bfloat16, device=DEV)
+    check_decode(w, "e4m3", torch.bfloat16, None, out=odd.as_strided((3, 14, 64), (897, 64, 1)))
+
+
+def test_decode_large_and_small_queries():
+    """q far outside fp16's range, and rows of zeros."""
+    w = _with_lengths(2, [40, 100, 3], 14, 2, 64, 16)
+    rng = np.random.default_rng(4)
+    for size in (1e-30, 1e-8, 30.0):
+        q = dev(rng.normal(size=(3, 14, 64)) * size).to(torch.bfloat16)
+        q[1, 3] = 0.0
+        check_decode(w, "e4m3", torch.bfloat16, 2, q=q)
+    # the same scores from a huge q and a tiny softmax scale
+    w.scale = 1e-25
+    check_decode(w, "int8", torch.bfloat16, 2, q=dev(rng.normal(size=(3, 14, 64)) * 1e24).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("fmt,dtype,bs", [
+    ("e4m3", torch.bfloat16, 16), ("e4m3", torch.bfloat16, 8), ("e4m3", torch.float32, 16),
+    ("int8", torch.bfloat16, 16), ("int8", torch.bfloat16, 8), ("int8", torch.float32, 5)])
+def test_decode_garbage_past_the_context(fmt, dtype, bs):
+    """NaN codes and scales in rows and blocks that no sequence reaches change nothing."""
+    w = _with_lengths(5, [17, 1, 40, 9, 0], 14, 2, 64, bs)
+    rng = np.random.default_rng(2)
+    kc, ks = make_pool(rng, w.num_blocks, bs, 2, 64, fmt)
+    q = dev(rng.normal(size=(5, 14, 64))).to(dtype)
+    used = np.zeros(w.num_blocks * bs, bool)
+    held = np.zeros(w.num_blocks, bool)
+    for i, n in enumerate(w.context_lens):
+        p = np.arange(n)
+        used[w.block_tables[i, p // bs] * bs + p % bs] = True
+        held[w.block_tables[i, p // bs]] = True
+    bt, ctx = dev(w.block_tables), dev(w.context_lens)
+
+    def run(codes, scale):
+        pool, sc = codes_to(codes, fmt), dev(scale.astype(np.float32))
+        return irb.paged_decode_q8(q, pool, pool, sc, sc, bt, ctx, w.scale, bs)
+
+    clean = run(kc, ks)
+    dirty, dsc = kc.copy(), ks.copy()
+    dirty[~used] = np.nan if fmt == "e4m3" else 127
+    dsc[~held] = np.nan
+    assert torch.equal(run(dirty, dsc), clean)
+    assert not clean[4].any()
+
+
+@pytest.mark.parametrize("dtype,bs", [(torch.bfloat16, 16), (torch.float32, 16)])
+def test_decode_nan_in_the_history_reaches_the_row(dtype, bs):
+    w = _with_lengths(5, [17, 1, 300], 14, 2, 64, bs)
+    rng = np.random.default_rng(2)
+    kc, ks = make_pool(rng, w.num_blocks, bs, 2, 64, "e4m3")
+    vc, vs = make_pool(rng, w.num_blocks, bs, 2, 64, "e4m3")
+    q = dev(rng.normal(size=(3, 14, 64))).to(dtype)
+    kc[w.block_tables[1, 0] * bs, 0, 3] = np.nan          # the only key of row 1, head group 0
+    vc[w.block_tables[2, 2] * bs + 1, 1, 9] = np.nan       # one element of V
+    out = irb.paged_decode_q8(q, codes_to(kc, "e4m3"), codes_to(vc, "e4m3"),
+                              dev(ks.astype(np.float32)), dev(vs.astype(np.float32)),
+                              dev(w.block_tables), dev(w.context_lens), w.scale, bs)
+    bad = torch.isnan(out).cpu()
+    want = torch.zeros_like(bad)
+    want[1, :7] = True
+    want[2, 7:, 9] = True
+    assert torch.equal(bad, want)
+
+
+def test_decode_scales_of_any_value():
+    """Scales that are no powers of two, and very different ones in one sequence."""
+    w = _with_lengths(5, [60, 33], 14, 2, 64, 16)
+    rng = np.random.default_rng(2)
+    for fmt, bs in (("int8", 16), ("e4m3", 8)):
+        w = _with_lengths(5, [60, 33], 14, 2, 64, bs)
+        kc, _ = make_pool(rng, w.num_blocks, bs, 2, 64, fmt)
+        ks = np.float32(rng.uniform(0.001, 0.01, size=(w.num_blocks, 2)))
+        vs = np.float32(np.exp(rng.normal(size=(w.num_blocks, 2)) * 8))
+        q = dev(rng.normal(size=(2, 14, 64))).to(torch.float16)
+        got = host(irb.paged_decode_q8(q, codes_to(kc, fmt), codes_to(kc, fmt), dev(ks), dev(vs),
+                                       dev(w.block_tables), dev(w.context_lens), w.scale, bs))
+        kv, vv = q8.values(kc, ks, bs), q8.values(kc, vs, bs)
+        for i, n in enumerate(w.context_lens):
+            want, weighted, size = q8.attend(host(q[i]), q8.history(kv, w.block_tables[i], n, bs),
+                                             q8.history(vv, w.block_tables[i], n, bs), w.scale)
+            tol = attend_tolerance(want, weighted, size, n, 64, torch.float16, True)
+            sure = np.abs(want) < 6e4   # fp16 outputs beyond its range are infinite
+            assert (np.abs(got[i] - want)[sure] <= tol[sure]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_decode_bad_block_ids_are_flagged(dtype):
+    w = _with_lengths(5, [60, 33], 14, 2, 64, 16)
+    rng = np.random.default_rng(2)
+    kc, ks = make_pool(rng, w.num_blocks, 16, 2, 64, "e4m3")
+    bt = w.block_tables.copy()
+    bt[0, 1], bt[0, 2] = -5, w.num_blocks
+    q = dev(rng.normal(size=(2, 14, 64))).to(dtype)
+    sc, pool = dev(ks.astype(np.float32)), codes_to(kc, "e4m3")
+    out = irb.paged_decode_q8(q, pool, pool, sc, sc, dev(bt), dev(w.context_lens), w.scale, 16)
+    with pytest.raises(irb.DeviceError, match="BLOCK_ID"):
+        irb.check_device_errors()
+    good = irb.paged_decode_q8(q, pool, pool, sc, sc, dev(w.block_tables), dev(w.context_lens),
+                               w.scale, 16)
+    # the other sequence is untouched (its pieces may be cut alike: same lengths)
+    assert torch.equal(out[1], good[1])
+
+
+def test_decode_is_deterministic_and_replays():
+    w = _with_lengths(9, [700, 33, 1200, 5], 28, 4, 128, 16)
+    rng = np.random.default_rng(2)
+    kc, ks = make_pool(rng, w.num_blocks, 16, 4, 128, "e4m3")
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    bt, ctx = dev(w.block_tables), dev(w.context_lens)
+    q = dev(rng.normal(size=(4, 28, 128))).to(torch.bfloat16)
+    q2 = dev(rng.normal(size=(4, 28, 128))).to(torch.bfloat16)
+    call = lambda x, out=None: irb.paged_decode_q8(x, pool, pool, sc, sc, bt, ctx, w.scale, 16,  # noqa: E731
+                                                   out=out)
+    first, second = call(q), call(q2)
+    assert torch.equal(call(q), first)
+    out1, out2 = torch.empty_like(q), torch.empty_like(q)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        call(q, out1)
+    with torch.cuda.graph(g2):
+        call(q2, out2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):   # two replayed graphs at once: neither shares scratch
+        g1.replay()
+        with torch.cuda.stream(side):
+            g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out1, first) and torch.equal(out2, second)
+
+
+# ---------------------------------------------------------------- prefill
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("h,hkv,d,bs,spans", [
+    (28, 4, 128, 16, [(0, 130), (17, 1), (50, 40)]), (14, 2, 64, 16, [(3, 5), (0, 1), (0, 200)]),
+    (4, 4, 128, 12, [(20, 30), (0, 7)]), (16, 1, 64, 8, [(9, 33)]),
+])
+def test_prefill(h, hkv, d, bs, spans, dtype, fmt):
+    """Against 64 bits: the tensor-core kernel rounds P to the type (half a unit each)."""
+    rng = np.random.default_rng(h + d)
+    f = wl.prefill_frame("t", 3, [s for s, _ in spans], [n for _, n in spans], h, hkv, d, bs)
+    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    vc, vs = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    q = dev(rng.normal(size=(f.total_q, h, d))).to(dtype)
+    got = host(irb.paged_prefill_q8(q, codes_to(kc, fmt), codes_to(vc, fmt),
+                                    dev(ks.astype(np.float32)), dev(vs.astype(np.float32)),
+                                    dev(f.block_tables), dev(f.context_lens), dev(f.q_start),
+                                    f.scale, bs))
+    kv, vv = q8.values(kc, ks, bs), q8.values(vc, vs, bs)
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for i, (start, n) in enumerate(spans):
+        for r in range(0, n, 1 if n < 50 else 13):
+            t = start + r + 1
+            row = int(f.q_start[i]) + r
+            want, weighted, size = q8.attend(host(q[row]),
+                                             q8.history(kv, f.block_tables[i], t, bs),
+                                             q8.history(vv, f.block_tables[i], t, bs), f.scale)
+            tol = attend_tolerance(want, weighted, size, t, d, dtype, False)
+            # weights rounded to the type; in fp16 a weight below 2^-14 (of a
+            # largest of 1) is rounded to a multiple of 2^-24, so it is off by
+            # up to 2^-25 whatever its size: t of them move sum p v / sum p,
+            # whose denominator is at least 1, by up to t 2^-25 max |v|. Rows of
+            # the expanded pool below fp16's normal range: 2^-25 each likewise
+            tol = tol + 2 * half * weighted
+            if dtype == torch.float16:
+                vmax = np.abs(q8.history(vv, f.block_tables[i], t, bs)).max()
+                tol = tol + t * 2.0 ** -25 * vmax + 2.0 ** -24
+            err = np.abs(got[row] - want)
+            assert (err <= tol).all(), (i, r, float((err - tol).max()))
+
+
+def test_prefill_row_is_the_decode_row():
+    """A prompt's last row and the decode of the same token agree within both bounds."""
+    rng = np.random.default_rng(0)
+    h, hkv, d, bs = 28, 4, 128, 16
+    f = wl.prefill_frame("t", 3, [0], [100], h, hkv, d, bs)
+    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, "e4m3")
+    q = dev(rng.normal(size=(100, h, d))).to(torch.bfloat16)
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    bt, ctx = dev(f.block_tables), dev(f.context_lens)
+    a = irb.paged_prefill_q8(q, pool, pool, sc, sc, bt, ctx, dev(f.q_start), f.scale, bs)[-1]
+    b = irb.paged_decode_q8(q[-1:], pool, pool, sc, sc, bt, ctx, f.scale, bs)[0]
+    _, weighted, _ = q8.attend(host(q[99]), *[q8.history(q8.values(kc, ks, bs), f.block_tables[0],
+                                                         100, bs)] * 2, f.scale)
+    # two output roundings and P in bf16 (2^-8) and fp16 (2^-11)
+    assert (np.abs(host(a) - host(b)) <= (2 * 2.0 ** -8 + 2 * 2.0 ** -8 + 2.0 ** -10) * weighted).all()
+
+
+# ---------------------------------------------------------------- a run of them together
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_prompt_then_decode_steps(fmt):
+    """norm + rotation, quantising write, prefill and decode as one layer of a
+    model would run them, each step against 64 bits on the same codes."""
+    rng = np.random.default_rng(11)
+    h, hkv, d, bs, nb = 14, 2, 64, 16, 12
+    dt = torch.bfloat16
+    kp, vp = (torch.zeros(nb * bs, hkv, d, dtype=torch.int8, device=DEV).view(FMT[fmt])
+              for _ in range(2))
+    ks, vs = (torch.zeros(nb, hkv, device=DEV) for _ in range(2))
+    table = rng.permutation(nb).astype(np.int32)[None]
+    wq, wk = (dev(1 + 0.1 * rng.normal(size=d)).to(dt) for _ in range(2))
+    inv = 1e4 ** (-np.arange(0, d, 2) / d)
+    pos = 0
+    for n in (37, 1, 1, 9, 1):
+        x = dev(rng.normal(size=(n, (h + 2 * hkv) * d))).to(dt)
+        p = np.arange(pos, pos + n)
+        ang = np.concatenate([p[:, None] * inv] * 2, axis=1)
+        cos, sin = dev(np.cos(ang).astype(np.float32)), dev(np.sin(ang).astype(np.float32))
+        q, k = irb.qk_norm_rope(x[:, :h * d].view(n, h, d),
+                                x[:, h * d:(h + hkv) * d].view(n, hkv, d), wq, wk, cos, sin, 1e-6)
+        slots = table[0, p // bs].astype(np.int64) * bs + p % bs
+        irb.cache_write_q8(k, x[:, (h + hkv) * d:].view(n, hkv, d), kp, vp, ks, vs, dev(slots), bs)
+        pos += n
+        ctx = dev(np.array([pos], np.int32))
+        if n == 1:
+            out = irb.paged_decode_q8(q, kp, vp, ks, vs, dev(table), ctx, d ** -0.5, bs)
+        else:
+            out = irb.paged_prefill_q8(q, kp, vp, ks, vs, dev(table), ctx,
+                                       dev(np.array([0, n], np.int32)), d ** -0.5, bs)
+        kv, vv = (q8.values(host(c), host(s), bs) for c, s in ((kp, ks), (vp, vs)))
+        for r in range(n):
+            t = pos - n + r + 1
+            want, weighted, size = q8.attend(host(q[r]), q8.history(kv, table[0], t, bs),
+                                             q8.history(vv, table[0], t, bs), d ** -0.5)
+            tol = attend_tolerance(want, weighted, size, t, d, dt, False) + 2 * 2.0 ** -8 * weighted
+            assert (np.abs(host(out[r]) - want) <= tol).all()
+    # what the cache holds is off by the quantisation alone
+    back = irb.cache_gather_q8(kp, ks, dev(slots), bs, torch.float32)
+    unit = ks.max().item() * (0.5 if fmt == "int8" else 16)
+    assert (back - k.float()).abs().max().item() <= 2 * unit
