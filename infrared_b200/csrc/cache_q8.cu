@@ -2,14 +2,16 @@
 // rows of the compute type (the pool a prefill call attends over).
 //
 // The write. Every (block, kv head) of a pool has one scale, so the rows a
-// call brings to one block are handled together, by one CTA, whatever order
-// they come in: the call's tokens are grouped by block, the group's first
-// finder owns the block, and src[offset] holds the token that brings that
-// row (the last one where a slot appears twice). A warp takes one (K or V,
-// kv head) of the block: it finds the largest magnitude of the new rows,
+// call brings to one block are handled together, whatever order they come in:
+// the call's tokens are grouped by block, and src(offset) is the token that
+// brings that row (the last one where a slot appears twice). A warp takes one
+// (K or V, kv head) of the block: it finds the largest magnitude of the new
+// rows,
 //   s' = max(s, scale_for(amax))          (s counts as 0 when row 0 is new),
 // rescales the codes that stay if s' > s, and writes the new codes. Nothing
-// is summed, so the result does not depend on the order of the tokens.
+// is summed, so the result does not depend on the order of the tokens. The
+// warp loads up to 16 rows at once and keeps them in registers between the
+// two steps, so that rows are read once.
 #include "kernels.h"
 #include "quant.cuh"
 
@@ -19,145 +21,269 @@ namespace {
 
 constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
+// Calls of up to this many tokens find each block's rows by reading all slots.
+constexpr int64_t kScanTokens = 1024;
 constexpr unsigned kAll = 0xffffffffu;
+
+__device__ __forceinline__ void wait_prior_grid() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Launch with programmatic stream serialization: the grid may be set up while
+// the one before it in the stream still runs, and waits for it itself.
+template <typename... P, typename... A>
+int launch_behind(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                  A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+}
 
 struct Q8WriteArgs {
   const void* src[2];  // k, v rows
-  int64_t stride[2];   // elements between tokens
+  int stride[2];       // elements between tokens
   uint8_t* pool[2];
   float* scale[2];  // [num_blocks, Hkv]
   const int64_t* slots;
   int64_t n, num_slots;
   int Hkv, D, bs;
-  int vec;  // rows are read in 4-element vectors
   int32_t* err;
 };
-
-// Four elements of a row as fp32.
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, int vec) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      return *reinterpret_cast<const float4*>(p);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-      return make_float4(a.x, a.y, b.x, b.y);
-    }
-  }
-  return make_float4(DT<T>::to_f(p[0]), DT<T>::to_f(p[1]), DT<T>::to_f(p[2]), DT<T>::to_f(p[3]));
-}
 
 __device__ __forceinline__ bool finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
 }
 
-// One (side, kv head) of block `blk`, by one warp; src[] in shared memory.
-// Lanes cover D in groups of 4 elements, RP = 128 / D rows at a time.
-template <typename T, typename C>
-__device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, const int* src, int side, int h) {
-  constexpr bool kInt = std::is_same<C, int8_t>::value;
-  const int lane = threadIdx.x & 31;
-  const int lpr = a.D / 4;         // lanes per row
-  const int rp = 32 / lpr;         // rows per pass
-  const int sub = lane / lpr, col = (lane % lpr) * 4;
-  const T* in = reinterpret_cast<const T*>(a.src[side]) + static_cast<int64_t>(h) * a.D + col;
-  const int64_t stride = a.stride[side];
-  const int64_t row_bytes = static_cast<int64_t>(a.Hkv) * a.D;
-  uint8_t* dst = a.pool[side] + (blk * a.bs) * row_bytes + static_cast<int64_t>(h) * a.D + col;
+// Larger of two pairs; NaN where either is NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
-  float amax = 0.f;
-  bool bad = false;
-#pragma unroll 4
-  for (int r = sub; r < a.bs; r += rp) {
-    const int t = src[r];
-    if (t < 0) continue;
-    const float4 x = load4<T>(in + t * stride, a.vec);
-    const float v[4] = {x.x, x.y, x.z, x.w};
+// Four elements of a row, as loaded.
+template <typename T> struct Four {
+  uint2 w;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
+      w = *reinterpret_cast<const uint2*>(p);
+    } else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+      w = make_uint2(u[0] | (static_cast<uint32_t>(u[1]) << 16),
+                     u[2] | (static_cast<uint32_t>(u[3]) << 16));
+    }
+  }
+  // Running maximum of the magnitudes, two halves side by side; NaN stays.
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+    return max2<T>(m, max2<T>(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ float4 value() const {
+    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+  static __device__ __forceinline__ float magnitude(uint32_t m) {
+    const float2 t = unpack2<T>(max2<T>(m, m >> 16));
+    return t.x;
+  }
+};
+template <> struct Four<float> {
+  float4 v;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (VEC)
+      v = *reinterpret_cast<const float4*>(p);
+    else
+      v = make_float4(p[0], p[1], p[2], p[3]);
+  }
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+    const uint32_t a = max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu);
+    const uint32_t b = max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu);
+    return max(m, max(a, b));
+  }
+  __device__ __forceinline__ float4 value() const { return v; }
+  static __device__ __forceinline__ float magnitude(uint32_t m) { return __uint_as_float(m); }
+};
+
+// One (side, kv head) of block `blk`, by one warp. Lanes cover D in groups of
+// 4 elements, 128 / D rows at a time, 16 such passes at once. src(r) is called
+// by all lanes of the warp together.
+template <typename T, typename C, bool VEC, typename Src>
+__device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int side, int h) {
+  constexpr bool kInt = std::is_same<C, int8_t>::value;
+  constexpr int kPass = 16;
+  const int lane = threadIdx.x & 31;
+  const bool wide = a.D == 128;  // 32 lanes per row, else 16
+  const int rp = wide ? 1 : 2;   // rows per pass
+  const int sub = wide ? 0 : lane >> 4, col = (wide ? lane : lane & 15) * 4;
+  const T* in = reinterpret_cast<const T*>(a.src[side]) + h * a.D + col;
+  const int stride = a.stride[side];
+  const int row_bytes = a.Hkv * a.D;  // (a block's bytes stay below 2^31)
+  uint8_t* dst = a.pool[side] + blk * a.bs * row_bytes + (h * a.D + col);
+  float* sp = a.scale[side] + blk * a.Hkv + h;
+  const float before = *sp;  // (loaded beside the rows)
+  const bool begun = src(0) >= 0;
+  // the last of the block's new rows stands in for those that are not new,
+  // which leaves the maximum as it is and the loads without a branch
+  int some = -1;
+  for (int base = 0; base < a.bs; base += 32)
+    some = max(some, src(base + lane < a.bs ? base + lane : 0));
+  some = __reduce_max_sync(kAll, some);
+
+  Four<T> x[kPass];
+  uint32_t have = 0;  // bit u: pass u of the rows in registers is a new row
+  auto load = [&](int base) {
+    have = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (finite(v[i])) amax = fmaxf(amax, fabsf(v[i]));
-      else bad = true;
+    for (int u = 0; u < kPass; ++u) {
+      const int r = base + u * rp + sub;
+      int t = src(r < a.bs ? r : 0);
+      if (r < a.bs && t >= 0)
+        have |= 1u << u;
+      else
+        t = some;
+      x[u].template load<VEC>(in + static_cast<int64_t>(t) * stride);
+    }
+  };
+  const int chunk = kPass * rp;
+  uint32_t m = 0;
+  for (int base = 0; base < a.bs; base += chunk) {
+    load(base);
+#pragma unroll
+    for (int u = 0; u < kPass; ++u) m = x[u].top(m);
+  }
+  float amax = Four<T>::magnitude(m);
+  const bool bad = __any_sync(kAll, !finite(amax));
+  if (bad) {  // the largest finite one
+    amax = 0.f;
+    for (int base = 0; base < a.bs; base += chunk) {
+      load(base);
+#pragma unroll
+      for (int u = 0; u < kPass; ++u) {
+        const float4 f = x[u].value();
+        const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (finite(v[i])) amax = fmaxf(amax, fabsf(v[i]));
+      }
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, o));
-  bad = __any_sync(kAll, bad);
 
-  float* sp = a.scale[side] + blk * a.Hkv + h;
-  const bool begun = src[0] >= 0;
-  const float old = begun ? 0.f : *sp;
+  const float old = begun ? 0.f : before;
   const float need = scale_for<C>(amax);
   float now = old > need ? old : need;
   // int8 has no code for a value that is not finite: its block reads as NaN
   // until it is begun again
   if (kInt && (bad || old != old)) now = __uint_as_float(0x7fc00000u);
-  __syncwarp();  // every lane has read the old scale
+  const float inv = pow2_reciprocal(now);
   if (lane == 0) *sp = now;
 
   if (!begun && now != old && now == now) {
     // rescale the codes that stay
-    const float inv = pow2_reciprocal(now);
     const float ratio = inv != 0.f ? old * inv : old / now;
-    for (int r = sub; r < a.bs; r += rp) {
-      if (src[r] >= 0) continue;
+    for (int base = 0; base < a.bs; base += rp) {
+      const int r = base + sub;
+      const int t = src(r < a.bs ? r : 0);
+      if (r >= a.bs || t >= 0) continue;
       uint32_t* p = reinterpret_cast<uint32_t*>(dst + r * row_bytes);
-      float4 x = decode4<C>(*p);
-      x.x *= ratio;
-      x.y *= ratio;
-      x.z *= ratio;
-      x.w *= ratio;
-      *p = encode4<C>(x);
+      float4 f = decode4<C>(*p);
+      f.x *= ratio;
+      f.y *= ratio;
+      f.z *= ratio;
+      f.w *= ratio;
+      *p = encode4<C>(f);
     }
   }
-  const float inv = pow2_reciprocal(now);
-#pragma unroll 4
-  for (int r = sub; r < a.bs; r += rp) {
-    const int t = src[r];
-    if (t < 0) continue;
-    float4 x = load4<T>(in + t * stride, a.vec);
-    float v[4] = {x.x, x.y, x.z, x.w};
+  if (!bad && inv != 0.f) {
+    // every value finite and the scale a power of two: no case to tell apart
+    for (int base = 0; base < a.bs; base += chunk) {
+      if (chunk < a.bs) load(base);
+      uint8_t* row = dst + (base + sub) * row_bytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!finite(v[i])) v[i] = __uint_as_float(0x7fc00000u);
-      else v[i] = inv != 0.f ? v[i] * inv : v[i] / now;
+      for (int u = 0; u < kPass; ++u) {
+        const float4 f = x[u].value();
+        const uint32_t c = encode4<C>(make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv));
+        if ((have >> u) & 1u) *reinterpret_cast<uint32_t*>(row + u * rp * row_bytes) = c;
+      }
     }
+    return;
+  }
+  const float nan = __uint_as_float(0x7fc00000u);
+  for (int base = 0; base < a.bs; base += rp) {
+    const int r = base + sub;
+    const int t = src(r < a.bs ? r : 0);
+    if (r >= a.bs || t < 0) continue;
+    Four<T> one;
+    one.template load<VEC>(in + static_cast<int64_t>(t) * stride);
+    const float4 f = one.value();
     *reinterpret_cast<uint32_t*>(dst + r * row_bytes) =
-        encode4<C>(make_float4(v[0], v[1], v[2], v[3]));
+        encode4<C>(make_float4(finite(f.x) ? f.x / now : nan, finite(f.y) ? f.y / now : nan,
+                               finite(f.z) ? f.z / now : nan, finite(f.w) ? f.w / now : nan));
   }
 }
 
 // One CTA per token (x) and group of kQWarps tasks (y): the CTA of a block's
 // first token owns the block; it finds the others by reading all slots, which
 // takes no launch and no scratch of its own (for calls of few tokens).
-template <typename T, typename C>
+template <typename T, typename C, bool VEC>
 __global__ void __launch_bounds__(kQThreads) write_scan_kernel(const Q8WriteArgs a) {
   extern __shared__ int src[];
-  const int64_t i = blockIdx.x;
-  const int64_t s = a.slots[i];
+  wait_prior_grid();
+  const int i = blockIdx.x;
+  // every slot at once: one round trip
+  const int64_t s = a.slots[i], before = i > 0 ? a.slots[i - 1] : -1;
+  constexpr int kScan = static_cast<int>(kScanTokens) / kQThreads;
+  int64_t all[kScan];
+#pragma unroll
+  for (int u = 0; u < kScan; ++u) {
+    const int j = u * kQThreads + threadIdx.x;
+    all[u] = j < a.n ? a.slots[j] : -1;
+  }
   if (s < 0) return;  // padding row
   if (s >= a.num_slots) {
     if (threadIdx.x == 0 && blockIdx.y == 0) set_err(a.err, IR_DEVERR_SLOT);
     return;
   }
   const int64_t blk = s / a.bs, lo = blk * a.bs;
+  const int64_t near = before - lo;
+  if (near >= 0 && near < a.bs) return;  // its neighbour or an earlier token owns the block
   for (int r = threadIdx.x; r < a.bs; r += kQThreads) src[r] = -1;
   __syncthreads();
   bool earlier = false;
-  for (int64_t j = threadIdx.x; j < a.n; j += kQThreads) {
-    const int64_t off = a.slots[j] - lo;
+#pragma unroll
+  for (int u = 0; u < kScan; ++u) {
+    const int j = u * kQThreads + threadIdx.x;
+    const int64_t off = all[u] - lo;
     if (off < 0 || off >= a.bs) continue;
     earlier = earlier || j < i;
-    atomicMax(&src[off], static_cast<int>(j));
+    atomicMax(&src[off], j);
   }
   if (__syncthreads_or(earlier)) return;
   const int task = blockIdx.y * kQWarps + (threadIdx.x >> 5);
-  if (task < 2 * a.Hkv) quantise_task<T, C>(a, blk, src, task / a.Hkv, task % a.Hkv);
+  if (task < 2 * a.Hkv)
+    quantise_task<T, C, VEC>(a, blk, [&](int r) { return src[r]; }, task / a.Hkv,
+                             task % a.Hkv);
 }
 
 // Larger calls: the tokens' runs (neighbours in one block) are linked per
 // block first. head[blk] is the block's last linked run + 1 (0: none), next[i]
-// the run before it, owners[] the blocks in the order they were found.
+// the run before it, owners[] the first linked run of every block, in the
+// order they were found; count[0] is their number, count[1] that of the other
+// runs (mostly 0: every block's rows are one run, and no list is read).
 struct Q8Links {
   int* count;
   int* head;
@@ -167,58 +293,110 @@ struct Q8Links {
 
 __global__ void link_runs_kernel(const int64_t* slots, int64_t n, int64_t num_slots, int bs,
                                  const Q8Links l, int32_t* err) {
+  wait_prior_grid();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= n) return;
   const int64_t s = slots[i];
+  const int64_t p = i > 0 ? slots[i - 1] : -1;
   if (s < 0) return;
   if (s >= num_slots) {
     set_err(err, IR_DEVERR_SLOT);
     return;
   }
   const int64_t blk = s / bs;
-  if (i > 0) {
-    const int64_t off = slots[i - 1] - blk * bs;
-    if (off >= 0 && off < bs) return;  // not the first of its run
-  }
+  const int64_t off = p - blk * bs;
+  if (off >= 0 && off < bs) return;  // not the first of its run
   const int prev = atomicExch(&l.head[blk], static_cast<int>(i) + 1);
   l.next[i] = prev;
-  if (prev == 0) l.owners[atomicAdd(l.count, 1)] = static_cast<int>(blk);
+  if (prev == 0)
+    l.owners[atomicAdd(l.count, 1)] = static_cast<int>(i);
+  else
+    atomicAdd(l.count + 1, 1);
 }
 
-template <typename T, typename C>
+// Calls f(in, offset, token) for the rows of the run that starts at `first`,
+// then of the block's other runs, by one warp.
+template <typename F>
+__device__ __forceinline__ void walk_runs(const Q8WriteArgs& a, const Q8Links& l, int64_t blk,
+                                          bool others, int first, F f) {
+  const int lane = threadIdx.x & 31;
+  const int64_t lo = blk * a.bs;
+  for (int run = others ? l.head[blk] : first + 1; run != 0;) {
+    const int64_t start = run - 1;
+    run = others ? l.next[start] : 0;
+    for (int64_t j = start + lane;; j += 32) {
+      const int64_t off = j < a.n ? a.slots[j] - lo : -1;
+      const bool in = off >= 0 && off < a.bs;
+      // a run ends at its first token of another block
+      const unsigned m = __ballot_sync(kAll, in);
+      const int len = m == kAll ? 32 : __ffs(~m) - 1;
+      f(lane < len, static_cast<int>(off), static_cast<int>(j));
+      if (len < 32) break;
+    }
+  }
+}
+
+// Blocks of up to 32 rows: every warp takes a task of its own, lane r holding
+// the token of row r.
+template <typename T, typename C, bool VEC>
 __global__ void __launch_bounds__(kQThreads) write_runs_kernel(const Q8WriteArgs a,
                                                                const Q8Links l) {
-  extern __shared__ int src[];
-  const int count = *l.count;
+  __shared__ int rows[kQWarps][32];
+  wait_prior_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // this warp's task of every `step`-th block
+  const int tasks = 2 * a.Hkv, warps = gridDim.x * kQWarps;
+  const int w = blockIdx.x * kQWarps + warp;
+  const int step = warps / tasks, task = w % tasks;
+  const int count = w / tasks < step ? l.count[0] : 0;
+  const bool others = l.count[1] != 0;
+  int o = w / tasks;
+  int next = o < count ? l.owners[o] : 0;
+  for (; o < count; o += step) {
+    const int first = next;
+    if (step < count - o) next = l.owners[o + step];  // (arrives during this task)
+    const int64_t s0 = a.slots[first];
+    const int64_t blk = (s0 >> 31) ? s0 / a.bs : static_cast<uint32_t>(s0) / a.bs;
+    rows[warp][lane] = -1;
+    __syncwarp();
+    walk_runs(a, l, blk, others, first, [&](bool in, int off, int j) {
+      if (in) atomicMax(&rows[warp][off], j);
+    });
+    __syncwarp();
+    const int mine = rows[warp][lane];
+    __syncwarp();
+    quantise_task<T, C, VEC>(a, blk, [&](int r) { return __shfl_sync(kAll, mine, r); },
+                             task / a.Hkv, task % a.Hkv);
+  }
+}
+
+// Larger blocks: a CTA per block, its rows' tokens in shared memory.
+template <typename T, typename C, bool VEC>
+__global__ void __launch_bounds__(kQThreads) write_blocks_kernel(const Q8WriteArgs a,
+                                                                 const Q8Links l) {
+  extern __shared__ int src[];
+  wait_prior_grid();
+  const int count = l.count[0];
+  const bool others = l.count[1] != 0;
+  const int warp = threadIdx.x >> 5;
   for (int o = blockIdx.x; o < count; o += gridDim.x) {
-    const int64_t blk = l.owners[o], lo = blk * a.bs;
+    const int first = l.owners[o];
+    const int64_t blk = a.slots[first] / a.bs;
     for (int r = threadIdx.x; r < a.bs; r += kQThreads) src[r] = -1;
     __syncthreads();
-    if (warp == 0) {
-      for (int run = l.head[blk]; run != 0;) {
-        const int64_t first = run - 1;
-        for (int64_t j = first + lane;; j += 32) {
-          const int64_t off = j < a.n ? a.slots[j] - lo : -1;
-          const bool in = off >= 0 && off < a.bs;
-          // a run ends at its first token of another block
-          const unsigned m = __ballot_sync(kAll, in);
-          const int len = m == kAll ? 32 : __ffs(~m) - 1;
-          if (lane < len) atomicMax(&src[off], static_cast<int>(j));
-          if (len < 32) break;
-        }
-        run = l.next[first];
-      }
-    }
+    if (warp == 0)
+      walk_runs(a, l, blk, others, first, [&](bool in, int off, int j) {
+        if (in) atomicMax(&src[off], j);
+      });
     __syncthreads();
     for (int task = warp; task < 2 * a.Hkv; task += kQWarps)
-      quantise_task<T, C>(a, blk, src, task / a.Hkv, task % a.Hkv);
+      quantise_task<T, C, VEC>(a, blk, [&](int r) { return src[r]; }, task / a.Hkv,
+                               task % a.Hkv);
     __syncthreads();
   }
 }
 
-// 16 codes to 16 values of T, multiplied by the scale in fp32 and rounded once;
-// finite values beyond T's range saturate.
+// Finite values beyond T's range saturate.
 template <typename T>
 __device__ __forceinline__ float saturate(float x) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -230,68 +408,118 @@ __device__ __forceinline__ float saturate(float x) {
   return x;
 }
 
+// 8 codes to 8 values of T, multiplied by the scale in fp32 and rounded once.
 template <typename T, typename C>
-__device__ __forceinline__ void store16(T* out, uint4 codes, float s, int vec) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+__device__ __forceinline__ void store8(T* out, uint2 codes, float s, int vec) {
+  constexpr float kLargest = std::is_same<C, int8_t>::value ? 127.f : 448.f;
+  constexpr float kTop = std::is_same<T, __half>::value ? 65504.f : 3.38e38f;
+  float4 f[2] = {decode4<C>(codes.x), decode4<C>(codes.y)};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 x = decode4<C>(w[i]);
-    const float a = saturate<T>(x.x * s), b = saturate<T>(x.y * s), c = saturate<T>(x.z * s),
-                d = saturate<T>(x.w * s);
-    T* p = out + 4 * i;
-    if (!vec) {
-      p[0] = DT<T>::from_f(a);
-      p[1] = DT<T>::from_f(b);
-      p[2] = DT<T>::from_f(c);
-      p[3] = DT<T>::from_f(d);
-    } else if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
-    } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
+  for (int i = 0; i < 2; ++i) f[i] = make_float4(f[i].x * s, f[i].y * s, f[i].z * s, f[i].w * s);
+  if (sizeof(T) == 2 && fabsf(s) > kTop / kLargest) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      f[i] = make_float4(saturate<T>(f[i].x), saturate<T>(f[i].y), saturate<T>(f[i].z),
+                         saturate<T>(f[i].w));
+  }
+  if (!vec) {
+    const float v[8] = {f[0].x, f[0].y, f[0].z, f[0].w, f[1].x, f[1].y, f[1].z, f[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = DT<T>::from_f(v[i]);
+  } else if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(out)[0] = f[0];
+    reinterpret_cast<float4*>(out)[1] = f[1];
+  } else {
+    *reinterpret_cast<uint4*>(out) =
+        make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[0].z, f[0].w), pack2<T>(f[1].x, f[1].y),
+                   pack2<T>(f[1].z, f[1].w));
+  }
+}
+
+// Threads that cover a row of Hkv * D codes in pieces of 8: `tpr` of them side
+// by side, or all of the CTA in turns; a CTA holds threads() of them.
+__host__ __device__ inline int piece_threads(int pieces) {
+  return pieces >= 256 ? 256 : 256 / pieces * pieces;
+}
+
+// Rows by slot; a thread reads the same piece of kRows rows at once, and the
+// slots of its next rows before these arrive.
+constexpr int kRows = 4;
+template <typename T, typename C>
+__global__ void __launch_bounds__(256)
+    gather_q8_kernel(T* out, const uint8_t* pool, const float* scale, const int64_t* slots,
+                     int64_t n, int Hkv, int D, int bs, int shift, int64_t num_slots, int vec,
+                     int32_t* err) {
+  wait_prior_grid();
+  const int pieces = Hkv * D / 8;
+  const int tpr = pieces < 256 ? pieces : 256;
+  const int side = blockDim.x / tpr;  // rows side by side
+  const int c0 = threadIdx.x % tpr;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * side * kRows;
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * side * kRows + threadIdx.x / tpr;
+  int64_t next[kRows];
+  auto fetch = [&](int64_t from) {
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) next[u] = from + u * side < n ? slots[from + u * side] : 0;
+  };
+  fetch(row0);
+  for (; row0 < n; row0 += step) {
+    int64_t s[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      s[u] = next[u];
+      if (s[u] < 0 || s[u] >= num_slots) {
+        s[u] = -1;
+        if (c0 == 0) set_err(err, IR_DEVERR_SLOT);
+      }
+    }
+    for (int c = c0; c < pieces; c += tpr) {
+      const int h = c * 8 / D;
+      uint2 codes[kRows];
+      float sc[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int64_t at = s[u] < 0 ? 0 : s[u];
+        const int64_t blk = shift >= 0 ? at >> shift : at / bs;
+        codes[u] = reinterpret_cast<const uint2*>(pool)[at * pieces + c];
+        sc[u] = scale[blk * Hkv + h];
+      }
+      if (c + tpr >= pieces) fetch(row0 + step);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int64_t r = row0 + u * side;
+        if (s[u] < 0) codes[u] = make_uint2(0u, 0u), sc[u] = 0.f;
+        if (r < n) store8<T, C>(out + (r * pieces + c) * 8, codes[u], sc[u], vec);
+      }
     }
   }
 }
 
-template <typename T, typename C>
-__global__ void gather_q8_kernel(T* out, const uint8_t* pool, const float* scale,
-                                 const int64_t* slots, int64_t n, int Hkv, int D, int bs,
-                                 int64_t num_slots, int vec, int32_t* err) {
-  const int cpr = Hkv * D / 16;  // 16-code chunks per row
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= n * cpr) return;
-  const int64_t r = i / cpr;
-  const int c = static_cast<int>(i - r * cpr);
-  const int64_t s = slots[r];
-  T* dst = out + i * 16;
-  if (s < 0 || s >= num_slots) {
-    if (c == 0) set_err(err, IR_DEVERR_SLOT);
-    store16<T, C>(dst, make_uint4(0, 0, 0, 0), 0.f, vec);
-    return;
-  }
-  const uint4 codes = *reinterpret_cast<const uint4*>(pool + (s * cpr + c) * 16);
-  store16<T, C>(dst, codes, scale[s / bs * Hkv + c * 16 / D], vec);
-}
-
 // Blocks of the sequences' histories, each to its own place in a pool of T.
 template <typename T, typename C>
-__global__ void expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp,
-                                     const float* ks, const float* vs, const int32_t* bt,
-                                     int64_t bt_stride, const int32_t* ctx, int max_blocks,
-                                     int64_t num_blocks, int Hkv, int D, int bs) {
+__global__ void __launch_bounds__(256)
+    expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp, const float* ks,
+                         const float* vs, const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
+                         int max_blocks, int64_t num_blocks, int Hkv, int D, int bs) {
+  wait_prior_grid();
   const int sq = blockIdx.x;
   const int64_t c0 = ctx[sq];
-  const int cpr = Hkv * D / 16;
-  const int64_t chunks = static_cast<int64_t>(bs) * cpr;
+  const int pieces = Hkv * D / 8;
+  const int tpr = pieces < 256 ? pieces : 256;
+  const int side = blockDim.x / tpr;
   for (int j = blockIdx.y; j < max_blocks && static_cast<int64_t>(j) * bs < c0; j += gridDim.y) {
     const int64_t id = bt[sq * bt_stride + j];
     if (id < 0 || id >= num_blocks) continue;  // the attention kernel reports it
-    const int64_t base = id * chunks;
-    for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) {
-      const int h = static_cast<int>(i % cpr) * 16 / D;
-      const uint4 kc = reinterpret_cast<const uint4*>(kp)[base + i];
-      const uint4 vc = reinterpret_cast<const uint4*>(vp)[base + i];
-      store16<T, C>(kout + (base + i) * 16, kc, ks[id * Hkv + h], 1);
-      store16<T, C>(vout + (base + i) * 16, vc, vs[id * Hkv + h], 1);
+    for (int c = threadIdx.x % tpr; c < pieces; c += tpr) {
+      const float k = ks[id * Hkv + c * 8 / D], v = vs[id * Hkv + c * 8 / D];
+#pragma unroll 4
+      for (int r = threadIdx.x / tpr; r < bs; r += side) {
+        const int64_t at = (id * bs + r) * pieces + c;
+        const uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
+        const uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
+        store8<T, C>(kout + at * 8, kc, k, 1);
+        store8<T, C>(vout + at * 8, vc, v, 1);
+      }
     }
   }
 }
@@ -311,15 +539,12 @@ int by_type(int dtype, F f) {
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Calls of up to this many tokens find each block's rows by reading all slots.
-constexpr int64_t kScanTokens = 1024;
-
 }  // namespace
 
 size_t cache_write_q8_workspace(int64_t n, int64_t num_blocks) {
   if (n <= kScanTokens) return 0;
   const int64_t owners = n < num_blocks ? n : num_blocks;
-  return align256(static_cast<size_t>(num_blocks + 1) * 4) + align256(static_cast<size_t>(n) * 4) +
+  return align256(static_cast<size_t>(num_blocks + 2) * 4) + align256(static_cast<size_t>(n) * 4) +
          align256(static_cast<size_t>(owners) * 4);
 }
 
@@ -332,8 +557,8 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   Q8WriteArgs a{};
   a.src[0] = k;
   a.src[1] = v;
-  a.stride[0] = k_stride;
-  a.stride[1] = v_stride;
+  a.stride[0] = static_cast<int>(k_stride);
+  a.stride[1] = static_cast<int>(v_stride);
   a.pool[0] = static_cast<uint8_t*>(k_pool);
   a.pool[1] = static_cast<uint8_t*>(v_pool);
   a.scale[0] = k_scale;
@@ -344,57 +569,71 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   a.Hkv = Hkv;
   a.D = D;
   a.bs = bs;
-  a.vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % (4 * eb)) == 0 &&
-          k_stride % 4 == 0 && v_stride % 4 == 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % (4 * eb)) == 0 &&
+                   k_stride % 4 == 0 && v_stride % 4 == 0;
   a.err = err;
   const size_t smem = static_cast<size_t>(bs) * 4;
   if (n <= kScanTokens) {
     const dim3 grid(static_cast<unsigned>(n), (2 * Hkv + kQWarps - 1) / kQWarps);
     return by_type(dtype, [&](auto t) {
       return by_format(fmt, [&](auto c) {
-        write_scan_kernel<decltype(t), decltype(c)><<<grid, kQThreads, smem, stream>>>(a);
-        return static_cast<int>(cudaGetLastError());
+        using T = decltype(t);
+        using C = decltype(c);
+        return launch_behind(vec ? write_scan_kernel<T, C, true> : write_scan_kernel<T, C, false>,
+                             grid, kQThreads, smem, stream, a);
       });
     });
   }
   const int64_t num_blocks = num_slots / bs;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  const size_t heads = align256(static_cast<size_t>(num_blocks + 1) * 4);
+  const size_t heads = align256(static_cast<size_t>(num_blocks + 2) * 4);
   Q8Links l;
   l.count = reinterpret_cast<int*>(w);
-  l.head = l.count + 1;
+  l.head = l.count + 2;
   l.next = reinterpret_cast<int*>(w + heads);
   l.owners = reinterpret_cast<int*>(w + heads + align256(static_cast<size_t>(n) * 4));
   cudaError_t e = cudaMemsetAsync(w, 0, heads, stream);
   if (e != cudaSuccess) return static_cast<int>(e);
-  link_runs_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(
-      slots, n, num_slots, bs, l, err);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  int64_t grid = n < num_blocks ? n : num_blocks;
+  int rc = launch_behind(link_runs_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0,
+                         stream, slots, n, num_slots, bs, l, err);
+  if (rc) return rc;
+  const int64_t blocks = n < num_blocks ? n : num_blocks;
+  const bool small = bs <= 32;
+  // (at least one warp for every task of a block)
+  const int64_t least = (2 * Hkv + kQWarps - 1) / kQWarps;
+  int64_t grid = small ? (blocks * 2 * Hkv + kQWarps - 1) / kQWarps : blocks;
   if (grid > static_cast<int64_t>(sms) * 8) grid = static_cast<int64_t>(sms) * 8;
+  if (small && grid < least) grid = least;
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
-      write_runs_kernel<decltype(t), decltype(c)>
-          <<<static_cast<unsigned>(grid), kQThreads, smem, stream>>>(a, l);
-      return static_cast<int>(cudaGetLastError());
+      using T = decltype(t);
+      using C = decltype(c);
+      auto kern = small ? (vec ? write_runs_kernel<T, C, true> : write_runs_kernel<T, C, false>)
+                        : (vec ? write_blocks_kernel<T, C, true> : write_blocks_kernel<T, C, false>);
+      return launch_behind(kern, dim3(static_cast<unsigned>(grid)), kQThreads, small ? 0 : smem,
+                           stream, a, l);
     });
   });
 }
 
 int launch_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
                            int64_t n, int Hkv, int D, int bs, int64_t num_slots, int dtype,
-                           int fmt, int32_t* err, cudaStream_t stream) {
-  const int64_t work = n * (static_cast<int64_t>(Hkv) * D / 16);
-  const unsigned grid = static_cast<unsigned>((work + 255) / 256);
+                           int fmt, int sms, int32_t* err, cudaStream_t stream) {
+  const int pieces = Hkv * D / 8, threads = piece_threads(pieces);
+  const int64_t rows = static_cast<int64_t>(pieces < 256 ? threads / pieces : 1) * kRows;
+  int64_t grid = (n + rows - 1) / rows;
+  if (grid > static_cast<int64_t>(sms) * 4) grid = static_cast<int64_t>(sms) * 4;
   const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  int shift = 0;  // log2(bs), or -1
+  while ((1 << shift) < bs && shift < 30) ++shift;
+  if ((1 << shift) != bs) shift = -1;
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
       using T = decltype(t);
-      gather_q8_kernel<T, decltype(c)><<<grid, 256, 0, stream>>>(
-          static_cast<T*>(out), static_cast<const uint8_t*>(pool), scale, slots, n, Hkv, D, bs,
-          num_slots, vec, err);
-      return static_cast<int>(cudaGetLastError());
+      return launch_behind(gather_q8_kernel<T, decltype(c)>, dim3(static_cast<unsigned>(grid)),
+                           threads, 0, stream,
+                           static_cast<T*>(out), static_cast<const uint8_t*>(pool), scale, slots,
+                           n, Hkv, D, bs, shift, num_slots, vec, err);
     });
   });
 }
@@ -410,11 +649,11 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
       using T = decltype(t);
-      expand_blocks_kernel<T, decltype(c)><<<grid, 256, 0, stream>>>(
-          static_cast<T*>(k_out), static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
-          static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride, ctx, max_blocks,
-          num_blocks, Hkv, D, bs);
-      return static_cast<int>(cudaGetLastError());
+      return launch_behind(expand_blocks_kernel<T, decltype(c)>, grid,
+                           piece_threads(Hkv * D / 8), 0, stream, static_cast<T*>(k_out),
+                           static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
+                           static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride,
+                           ctx, max_blocks, num_blocks, Hkv, D, bs);
     });
   });
 }

@@ -1127,6 +1127,8 @@ int ir_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_t v_
   const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
   if (k_stride < row || v_stride < row)
     return fail(IR_ERR_INVALID_ARG, "token stride < Hkv*D");
+  if (k_stride > INT32_MAX || v_stride > INT32_MAX)
+    return fail(IR_ERR_UNSUPPORTED, "token stride of 2^31 elements or more");
   if (!k || !v || !k_pool || !v_pool || !k_scale || !v_scale || !slot_mapping)
     return fail(IR_ERR_INVALID_ARG, "null pointer");
   if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
@@ -1157,9 +1159,12 @@ int ir_cache_gather_q8(void* out, const void* pool, const float* scale, const in
   if (num_rows == 0) return IR_OK;
   if (!out || !pool || !scale || !slots) return fail(IR_ERR_INVALID_ARG, "null pointer");
   if (!aligned(pool, 16)) return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
+  int sms = 1;
+  const int e = cached(-1, sm_count_now, 0, &sms);
+  if (e) return cuda_status(e, "device query");
   return cuda_status(irb::launch_cache_gather_q8(out, pool, scale, slots, num_rows, num_kv_heads,
                                                  head_dim, block_size, num_slots, dtype,
-                                                 kv_format, err_flag,
+                                                 kv_format, sms, err_flag,
                                                  static_cast<cudaStream_t>(stream)),
                      "8-bit cache gather launch");
 }

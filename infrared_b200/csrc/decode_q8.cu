@@ -4,26 +4,30 @@
 //
 // Work partition, pieces and merge are the 16-bit kernel's (decode_common.cuh).
 // A CTA owns HG kv heads and one share of the 16-token tiles. The producer
-// warp resolves 32 tiles at a time and sends items of up to W = kConsumers / HG
+// warp resolves 32 tiles at a time and sends items of up to W = 8 / HG
 // neighbouring tiles of one sequence through a ring of stages; its lanes issue
 // the tiles' tensor copies (one box per block and side: [HG][rows][D] bytes)
 // and copy the blocks' scales with 4-byte asynchronous copies that complete on
-// the same barrier. Consumer warp (head, w) takes tile w of every item, so
-// that kConsumers warps work whatever the head count; at the end of a segment
-// the W warps of a head combine their states through shared memory.
+// the same barrier. Two sets of 8 consumer warps take the items in turn, warp
+// (head, w) of a set tile w of the item: the work on a tile is a chain of
+// dependent steps, so the warps of an SM hide one another's latency (8 warps
+// alone: 43 us for 64 sequences of 512-4096 tokens, against 33 us). For
+// groups of 9-16 query heads both sets take every item, each for 8 of the
+// heads. At the end of a segment the warps of a head combine their states
+// through shared memory, in halves.
 //
-// Mathematics of a tile (16 tokens, one kv head, up to 8 query heads per set):
+// Mathematics of a tile (16 tokens, one kv head, 8 query heads):
 //   S^T[16 x 8] = K[16 x D] . Q^T     (codes as fp16, q as fp16)
 //   s = S * (k scale of the block) * (2^-e of the q row) * softmax scale
-//   O^T[D x 8]  = O^T * alpha + (v scale of the block) * (V^T . P^T)
+//   O^T[D x 8] += (v scale of the block) * (V^T . P^T),  P = 2^(s - m + 7)
 // A code is exact in fp16. q is multiplied by a power of two that puts its
 // row's largest magnitude in [2^13, 2^14), so its 8 (bf16) or 11 (fp16) bits
-// stay exact down to 2^-27 of that. P is fp16 with exponents shifted by 2^7:
-// one rounding of 2^-12 per weight, small weights kept down to 2^-31 of the
-// largest. Scales are applied in fp32 to the fp32 accumulators, so they may
-// have any value; the products P.V of one tile start from zero to keep the
-// blocks' scales apart, at the cost of an FMA in place of the multiply that
-// rescales the accumulator anyway.
+// stay exact down to 2^-27 of that. The reference m of a row is raised, and O
+// rescaled, only when a score exceeds it by more than 8: P stays below 2^15,
+// in fp16 with one rounding of 2^-11 per weight, and weights down to 2^-29 of
+// the largest keep a nonzero value. Scales are applied in fp32 to the fp32
+// accumulators, so they may have any value; the products P.V of one tile
+// start from zero to keep the blocks' scales apart.
 //
 // The tensor-core instructions are the warp-level form, as in the 16-bit
 // kernel: 7 query heads per K/V byte stay far below the ridge, and the codes
@@ -45,24 +49,31 @@ namespace irb {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kConsumers = 8;             // consumer warps
+constexpr int kConsumers = 8;      // consumer warps
 constexpr int kThreads = 32 * (kConsumers + 1);
-constexpr float kPShift = 7.f;            // P is scaled by 2^7
+constexpr float kPShift = 7.f;     // P is scaled by 2^7
+constexpr float kSlack = 8.f;      // scores may exceed their row's reference by this
 
 struct __align__(16) ItemQ8 {
   int b;
   int unit;
   int ntok;   // valid tokens of the item (16 per tile but the last)
-  int flags;  // bits 0-7: tiles whose copies were issued
+  int flags;  // bits 0-15: tiles whose copies were issued
 };
-constexpr int kSegStart = 1 << 8;  // first item of a segment
-constexpr int kWhole = 1 << 9;     // the segment is the whole sequence
-constexpr int kEnd = 1 << 10;      // end-of-stream marker
-constexpr int kQBuf1 = 1 << 11;    // the segment's q rows are in buffer 1
+constexpr int kSegStart = 1 << 16;  // first item of a segment
+constexpr int kWhole = 1 << 17;     // the segment is the whole sequence
+constexpr int kEnd = 1 << 18;       // end-of-stream marker
+constexpr int kQBuf1 = 1 << 19;     // the segment's q rows are in buffer 1
 
-template <int D, int HG, int R, int NS, int NQ>
+// SETS: a group of 9-16 query heads, as two sets of 8 with a state each.
+template <int D, int HG, int R, int NS, bool SETS>
 struct LayoutQ8 {
-  static constexpr int W = kConsumers / HG;       // tiles per item
+  static constexpr int kRows = SETS ? 2 * HG : HG;   // (head, query set) pairs
+  static constexpr int WT = kConsumers / kRows;      // warps that share a pair's state
+  // tiles a warp takes of an item at once (of 8-row blocks one: their second
+  // set of scales and products takes the place)
+  static constexpr int kPair = R == 8 ? 1 : 2;
+  static constexpr int W = WT * kPair;               // tiles per item
   static constexpr int NB = kTile / R;            // blocks per tile
   static constexpr int kRegion = R * D;           // one head of one box
   static constexpr int kBox = HG * kRegion;       // one box
@@ -70,41 +81,31 @@ struct LayoutQ8 {
   static constexpr int kTileBytes = 2 * kSide;
   static constexpr int kStage = W * kTileBytes;
   static constexpr int kScales = W * NB * 2 * HG;  // floats per stage
+  static constexpr int kSteps = 5;                 // barriers of a combination
   static constexpr int off_scale = NS * kStage;
   static constexpr int off_desc = off_scale + NS * kScales * 4;
-  static constexpr int off_bar = off_desc + NS * 16;  // full[NS], empty[NS], qfree[2], head[HG]
-  static constexpr int off_misc = (off_bar + (2 * NS + 2 + HG) * 8 + 15) / 16 * 16;
-  // misc: RangeInfo (64 B) + block-scan scratch; then (m, l) of every warp
+  // full[NS], empty[NS], qfree[2], then kSteps per pair
+  static constexpr int off_bar = off_desc + NS * 16;
+  static constexpr int off_misc = (off_bar + (2 * NS + 2 + kRows * kSteps) * 8 + 15) / 16 * 16;
+  // misc: RangeInfo (64 B) + block-scan scratch; then (m, l) of every warp, twice
   static constexpr int off_ml = off_misc + 64 + (kConsumers + 1) * 8 + 8;
-  static constexpr int kMl = kConsumers * NQ * 8 * 2;  // floats
-  static constexpr int kFlushStride = D + 4;
-  static constexpr int kFlushFloats = NQ * 8 * kFlushStride;  // per consumer warp
-  static constexpr int off_flush = (off_ml + kMl * 4 + 15) / 16 * 16;
-  static constexpr int kQBuf = HG * NQ * 8 * D * 2;
-  static constexpr int off_q = (off_flush + kConsumers * kFlushFloats * 4 + 127) / 128 * 128;
+  static constexpr int kMl = kConsumers * 8 * 2;  // floats of one copy
+  static constexpr int kPart = 8 * D;             // floats of one warp's O
+  static constexpr int off_part = (off_ml + 2 * kMl * 4 + 15) / 16 * 16;
+  static constexpr int kParts = kRows * (WT / 2);
+  static constexpr int kQBuf = HG * (SETS ? 16 : 8) * D * 2;
+  static constexpr int off_q = (off_part + kParts * kPart * 4 + 127) / 128 * 128;
   static constexpr int kBytes = off_q + 2 * kQBuf;
   static constexpr int kAlloc = kBytes + 1024;  // slack for 1 KB alignment
 };
 
 // Stages that fit in one CTA's shared memory beside the other buffers.
-template <int D, int HG, int R, int NQ>
+template <int D, int HG, int R, bool SETS, int NS = 12>
 constexpr int stages_q8() {
-  using L0 = LayoutQ8<D, HG, R, 0, NQ>;
-  constexpr int per = L0::kStage + L0::kScales * 4 + 16 + 16;
-  constexpr int n = (227 * 1024 - L0::kAlloc - 256) / per;
-  return n < 2 ? 2 : (n > 12 ? 12 : n);
-}
-
-// Four-byte asynchronous copy global -> shared, and this thread's arrival on
-// `bar` once its earlier copies have landed (counted in the barrier's own
-// expected arrivals).
-__device__ __forceinline__ void copy4_async(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  if constexpr (NS == 2 || LayoutQ8<D, HG, R, NS, SETS>::kAlloc <= 227 * 1024)
+    return NS;
+  else
+    return stages_q8<D, HG, R, SETS, NS - 1>();
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -127,12 +128,12 @@ __device__ __forceinline__ int chunk_off(int r, int c) {
   return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-template <typename T, typename C, int D, int HG, int R, int NQ, int NS>
+template <typename T, typename C, int D, int HG, int R, bool SETS, int NS>
 __global__ void __launch_bounds__(kThreads, 1)
     decode_q8_kernel(const __grid_constant__ CUtensorMap tmk,
                      const __grid_constant__ CUtensorMap tmv, const DecodeArgs a, int q_bulk) {
-  using L = LayoutQ8<D, HG, R, NS, NQ>;
-  constexpr int W = L::W, NB = L::NB;
+  using L = LayoutQ8<D, HG, R, NS, SETS>;
+  constexpr int W = L::W, NB = L::NB, WT = L::WT, kPair = L::kPair;
   constexpr int KS = D / 16;  // k-steps of Q.K, m-tiles of P.V
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::off_bar);
   uint64_t* empty = full + NS;
   uint64_t* qfree = empty + NS;
-  uint64_t* hbar = qfree + 2;  // the W warps of a head meet here at a segment's end
+  uint64_t* hbar = qfree + 2;  // kSteps per (head, query set): the warps of a row's state
   RangeInfo* ri = reinterpret_cast<RangeInfo*>(smem + L::off_misc);
   static_assert(sizeof(RangeInfo) <= 64, "RangeInfo fits its shared-memory slot");
   int64_t* sm_scan = reinterpret_cast<int64_t*>(smem + L::off_misc + 64);
@@ -152,12 +153,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 33);  // the copies' byte count, and every producer lane
+      mbar_init(&full[i], 1);
       mbar_init(&empty[i], kConsumers);
     }
     mbar_init(&qfree[0], kConsumers);
     mbar_init(&qfree[1], kConsumers);
-    for (int i = 0; i < HG; ++i) mbar_init(&hbar[i], W);
+    for (int i = 0; i < L::kRows; ++i) {
+      mbar_init(&hbar[i * L::kSteps], WT);  // (m, l) of every warp written
+      for (int k = 1; k < L::kSteps; ++k)   // step k: half of the rest wrote its O
+        mbar_init(&hbar[i * L::kSteps + k], (WT >> k) > 0 ? WT >> k : 1);
+    }
     fence_mbar_init();
   }
   if (threadIdx.x == 32) {
@@ -172,13 +177,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    // Lane i resolves tile t + i: its sequence, block and scales. Tiles of one
+    // aligned group of W lanes and one segment are an item, led by their
+    // first lane; then, item by item, the lanes of an item issue their own
+    // copies and store their own scales, so that little is left to do between
+    // a stage falling free and its copies.
     int b = ri->b_first;
     int64_t pb = ri->p_first;
     int nb = tiles_of(a, b);
-    int seg_base = 0;  // segments started before this batch
-    uint32_t item = 0;
+    int seg = -1;  // segments started before this batch, less one
+    uint32_t slot = 0, par = 1;
     bool abort = false;
-    for (int64_t t = start; t < end && !abort;) {
+    const float* kscale = a.k_scale + kv0;
+    const float* vscale = a.v_scale + kv0;
+    for (int64_t t = start; t < end && !abort; t += 32) {
       const int64_t tt = t + lane;
       const bool active = tt < end;
       int lb = b, ln = nb;
@@ -191,10 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const int j = static_cast<int>(tt - lp);
-      const int tok0 = j * kTile;
       int nvalid = 0, id0 = 0, id1 = -1, row0 = 0;
-      bool ok = false, seg_start = false, whole = false;
+      bool ok = false, seg_start = false;
       if (active) {
+        const int tok0 = j * kTile;
         nvalid = min(kTile, clamp_ctx(a.context_lens[lb], a) - tok0);
         const int32_t* btr = a.block_tables + lb * a.bt_stride;
         const int blk = tok0 / a.bs;
@@ -207,107 +219,94 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) set_err(a.err, IR_DEVERR_BLOCK_ID);
         seg_start = (tt == start) || (j == 0);
-        whole = (lp >= start) && (lp + ln <= end);
+      }
+      const bool whole = (lp >= start) && (lp + ln <= end);
+      // scales [block][side][head] of this tile (in flight until they are stored)
+      float sc[NB * 2 * HG];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int64_t id = i == 0 ? id0 : id1;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          sc[(2 * i) * HG + h] = ok && id >= 0 ? kscale[id * a.Hkv + h] : 0.f;
+          sc[(2 * i + 1) * HG + h] = ok && id >= 0 ? vscale[id * a.Hkv + h] : 0.f;
+        }
       }
       const unsigned starts = __ballot_sync(kFull, active && seg_start);
       const unsigned oks = __ballot_sync(kFull, ok);
+      const unsigned lead = __ballot_sync(kFull, active && (seg_start || lane % W == 0));
+      const unsigned upto = lane == 31 ? kFull : (2u << lane) - 1u;
+      const unsigned mine = lead & upto;  // leaders up to this lane: the last is its own
+      const int leader = active ? 31 - __clz(mine) : -1;
+      const unsigned after = lead & ~upto;
       const int nact = (end - t) < 32 ? static_cast<int>(end - t) : 32;
-      int k = 0;
-      while (k < nact) {
-        // tiles k .. k + n - 1: neighbours of one segment
-        const unsigned later = starts & ~((2u << k) - 1u);
-        const int lim = (k < 31 && later) ? __ffs(later) - 1 : nact;
-        const int n = min(W, lim - k);
-        if (n < W && lim == nact && t + nact < end && k > 0) break;  // look further first
-        const uint32_t slot = item % NS;
-        const uint32_t par = ((item / NS) & 1u) ^ 1u;
-        const bool first = (starts >> k) & 1u;
-        const int seg = seg_base + __popc(starts & ((2u << k) - 1u)) - 1;
-        const bool with_q = q_bulk && first;
-        int good = 1;
-        if (lane == 0) {
-          good = mbar_wait_bounded(&empty[slot], par) ? 1 : 0;
-          if (good && with_q && seg >= 2)
-            good = mbar_wait_bounded(&qfree[seg & 1], ((seg >> 1) + 1) & 1) ? 1 : 0;
+      // for leaders: tiles of the item, valid tokens, bytes and flags
+      const int n = (after ? __ffs(after) - 1 : nact) - lane;
+      const int last = __shfl_sync(kFull, nvalid, (lane + n - 1) & 31);
+      const unsigned issued = (oks >> lane) & ((1u << (n > 0 ? n : 0)) - 1u);
+      const int kseg = seg + __popc(starts & upto);
+      uint32_t bytes = __popc(issued) * static_cast<uint32_t>(L::kTileBytes);
+      if (R == 8 && last <= 8 && n > 0 && ((issued >> (n - 1)) & 1u)) bytes -= 2u * L::kBox;
+      const ItemQ8 it{lb, g, (n - 1) * kTile + last,
+                      static_cast<int>(issued) | (seg_start ? kSegStart : 0) |
+                          (whole ? kWhole : 0) | ((kseg & 1) ? kQBuf1 : 0)};
+      const uint32_t qrows = static_cast<uint32_t>(HG * a.n_rep * D * 2);
+
+      for (unsigned left = lead; left != 0; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        bool good = mbar_wait_bounded(&empty[slot], par);
+        if (q_bulk && ((starts >> k) & 1u)) {
+          const int sg = __shfl_sync(kFull, kseg, k);
+          if (sg >= 2) good = good && mbar_wait_bounded(&qfree[sg & 1], ((sg >> 1) + 1) & 1);
         }
-        if (!__shfl_sync(kFull, good, 0)) {
+        if (!__all_sync(kFull, good)) {
           if (lane == 0) set_err(a.err, IR_DEVERR_TIMEOUT);
           abort = true;
           break;
         }
-        const int kb = __shfl_sync(kFull, lb, k);
-        const int last_valid = __shfl_sync(kFull, nvalid, k + n - 1);
-        const int kwhole = __shfl_sync(kFull, whole ? 1 : 0, k);
-        const unsigned issued = (oks >> k) & ((1u << n) - 1u);
-        uint8_t* st = smem + slot * L::kStage;
-        if (lane == 0) {
-          desc[slot] = ItemQ8{kb, g, (n - 1) * kTile + last_valid,
-                              static_cast<int>(issued) | (first ? kSegStart : 0) |
-                                  (kwhole ? kWhole : 0) | ((seg & 1) ? kQBuf1 : 0)};
-          uint32_t bytes = 0;
-          for (int w = 0; w < n; ++w)
-            if ((issued >> w) & 1u)
-              bytes += (R == 8 && w == n - 1 && last_valid <= 8) ? 2u * L::kBox
-                                                                  : static_cast<uint32_t>(
-                                                                        L::kTileBytes);
-          const uint32_t qrows = static_cast<uint32_t>(HG * a.n_rep * D * 2);
-          mbar_arrive_expect_tx(&full[slot], bytes + (with_q ? qrows : 0u));
-          if (with_q)
-            bulk_load(smem + L::off_q + (seg & 1) * L::kQBuf,
-                      reinterpret_cast<const T*>(a.q) + kb * a.q_stride +
-                          static_cast<int64_t>(kv0 * a.n_rep) * D,
-                      qrows, &full[slot]);
+        if (leader == k) {
+          uint8_t* td = smem + slot * L::kStage + (lane - k) * L::kTileBytes;
+          if (ok) {
+            tma_load_3d(td, &tmk, &full[slot], 0, row0, kv0);
+            tma_load_3d(td + L::kSide, &tmv, &full[slot], 0, row0, kv0);
+            if (R == 8 && id1 >= 0) {
+              tma_load_3d(td + L::kBox, &tmk, &full[slot], 0, id1 * a.bs, kv0);
+              tma_load_3d(td + L::kSide + L::kBox, &tmv, &full[slot], 0, id1 * a.bs, kv0);
+            }
+          }
+          if (lane == k) {
+            desc[slot] = it;
+            if (q_bulk && seg_start)
+              bulk_load(smem + L::off_q + (kseg & 1) * L::kQBuf,
+                        reinterpret_cast<const T*>(a.q) + lb * a.q_stride +
+                            static_cast<int64_t>(kv0 * a.n_rep) * D,
+                        qrows, &full[slot]);
+          }
+          float* so = scales + slot * L::kScales + (lane - k) * (NB * 2 * HG);
+#pragma unroll
+          for (int i = 0; i < NB * 2 * HG; ++i) so[i] = sc[i];
         }
         __syncwarp();
-        if (lane >= k && lane < k + n && ok) {
-          uint8_t* td = st + (lane - k) * L::kTileBytes;
-          tma_load_3d(td, &tmk, &full[slot], 0, row0, kv0);
-          tma_load_3d(td + L::kSide, &tmv, &full[slot], 0, row0, kv0);
-          if (R == 8 && id1 >= 0) {
-            tma_load_3d(td + L::kBox, &tmk, &full[slot], 0, id1 * a.bs, kv0);
-            tma_load_3d(td + L::kSide + L::kBox, &tmv, &full[slot], 0, id1 * a.bs, kv0);
-          }
+        if (lane == k) mbar_arrive_expect_tx(&full[slot], bytes + (q_bulk && seg_start ? qrows : 0u));
+        if (++slot == NS) {
+          slot = 0;
+          par ^= 1u;
         }
-        // scales[tile][block][side][head]
-        float* sc = scales + slot * L::kScales;
-#pragma unroll
-        for (int base = 0; base < L::kScales; base += 32) {
-          const int i = base + lane;
-          const int w = i / (NB * 2 * HG), rem = i % (NB * 2 * HG);
-          const int blk = rem / (2 * HG), side = rem / HG % 2, h = rem % HG;
-          const int src = (k + w) & 31;
-          const int i0 = __shfl_sync(kFull, id0, src), i1 = __shfl_sync(kFull, id1, src);
-          const int id = blk == 0 ? i0 : i1;
-          if (i < L::kScales && w < n && ((issued >> w) & 1u) && id >= 0)
-            copy4_async(sc + i, (side ? a.v_scale : a.k_scale) +
-                                    static_cast<int64_t>(id) * a.Hkv + kv0 + h);
-        }
-        arrive_after_copies(&full[slot]);
-        ++item;
-        k += n;
       }
-      if (abort) break;
-      seg_base += __popc(starts & (k >= 32 ? kFull : ((1u << k) - 1u)));
-      // the cursor at the last tile issued
-      b = __shfl_sync(kFull, lb, k - 1);
-      pb = __shfl_sync(kFull, lp, k - 1);
-      nb = __shfl_sync(kFull, ln, k - 1);
-      t += k;
+      seg += __popc(starts);
+      b = __shfl_sync(kFull, lb, nact - 1);
+      pb = __shfl_sync(kFull, lp, nact - 1);
+      nb = __shfl_sync(kFull, ln, nact - 1);
     }
     if (!abort) {
-      const uint32_t slot = item % NS;
-      const uint32_t par = ((item / NS) & 1u) ^ 1u;
-      int good = 1;
-      if (lane == 0) good = mbar_wait_bounded(&empty[slot], par) ? 1 : 0;
-      if (__shfl_sync(kFull, good, 0)) {
-        if (lane == 0) {
+      const bool good = mbar_wait_bounded(&empty[slot], par);
+      if (lane == 0) {
+        if (good) {
           desc[slot] = ItemQ8{0, 0, 0, kEnd};
           mbar_arrive(&full[slot]);
+        } else {
+          set_err(a.err, IR_DEVERR_TIMEOUT);
         }
-        __syncwarp();
-        mbar_arrive(&full[slot]);
-      } else if (lane == 0) {
-        set_err(a.err, IR_DEVERR_TIMEOUT);
       }
     }
     return;
@@ -315,8 +314,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // -------------------------------------------------------------- consumers
   const int cw = warp - 1;
-  const int head = cw / W, w = cw % W;
+  const int row = cw / WT, part = cw % WT;  // the state this warp shares, its place there
+  const int first = row * WT;               // place of the row's first warp
+  const int head = SETS ? row / 2 : row, set = SETS ? row % 2 : 0;
   const int kvh = kv0 + head;
+  const int n0 = SETS ? set * 8 : 0;             // first query head of the set
+  const int nq = min(8, a.n_rep - n0);           // query heads of the set
   const int grp = lane >> 2, qq = lane & 3, qd = qq * 2;
   const int tg = (grp & 1) ? 4 + ((grp >> 1) ^ 1) : grp >> 1;  // token of fragment row grp
   // byte offsets of this lane's reads within one 8-row half of a region
@@ -332,132 +335,135 @@ __global__ void __launch_bounds__(kThreads, 1)
   // second half of a tile: 8 rows on in the same box, or the second box
   constexpr int kHalf = R == 8 ? L::kBox : 8 * D;
 
-  float acc[NQ][KS][4];
-  float m[NQ][2], l[NQ][2], qinv[NQ][2];
-  uint32_t qf[NQ][KS][2];
+  float acc[KS][4];
+  float m[2], l[2], qinv[2] = {0.f, 0.f};
+  uint32_t qf[KS][2];
   auto reset = [&]() {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-      for (int i = 0; i < KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
-    }
+    for (int i = 0; i < KS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
   };
   reset();
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    qinv[n][0] = qinv[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) qf[n][i][0] = qf[n][i][1] = 0u;
-  }
+  for (int i = 0; i < KS; ++i) qf[i][0] = qf[i][1] = 0u;
   int seg_b = -1, seg_unit = 0;
   bool seg_whole = false, have_seg = false;
-  uint32_t meets = 0;  // phases of hbar passed
-  float* ml = reinterpret_cast<float*>(smem + L::off_ml);
-  float* fl = reinterpret_cast<float*>(smem + L::off_flush) + cw * L::kFlushFloats;
+  uint32_t flushes = 0;
 
-  // The W warps of this head wait for one another (bounded).
-  auto meet = [&]() {
-    if (W == 1) {
-      __syncwarp();
-      return true;
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&hbar[head]);
-    const bool ok = mbar_wait_bounded(&hbar[head], meets & 1u);
-    ++meets;
-    return __all_sync(kFull, ok) != 0;
-  };
-
-  // Combine the W states of the finished segment and write its rows: the
-  // output (whole sequences) or a normalised fp32 piece.
+  // Combine the WT states of the finished segment and write its rows: the
+  // output (whole sequences) or a normalised fp32 piece. (m, l) are exchanged
+  // first, so every warp brings its O to the common scale itself; then in each
+  // step the upper half of the remaining warps hands its O to the lower half
+  // through the buffer it last read (the first step: the reader's own).
   auto flush = [&]() {
-    const int nr = a.n_rep;
-    const int64_t pslot = static_cast<int64_t>(kvh) * a.ws_slots + seg_unit + seg_b;
+    uint64_t* bar = hbar + row * L::kSteps;
+    const uint32_t par = flushes & 1u;
+    float2* ml = reinterpret_cast<float2*>(smem + L::off_ml) + (flushes & 1u) * (L::kMl / 2);
+    ++flushes;
+    float f[2], lse[2];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int j = 0; j < 2; ++j) {
+      l[j] += __shfl_xor_sync(kFull, l[j], 4);
+      l[j] += __shfl_xor_sync(kFull, l[j], 8);
+      l[j] += __shfl_xor_sync(kFull, l[j], 16);
+      if (WT > 1 && grp == 0) ml[(first + part) * 8 + qd + j] = make_float2(m[j], l[j]);
+    }
+    if (WT > 1) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[0]);
+      if (!__all_sync(kFull, mbar_wait_bounded(&bar[0], par))) return false;
+    }
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        float x = l[n][jj];
-        x += __shfl_xor_sync(kFull, x, 4);
-        x += __shfl_xor_sync(kFull, x, 8);
-        x += __shfl_xor_sync(kFull, x, 16);
-        l[n][jj] = x;
-        if (grp == 0) {
-          float* p = ml + ((cw * NQ + n) * 8 + qd + jj) * 2;
-          p[0] = m[n][jj];
-          p[1] = x;
-        }
+    for (int j = 0; j < 2; ++j) {
+      float M = m[j], Ls = 0.f;
+      if (WT > 1) {
+        M = -INFINITY;
+#pragma unroll 4
+        for (int i = 0; i < WT; ++i) M = fmaxf(M, ml[(first + i) * 8 + qd + j].x);
       }
-    if (!meet()) return false;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-          M = fmaxf(M, ml[(((head * W + i) * NQ + n) * 8 + qd + jj) * 2]);
-        const float use = M == -INFINITY ? 0.f : M;
-        float Ls = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float* p = ml + (((head * W + i) * NQ + n) * 8 + qd + jj) * 2;
-          Ls += p[1] * ex2(p[0] - use);
-        }
-        // nothing attended: zero (a NaN sum is not nothing)
-        const float f = Ls == 0.f ? 0.f : ex2(m[n][jj] - use) / Ls;
-        float* row = fl + (n * 8 + qd + jj) * L::kFlushStride + pc * (D / 8);
-#pragma unroll
-        for (int i = 0; i < KS; i += 2)
-          *reinterpret_cast<float4*>(row + 2 * i) =
-              make_float4(acc[n][i][jj] * f, acc[n][i][jj + 2] * f, acc[n][i + 1][jj] * f,
-                          acc[n][i + 1][jj + 2] * f);
-      }
-    if (!seg_whole && w == 0 && lane < nr) {
-      // (read here: past the second meeting a faster warp may be at the next
-      // segment's end)
-      float M = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        M = fmaxf(M, ml[(((head * W + i) * NQ) * 8 + lane) * 2]);
       const float use = M == -INFINITY ? 0.f : M;
-      float Ls = 0.f;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float* p = ml + (((head * W + i) * NQ) * 8 + lane) * 2;
-        Ls += p[1] * ex2(p[0] - use);
-      }
-      a.ws_lse[pslot * nr + lane] = Ls == 0.f ? -INFINITY : use + log2f(Ls) - kPShift;
-    }
-    if (!meet()) return false;
-    const float* f0 = reinterpret_cast<const float*>(smem + L::off_flush) +
-                      head * W * L::kFlushFloats;
-    constexpr int kPer = D / 8;
-    for (int c = w * 32 + lane; c < nr * kPer; c += 32 * W) {
-      const int n = c / kPer, d = (c % kPer) * 8;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float* p = f0 + i * L::kFlushFloats + n * L::kFlushStride + d;
-        const float4 u = *reinterpret_cast<const float4*>(p);
-        const float4 v = *reinterpret_cast<const float4*>(p + 4);
-        x.x += u.x, x.y += u.y, x.z += u.z, x.w += u.w;
-        y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
-      }
-      if (seg_whole) {
-        T* dst = reinterpret_cast<T*>(a.out) + seg_b * a.out_stride +
-                 static_cast<int64_t>(kvh * nr + n) * D + d;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w),
-                                                    pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+      if (WT > 1) {
+#pragma unroll 4
+        for (int i = 0; i < WT; ++i) {
+          const float2 p = ml[(first + i) * 8 + qd + j];
+          Ls += p.y * ex2(p.x - use);
+        }
       } else {
-        float* dst = a.ws_o + (pslot * nr + n) * D + d;
-        *reinterpret_cast<float4*>(dst) = x;
-        *reinterpret_cast<float4*>(dst + 4) = y;
+        Ls = l[j] * ex2(m[j] - use);
+      }
+      // nothing attended: zero (a NaN sum is not nothing)
+      f[j] = Ls == 0.f ? 0.f : ex2(m[j] - use) / Ls;
+      lse[j] = Ls == 0.f ? -INFINITY : use + log2f(Ls) - kPShift;
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      acc[i][0] *= f[0];
+      acc[i][1] *= f[1];
+      acc[i][2] *= f[0];
+      acc[i][3] *= f[1];
+    }
+    // 16-byte pieces of a lane's D / 8 columns, rotated by its rows against bank conflicts
+    float* parts = reinterpret_cast<float*>(smem + L::off_part) + row * (WT / 2) * L::kPart +
+                   qd * D + pc * (D / 8);
+    auto piece = [&](int i) { return ((i / 2) ^ (qq & (D / 32 - 1))) * 4; };
+    int mine = part >= WT / 2 ? part - WT / 2 : part;  // buffer of this warp
+    int step = 1;
+    for (int h = WT / 2; h > 0; h >>= 1, ++step) {
+      if (part >= h) {
+        float* o = parts + mine * L::kPart;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < KS; i += 2)
+            *reinterpret_cast<float4*>(o + j * D + piece(i)) =
+                make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[step]);
+        break;
+      }
+      if (!__all_sync(kFull, mbar_wait_bounded(&bar[step], par))) return false;
+      // warp part + h wrote the buffer it last read: its own place's in the
+      // first step, then the one it read in the step before
+      mine = h == WT / 2 ? part : mine + h;
+      const float* o = parts + mine * L::kPart;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < KS; i += 2) {
+          const float4 x = *reinterpret_cast<const float4*>(o + j * D + piece(i));
+          acc[i][j] += x.x;
+          acc[i][j + 2] += x.y;
+          acc[i + 1][j] += x.z;
+          acc[i + 1][j + 2] += x.w;
+        }
+    }
+    if (part == 0) {
+      const int64_t pslot = static_cast<int64_t>(kvh) * a.ws_slots + seg_unit + seg_b;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + qd + j;
+        if (qd + j >= nq) continue;
+        if (seg_whole) {
+          T* dst = reinterpret_cast<T*>(a.out) + seg_b * a.out_stride +
+                   static_cast<int64_t>(kvh * a.n_rep + n) * D + pc * (D / 8);
+#pragma unroll
+          for (int i = 0; i < KS; i += 4)
+            *reinterpret_cast<uint4*>(dst + 2 * i) =
+                make_uint4(pack2<T>(acc[i][j], acc[i][j + 2]),
+                           pack2<T>(acc[i + 1][j], acc[i + 1][j + 2]),
+                           pack2<T>(acc[i + 2][j], acc[i + 2][j + 2]),
+                           pack2<T>(acc[i + 3][j], acc[i + 3][j + 2]));
+        } else {
+          float* dst = a.ws_o + (pslot * a.n_rep + n) * D + pc * (D / 8);
+#pragma unroll
+          for (int i = 0; i < KS; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) =
+                make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
+          if (grp == 0) a.ws_lse[pslot * a.n_rep + n] = lse[j];
+        }
       }
     }
-    if (W == 1) __syncwarp();
     reset();
     return true;
   };
@@ -483,177 +489,209 @@ __global__ void __launch_bounds__(kThreads, 1)
       seg_unit = it.unit;
       seg_whole = (it.flags & kWhole) != 0;
       const int buf = (it.flags & kQBuf1) ? 1 : 0;
+      const int hr = n0 + grp;  // query head of the group
+      float v[D / 4];
+      float top = 0.f;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        const int hr = n * 8 + grp;  // query head of the group
-        float v[D / 4];
-        float top = 0.f;
+      for (int e = 0; e < D / 4; ++e) v[e] = 0.f;
+      if (hr < a.n_rep) {
+        if (q_bulk) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              smem + L::off_q + buf * L::kQBuf + (head * a.n_rep + hr) * D * 2);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
+          for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[c * 16 + e] = 0.f;
-        if (hr < a.n_rep) {
-          if (q_bulk) {
-            const uint4* src = reinterpret_cast<const uint4*>(
-                smem + L::off_q + buf * L::kQBuf + (head * a.n_rep + hr) * D * 2);
+            for (int u = 0; u < 2; ++u) {
+              const uint4 x = src[(qq + 4 * c) * 2 + u];
+              const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint4 x = src[(qq + 4 * c) * 2 + u];
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 f = unpack2<T>(xs[e]);
-                  v[c * 16 + u * 8 + 2 * e] = f.x;
-                  v[c * 16 + u * 8 + 2 * e + 1] = f.y;
-                }
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<T>(xs[e]);
+                v[c * 16 + u * 8 + 2 * e] = f.x;
+                v[c * 16 + u * 8 + 2 * e + 1] = f.y;
               }
-          } else {
-            const T* src = reinterpret_cast<const T*>(a.q) + it.b * a.q_stride +
-                           static_cast<int64_t>(kvh * a.n_rep + hr) * D;
+            }
+        } else {
+          const T* src = reinterpret_cast<const T*>(a.q) + it.b * a.q_stride +
+                         static_cast<int64_t>(kvh * a.n_rep + hr) * D;
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
+          for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[c * 16 + e] = DT<T>::to_f(src[(qq + 4 * c) * 16 + e]);
-          }
+            for (int e = 0; e < 16; ++e) v[c * 16 + e] = DT<T>::to_f(src[(qq + 4 * c) * 16 + e]);
         }
-#pragma unroll
-        for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(v[e]));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-        // 2^(13 - floor(log2 top)), exponents kept where both factors are normal
-        int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-        ex = ex < -100 ? -100 : (ex > 126 ? 126 : ex);
-        const float up = __uint_as_float(static_cast<uint32_t>(13 - ex + 127) << 23);
-        const float down = __uint_as_float(static_cast<uint32_t>(ex - 13 + 127) << 23);
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          const int o = (i >> 2) * 16 + (i & 3) * 4;
-          qf[n][i][0] = pack2<__half>(v[o] * up, v[o + 1] * up);
-          qf[n][i][1] = pack2<__half>(v[o + 2] * up, v[o + 3] * up);
-        }
-        const float inv = down * a.scale_log2;
-        qinv[n][0] = __shfl_sync(kFull, inv, qd * 4);
-        qinv[n][1] = __shfl_sync(kFull, inv, (qd + 1) * 4);
       }
+#pragma unroll
+      for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(v[e]));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+      // 2^(13 - floor(log2 top)), exponents kept where both factors are normal
+      int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      ex = ex < -100 ? -100 : (ex > 126 ? 126 : ex);
+      const float up = __uint_as_float(static_cast<uint32_t>(13 - ex + 127) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(ex - 13 + 127) << 23);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int o = (i >> 2) * 16 + (i & 3) * 4;
+        qf[i][0] = pack2<__half>(v[o] * up, v[o + 1] * up);
+        qf[i][1] = pack2<__half>(v[o + 2] * up, v[o + 3] * up);
+      }
+      const float inv = down * a.scale_log2;
+      qinv[0] = __shfl_sync(kFull, inv, qd * 4);
+      qinv[1] = __shfl_sync(kFull, inv, (qd + 1) * 4);
       if (q_bulk) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfree[buf]);
       }
     }
-    const int nvalid = ((it.flags >> w) & 1) ? min(kTile, it.ntok - w * kTile) : 0;
-    if (nvalid > 0) {
-      const uint32_t kbase = smem_u32(smem + slot * L::kStage + w * L::kTileBytes) +
-                             head * L::kRegion;
-      const uint32_t vbase = kbase + L::kSide;
-      const float* sc = scales + slot * L::kScales + w * (NB * 2 * HG) + head;
-      // scales of the tile's first and second 8 tokens
-      const float ks0 = sc[0], vs0 = sc[HG];
-      const float ks1 = NB == 2 ? (nvalid > 8 ? sc[2 * HG] : 0.f) : ks0;
-      const float vs1 = NB == 2 ? (nvalid > 8 ? sc[3 * HG] : 0.f) : vs0;
+    // this warp's neighbouring tiles of the item
+    int nv[kPair];
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      const int w = part * kPair + u;
+      nv[u] = ((it.flags >> w) & 1) ? max(0, min(kTile, it.ntok - w * kTile)) : 0;
+    }
+    if (nv[0] | nv[kPair - 1]) {
+      const uint32_t base = smem_u32(smem + slot * L::kStage + part * (kPair * L::kTileBytes)) +
+                            head * L::kRegion;
+      const float* sc = scales + slot * L::kScales + part * (kPair * NB * 2 * HG) + head;
+      // scales of each tile's first and second 8 tokens (0 where there are none)
+      float ks[kPair][2], vs[kPair][2];
+#pragma unroll
+      for (int u = 0; u < kPair; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool any = nv[u] > (NB == 2 ? 8 * i : 0);
+          const float* q = sc + (u * NB + (NB == 2 ? i : 0)) * 2 * HG;
+          ks[u][i] = any ? q[0] : 0.f;
+          vs[u][i] = any ? q[HG] : 0.f;
+        }
 
-      // V codes early: their reads overlap the score product
+      // S^T of both tiles; two accumulators each halve the dependent chain
+      float s[kPair][4], t[kPair][4];
+#pragma unroll
+      for (int u = 0; u < kPair; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] = t[u][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int u = 0; u < kPair; ++u) {
+          const uint32_t kb = base + u * L::kTileBytes + koff[c];
+          const uint4 x = lds128(kb), y = lds128(kb + kHalf);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a0, a1, a2, a3;
+            decode4_h<C>(xs[e], a0, a2);
+            decode4_h<C>(ys[e], a1, a3);
+            mma_16816<__half>((e & 1) ? t[u] : s[u], a0, a1, a2, a3, qf[c * 4 + e][0],
+                              qf[c * 4 + e][1]);
+          }
+        }
+
+      // V codes: their reads overlap the softmax
       constexpr int VW = D / 32;  // words per lane and token
-      uint32_t vw[4][VW];
-      {
-        const uint32_t at[4] = {vbase + va, vbase + vb, vbase + kHalf + va, vbase + kHalf + vb};
+      uint32_t vw[kPair][4][VW];
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) {
+        const uint32_t vb0 = base + u * L::kTileBytes + L::kSide;
+        const uint32_t at[4] = {vb0 + va, vb0 + vb, vb0 + kHalf + va, vb0 + kHalf + vb};
+        const int tk[4] = {ta, tb, ta + 8, tb + 8};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (D == 128) {
             const uint4 x = lds128(at[i]);
-            vw[i][0] = x.x, vw[i][1] = x.y, vw[i][2] = x.z, vw[i][3] = x.w;
+            vw[u][i][0] = x.x, vw[u][i][1] = x.y, vw[u][i][2] = x.z, vw[u][i][3] = x.w;
           } else {
             const uint2 x = lds64(at[i]);
-            vw[i][0] = x.x, vw[i][1] = x.y;
+            vw[u][i][0] = x.x, vw[u][i][1] = x.y;
           }
         }
-        if (nvalid < kTile) {
+        if (nv[u] < kTile) {
           // rows past the context may hold NaN codes, and 0 * NaN is NaN
-          const int tk[4] = {ta, tb, ta + 8, tb + 8};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (tk[i] >= nvalid) {
+            if (tk[i] >= nv[u]) {
 #pragma unroll
-              for (int e = 0; e < VW; ++e) vw[i][e] = 0u;
+              for (int e = 0; e < VW; ++e) vw[u][i][e] = 0u;
             }
         }
       }
 
-      float s[NQ][4];
+      // scores in log2 units (registers of s), [tile][half * 2 + head column]
+      float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int u = 0; u < kPair; ++u) {
+        const bool v0 = tg < nv[u], v1 = tg + 8 < nv[u];
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const uint4 x = lds128(kbase + koff[c]), y = lds128(kbase + kHalf + koff[c]);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t a0, a1, a2, a3;
-          decode4_h<C>(xs[e], a0, a2);
-          decode4_h<C>(ys[e], a1, a3);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-            mma_16816<__half>(s[n], a0, a1, a2, a3, qf[n][c * 4 + e][0], qf[n][c * 4 + e][1]);
+        for (int j = 0; j < 2; ++j) {
+          s[u][j] = v0 ? (s[u][j] + t[u][j]) * (qinv[j] * ks[u][0]) : -INFINITY;
+          s[u][j + 2] = v1 ? (s[u][j + 2] + t[u][j + 2]) * (qinv[j] * ks[u][1]) : -INFINITY;
+          mx[j] = max3(mx[j], s[u][j], s[u][j + 2]);
         }
       }
-
-      const bool v0 = tg < nvalid, v1 = tg + 8 < nvalid;
-      uint32_t pb0[NQ], pb1[NQ];
-      float alpha[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float p[4];
+      for (int j = 0; j < 2; ++j) {
+        mx[j] = fmaxf(mx[j], __shfl_xor_sync(kFull, mx[j], 4));
+        mx[j] = fmaxf(mx[j], __shfl_xor_sync(kFull, mx[j], 8));
+        mx[j] = fmaxf(mx[j], __shfl_xor_sync(kFull, mx[j], 16));
+      }
+      const bool up0 = mx[0] > m[0] + kSlack, up1 = mx[1] > m[1] + kSlack;
+      if (__any_sync(kFull, up0 || up1)) {
+        const float a0 = up0 ? ex2(m[0] - mx[0]) : 1.f, a1 = up1 ? ex2(m[1] - mx[1]) : 1.f;
+        if (up0) m[0] = mx[0];
+        if (up1) m[1] = mx[1];
+        l[0] *= a0;
+        l[1] *= a1;
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          const float s0 = v0 ? s[n][jj] * (qinv[n][jj] * ks0) : -INFINITY;
-          const float s1 = v1 ? s[n][jj + 2] * (qinv[n][jj] * ks1) : -INFINITY;
-          float mx = fmaxf(s0, s1);
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-          const float mnew = fmaxf(m[n][jj], mx);
-          const float muse = (mnew == -INFINITY) ? 0.f : mnew;
-          alpha[n][jj] = ex2(m[n][jj] - muse);
-          p[jj] = ex2(s0 - muse + kPShift);
-          p[jj + 2] = ex2(s1 - muse + kPShift);
-          l[n][jj] = l[n][jj] * alpha[n][jj] + p[jj] + p[jj + 2];
-          m[n][jj] = mnew;
+        for (int i = 0; i < KS; ++i) {
+          acc[i][0] *= a0;
+          acc[i][1] *= a1;
+          acc[i][2] *= a0;
+          acc[i][3] *= a1;
         }
-        pb0[n] = movmatrix_trans(pack2<__half>(p[0], p[1]));
-        pb1[n] = movmatrix_trans(pack2<__half>(p[2], p[3]));
+      }
+      const float r0 = kPShift - (m[0] == -INFINITY ? 0.f : m[0]);
+      const float r1 = kPShift - (m[1] == -INFINITY ? 0.f : m[1]);
+      uint32_t pb[kPair][2];
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) {
+        const float p0 = ex2(s[u][0] + r0), p1 = ex2(s[u][1] + r1);
+        const float p2 = ex2(s[u][2] + r0), p3 = ex2(s[u][3] + r1);
+        l[0] += p0 + p2;
+        l[1] += p1 + p3;
+        pb[u][0] = movmatrix_trans(pack2<__half>(p0, p1));
+        pb[u][1] = movmatrix_trans(pack2<__half>(p2, p3));
       }
 
-      // O^T = O^T * alpha + vs * (V^T . P^T)
+      // O^T += vs * (V^T . P^T)
+      auto add = [&](float* o, const float* x, float v) {
+        const unsigned long long v2 = f2pack(v, v);
+        const float2 y = f2unpack(fma2(v2, f2pack(x[0], x[1]), f2pack(o[0], o[1])));
+        const float2 z = f2unpack(fma2(v2, f2pack(x[2], x[3]), f2pack(o[2], o[3])));
+        o[0] = y.x, o[1] = y.y, o[2] = z.x, o[3] = z.y;
+      };
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        uint32_t a0[2], a1[2], a2[2], a3[2];
-        decode4_h<C>(__byte_perm(vw[0][e], vw[1][e], 0x5140), a0[0], a1[0]);
-        decode4_h<C>(__byte_perm(vw[0][e], vw[1][e], 0x7362), a0[1], a1[1]);
-        decode4_h<C>(__byte_perm(vw[2][e], vw[3][e], 0x5140), a2[0], a3[0]);
-        decode4_h<C>(__byte_perm(vw[2][e], vw[3][e], 0x7362), a2[1], a3[1]);
+      for (int e = 0; e < VW; ++e)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kPair; ++u) {
+          uint32_t a0[2], a1[2], a2[2], a3[2];
+          decode4_h<C>(__byte_perm(vw[u][0][e], vw[u][1][e], 0x5140), a0[0], a1[0]);
+          decode4_h<C>(__byte_perm(vw[u][0][e], vw[u][1][e], 0x7362), a0[1], a1[1]);
+          decode4_h<C>(__byte_perm(vw[u][2][e], vw[u][3][e], 0x5140), a2[0], a3[0]);
+          decode4_h<C>(__byte_perm(vw[u][2][e], vw[u][3][e], 0x7362), a2[1], a3[1]);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            float* o = acc[n][2 * e + u];
-            if (NB == 1) {
-              float x[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_16816<__half>(x, a0[u], a1[u], a2[u], a3[u], pb0[n], pb1[n]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] = fmaf(vs0, x[i], o[i] * alpha[n][i & 1]);
-            } else {
-              // two blocks: their products apart
-              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_16816<__half>(x, a0[u], a1[u], a2[u], a3[u], pb0[n], 0u);
-              mma_16816<__half>(y, a0[u], a1[u], a2[u], a3[u], 0u, pb1[n]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                o[i] = fmaf(vs1, y[i], fmaf(vs0, x[i], o[i] * alpha[n][i & 1]));
+          for (int i = 0; i < 2; ++i) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816<__half>(x, a0[i], a1[i], a2[i], a3[i], pb[u][0], NB == 1 ? pb[u][1] : 0u);
+            add(acc[2 * e + i], x, vs[u][0]);
+            if (NB == 2) {  // two blocks: their products apart
+              float y[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_16816<__half>(y, a0[i], a1[i], a2[i], a3[i], 0u, pb[u][1]);
+              add(acc[2 * e + i], y, vs[u][1]);
             }
           }
         }
-      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[slot]);
@@ -669,13 +707,12 @@ struct CallQ8 {
   cudaStream_t s;
 };
 
-template <typename T, typename C, int D, int HG, int R, int NQ>
+template <typename T, typename C, int D, int HG, int R, bool SETS>
 int run_q8(const CallQ8* call) {
-  constexpr int NS = stages_q8<D, HG, R, NQ>();
-  using L = LayoutQ8<D, HG, R, NS, NQ>;
-  static_assert(L::kAlloc <= 227 * 1024, "shared memory budget");
-  static_assert(NQ * 8 * 2 <= 32, "one lane per query head of a group");
-  auto kern = decode_q8_kernel<T, C, D, HG, R, NQ, NS>;
+  constexpr int NS = stages_q8<D, HG, R, SETS>();
+  using L = LayoutQ8<D, HG, R, NS, SETS>;
+  static_assert(L::kAlloc <= 227 * 1024 && NS >= 3, "shared memory budget");
+  auto kern = decode_q8_kernel<T, C, D, HG, R, SETS, NS>;
   cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -693,25 +730,25 @@ int run_q8(const CallQ8* call) {
       cudaLaunchKernelEx(&cfg, kern, *call->tmk, *call->tmv, *call->a, call->q_bulk));
 }
 
-template <typename T, typename C, int D, int HG, int NQ>
+template <typename T, typename C, int D, int HG, bool SETS>
 int by_rows(const CallQ8* c) {
-  return c->a->bs == 8 ? run_q8<T, C, D, HG, 8, NQ>(c) : run_q8<T, C, D, HG, 16, NQ>(c);
+  return c->a->bs == 8 ? run_q8<T, C, D, HG, 8, SETS>(c) : run_q8<T, C, D, HG, 16, SETS>(c);
 }
 template <typename T, typename C, int D>
 int by_heads(const CallQ8* c) {
   const int hg = q8_head_group(c->a->Hkv, c->a->n_rep);
   if (c->a->n_rep <= 8) {
     switch (hg) {
-      case 1: return by_rows<T, C, D, 1, 1>(c);
-      case 2: return by_rows<T, C, D, 2, 1>(c);
-      case 4: return by_rows<T, C, D, 4, 1>(c);
-      default: return by_rows<T, C, D, 8, 1>(c);
+      case 1: return by_rows<T, C, D, 1, false>(c);
+      case 2: return by_rows<T, C, D, 2, false>(c);
+      case 4: return by_rows<T, C, D, 4, false>(c);
+      default: return by_rows<T, C, D, 8, false>(c);
     }
   }
   switch (hg) {
-    case 1: return by_rows<T, C, D, 1, 2>(c);
-    case 2: return by_rows<T, C, D, 2, 2>(c);
-    default: return by_rows<T, C, D, 4, 2>(c);
+    case 1: return by_rows<T, C, D, 1, true>(c);
+    case 2: return by_rows<T, C, D, 2, true>(c);
+    default: return by_rows<T, C, D, 4, true>(c);
   }
 }
 template <typename T, typename C>

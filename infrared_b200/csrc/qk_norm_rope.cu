@@ -46,8 +46,46 @@ __device__ __forceinline__ void store_row4(T* p, float4 v) {
   }
 }
 
-// A group of D / 8 lanes takes heads [y * hpg, y * hpg + hpg) of one token;
-// heads 0 .. H-1 are the query's, the rest the key's.
+// Heads of one token by a group of D / 8 lanes, kBatch at a time: their loads
+// are all in flight before the first sum.
+constexpr int kBatch = 4;
+
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void norm_heads(const T* src, T* dst, int h0, int h1, float4 w0,
+                                           float4 w1, float4 c0, float4 c1, float4 s0, float4 s1,
+                                           float eps, int lo, int hi, bool live) {
+  for (int h = h0; h < h1; h += kBatch) {
+    float4 x[kBatch], y[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int hh = min(h + i, h1 - 1);
+      x[i] = load_row4<T, VEC>(src + hh * D + lo);
+      y[i] = load_row4<T, VEC>(src + hh * D + hi);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      float ss = x[i].x * x[i].x + x[i].y * x[i].y + x[i].z * x[i].z + x[i].w * x[i].w +
+                 y[i].x * y[i].x + y[i].y * y[i].y + y[i].z * y[i].z + y[i].w * y[i].w;
+#pragma unroll
+      for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss * (1.f / D) + eps);
+      const float4 u = make_float4(x[i].x * r * w0.x, x[i].y * r * w0.y, x[i].z * r * w0.z,
+                                   x[i].w * r * w0.w);
+      const float4 v = make_float4(y[i].x * r * w1.x, y[i].y * r * w1.y, y[i].z * r * w1.z,
+                                   y[i].w * r * w1.w);
+      if (live && h + i < h1) {
+        T* o = dst + (h + i) * D;
+        store_row4<T, VEC>(o + lo, make_float4(u.x * c0.x - v.x * s0.x, u.y * c0.y - v.y * s0.y,
+                                               u.z * c0.z - v.z * s0.z, u.w * c0.w - v.w * s0.w));
+        store_row4<T, VEC>(o + hi, make_float4(v.x * c1.x + u.x * s1.x, v.y * c1.y + u.y * s1.y,
+                                               v.z * c1.z + u.z * s1.z, v.w * c1.w + u.w * s1.w));
+      }
+    }
+  }
+}
+
+// Grid: tokens (x) and pieces of hpg heads (y); heads 0 .. H-1 are the
+// query's, the rest the key's.
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRopeArgs a) {
   constexpr int LPR = D / 8;
@@ -56,45 +94,28 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
   const bool live = t < a.n;
   const int64_t tok = live ? t : a.n - 1;  // idle groups follow along for the shuffles
   const int lo = lane * 4, hi = D / 2 + lane * 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float* cr = a.cos + tok * a.rope_stride;
   const float* sr = a.sin + tok * a.rope_stride;
   const float4 c0 = load_row4<float, VEC>(cr + lo), c1 = load_row4<float, VEC>(cr + hi);
   const float4 s0 = load_row4<float, VEC>(sr + lo), s1 = load_row4<float, VEC>(sr + hi);
   const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
-  const T* wq = static_cast<const T*>(a.w_q);
-  const T* wk = static_cast<const T*>(a.w_k);
   const int h0 = blockIdx.y * a.hpg;
   const int h1 = min(h0 + a.hpg, a.H + a.Hkv);
-  float4 w0 = one, w1 = one;
-  bool key = false;
-  if (wq) w0 = load_row4<T, VEC>(wq + lo), w1 = load_row4<T, VEC>(wq + hi);
-  for (int h = h0; h < h1; ++h) {
-    if (h >= a.H && !key) {
-      key = true;
-      w0 = w1 = one;
-      if (wk) w0 = load_row4<T, VEC>(wk + lo), w1 = load_row4<T, VEC>(wk + hi);
+  auto side = [&](const void* src, int64_t stride, void* dst, int64_t out_stride, const void* w,
+                  int from, int to) {
+    float4 w0 = one, w1 = one;
+    if (w) {
+      w0 = load_row4<T, VEC>(static_cast<const T*>(w) + lo);
+      w1 = load_row4<T, VEC>(static_cast<const T*>(w) + hi);
     }
-    const T* src = h < a.H ? static_cast<const T*>(a.q) + tok * a.q_stride + h * D
-                           : static_cast<const T*>(a.k) + tok * a.k_stride + (h - a.H) * D;
-    const float4 x = load_row4<T, VEC>(src + lo), y = load_row4<T, VEC>(src + hi);
-    float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y +
-               y.z * y.z + y.w * y.w;
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss * (1.f / D) + a.eps);
-    const float4 u = make_float4(x.x * r * w0.x, x.y * r * w0.y, x.z * r * w0.z, x.w * r * w0.w);
-    const float4 v = make_float4(y.x * r * w1.x, y.y * r * w1.y, y.z * r * w1.z, y.w * r * w1.w);
-    if (live) {
-      T* dst = h < a.H ? static_cast<T*>(a.q_out) + tok * a.qo_stride + h * D
-                       : static_cast<T*>(a.k_out) + tok * a.ko_stride + (h - a.H) * D;
-      store_row4<T, VEC>(dst + lo,
-                         make_float4(u.x * c0.x - v.x * s0.x, u.y * c0.y - v.y * s0.y,
-                                     u.z * c0.z - v.z * s0.z, u.w * c0.w - v.w * s0.w));
-      store_row4<T, VEC>(dst + hi,
-                         make_float4(v.x * c1.x + u.x * s1.x, v.y * c1.y + u.y * s1.y,
-                                     v.z * c1.z + u.z * s1.z, v.w * c1.w + u.w * s1.w));
-    }
-  }
+    norm_heads<T, D, VEC>(static_cast<const T*>(src) + tok * stride,
+                          static_cast<T*>(dst) + tok * out_stride, from, to, w0, w1, c0, c1, s0,
+                          s1, a.eps, lo, hi, live);
+  };
+  if (h0 < a.H) side(a.q, a.q_stride, a.q_out, a.qo_stride, a.w_q, h0, min(h1, a.H));
+  if (h1 > a.H)
+    side(a.k, a.k_stride, a.k_out, a.ko_stride, a.w_k, max(h0, a.H) - a.H, h1 - a.H);
 }
 
 template <typename T, int D>
@@ -102,14 +123,21 @@ int launch_norm_t(const NormRopeArgs& a, int vec, int sms, cudaStream_t s) {
   constexpr int kTok = kNormThreads / (D / 8);  // tokens per CTA
   const int64_t gx = (a.n + kTok - 1) / kTok;
   const int heads = a.H + a.Hkv;
+  // pieces of heads: whole tokens where these fill the GPU, else one batch
   NormRopeArgs b = a;
-  b.hpg = heads;
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>((heads + b.hpg - 1) / b.hpg));
-  if (vec)
-    qk_norm_rope_kernel<T, D, true><<<grid, kNormThreads, 0, s>>>(b);
-  else
-    qk_norm_rope_kernel<T, D, false><<<grid, kNormThreads, 0, s>>>(b);
-  return static_cast<int>(cudaGetLastError());
+  b.hpg = gx >= 2 * sms ? heads : kBatch;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(gx),
+                     static_cast<unsigned>((heads + b.hpg - 1) / b.hpg));
+  cfg.blockDim = dim3(kNormThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(
+      &cfg, vec ? qk_norm_rope_kernel<T, D, true> : qk_norm_rope_kernel<T, D, false>, b));
 }
 
 template <typename T>
