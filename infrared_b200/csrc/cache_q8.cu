@@ -25,6 +25,10 @@ constexpr int kQWarps = kQThreads / 32;
 constexpr int64_t kScanTokens = 1024;
 constexpr unsigned kAll = 0xffffffffu;
 
+// The next grid of the stream may be set up now / wait for the one before.
+__device__ __forceinline__ void let_next_grid_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void wait_prior_grid() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -73,61 +77,84 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Four elements of a row, as loaded.
-template <typename T> struct Four {
-  uint2 w;
+// Eight elements of a row, as loaded.
+template <typename T> struct Eight {
+  uint4 w;
   template <bool VEC>
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (VEC) {
-      w = *reinterpret_cast<const uint2*>(p);
+      w = *reinterpret_cast<const uint4*>(p);
     } else {
       const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-      w = make_uint2(u[0] | (static_cast<uint32_t>(u[1]) << 16),
-                     u[2] | (static_cast<uint32_t>(u[3]) << 16));
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = u[2 * i] | (static_cast<uint32_t>(u[2 * i + 1]) << 16);
+      w = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
   // Running maximum of the magnitudes, two halves side by side; NaN stays.
   __device__ __forceinline__ uint32_t top(uint32_t m) const {
-    return max2<T>(m, max2<T>(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu));
-  }
-  __device__ __forceinline__ float4 value() const {
-    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-    return make_float4(a.x, a.y, b.x, b.y);
+    return max2<T>(max2<T>(m, max2<T>(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu)),
+                   max2<T>(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
   }
   static __device__ __forceinline__ float magnitude(uint32_t m) {
-    const float2 t = unpack2<T>(max2<T>(m, m >> 16));
-    return t.x;
+    return unpack2<T>(max2<T>(m, m >> 16)).x;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<T>(u[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
   }
 };
-template <> struct Four<float> {
-  float4 v;
+template <> struct Eight<float> {
+  float4 a, b;
   template <bool VEC>
   __device__ __forceinline__ void load(const float* p) {
-    if constexpr (VEC)
-      v = *reinterpret_cast<const float4*>(p);
-    else
-      v = make_float4(p[0], p[1], p[2], p[3]);
+    if constexpr (VEC) {
+      a = reinterpret_cast<const float4*>(p)[0];
+      b = reinterpret_cast<const float4*>(p)[1];
+    } else {
+      a = make_float4(p[0], p[1], p[2], p[3]);
+      b = make_float4(p[4], p[5], p[6], p[7]);
+    }
   }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  // (the magnitudes' bits are in the order of the magnitudes, NaN above all)
   __device__ __forceinline__ uint32_t top(uint32_t m) const {
-    const uint32_t a = max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu);
-    const uint32_t b = max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu);
-    return max(m, max(a, b));
+    float v[8];
+    values(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
   }
-  __device__ __forceinline__ float4 value() const { return v; }
   static __device__ __forceinline__ float magnitude(uint32_t m) { return __uint_as_float(m); }
 };
 
+template <typename C>
+__device__ __forceinline__ uint2 encode8(const float (&v)[8]) {
+  return make_uint2(encode4<C>(make_float4(v[0], v[1], v[2], v[3])),
+                    encode4<C>(make_float4(v[4], v[5], v[6], v[7])));
+}
+
 // One (side, kv head) of block `blk`, by one warp. Lanes cover D in groups of
-// 4 elements, 128 / D rows at a time, 16 such passes at once. src(r) is called
-// by all lanes of the warp together.
+// 8 elements, 256 / D rows at a time, kPass such passes at once. src(r) is
+// called by all lanes of the warp together.
 template <typename T, typename C, bool VEC, typename Src>
-__device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int side, int h) {
+__device__ __forceinline__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int side,
+                                              int h) {
   constexpr bool kInt = std::is_same<C, int8_t>::value;
-  constexpr int kPass = 16;
+  constexpr int kPass = 8;
   const int lane = threadIdx.x & 31;
-  const bool wide = a.D == 128;  // 32 lanes per row, else 16
-  const int rp = wide ? 1 : 2;   // rows per pass
-  const int sub = wide ? 0 : lane >> 4, col = (wide ? lane : lane & 15) * 4;
+  const int sh = a.D == 128 ? 4 : 3;  // log2 of the lanes per row
+  const int rp = 32 >> sh;            // rows per pass
+  const int sub = lane >> sh, col = (lane & ((1 << sh) - 1)) * 8;
   const T* in = reinterpret_cast<const T*>(a.src[side]) + h * a.D + col;
   const int stride = a.stride[side];
   const int row_bytes = a.Hkv * a.D;  // (a block's bytes stay below 2^31)
@@ -142,7 +169,7 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
     some = max(some, src(base + lane < a.bs ? base + lane : 0));
   some = __reduce_max_sync(kAll, some);
 
-  Four<T> x[kPass];
+  Eight<T> x[kPass];
   uint32_t have = 0;  // bit u: pass u of the rows in registers is a new row
   auto load = [&](int base) {
     have = 0;
@@ -164,7 +191,7 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
 #pragma unroll
     for (int u = 0; u < kPass; ++u) m = x[u].top(m);
   }
-  float amax = Four<T>::magnitude(m);
+  float amax = Eight<T>::magnitude(m);
   const bool bad = __any_sync(kAll, !finite(amax));
   if (bad) {  // the largest finite one
     amax = 0.f;
@@ -172,16 +199,16 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
       load(base);
 #pragma unroll
       for (int u = 0; u < kPass; ++u) {
-        const float4 f = x[u].value();
-        const float v[4] = {f.x, f.y, f.z, f.w};
+        float v[8];
+        x[u].values(v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
           if (finite(v[i])) amax = fmaxf(amax, fabsf(v[i]));
       }
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, o));
+  // (bits of magnitudes are in their order)
+  amax = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(amax)));
 
   const float old = begun ? 0.f : before;
   const float need = scale_for<C>(amax);
@@ -199,13 +226,12 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
       const int r = base + sub;
       const int t = src(r < a.bs ? r : 0);
       if (r >= a.bs || t >= 0) continue;
-      uint32_t* p = reinterpret_cast<uint32_t*>(dst + r * row_bytes);
-      float4 f = decode4<C>(*p);
-      f.x *= ratio;
-      f.y *= ratio;
-      f.z *= ratio;
-      f.w *= ratio;
-      *p = encode4<C>(f);
+      uint2* p = reinterpret_cast<uint2*>(dst + r * row_bytes);
+      const uint2 c = *p;
+      const float4 f = decode4<C>(c.x), g = decode4<C>(c.y);
+      const float v[8] = {f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio,
+                          g.x * ratio, g.y * ratio, g.z * ratio, g.w * ratio};
+      *p = encode8<C>(v);
     }
   }
   if (!bad && inv != 0.f) {
@@ -215,9 +241,12 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
       uint8_t* row = dst + (base + sub) * row_bytes;
 #pragma unroll
       for (int u = 0; u < kPass; ++u) {
-        const float4 f = x[u].value();
-        const uint32_t c = encode4<C>(make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv));
-        if ((have >> u) & 1u) *reinterpret_cast<uint32_t*>(row + u * rp * row_bytes) = c;
+        float v[8];
+        x[u].values(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= inv;
+        const uint2 c = encode8<C>(v);
+        if ((have >> u) & 1u) *reinterpret_cast<uint2*>(row + u * rp * row_bytes) = c;
       }
     }
     return;
@@ -227,12 +256,13 @@ __device__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int si
     const int r = base + sub;
     const int t = src(r < a.bs ? r : 0);
     if (r >= a.bs || t < 0) continue;
-    Four<T> one;
+    Eight<T> one;
     one.template load<VEC>(in + static_cast<int64_t>(t) * stride);
-    const float4 f = one.value();
-    *reinterpret_cast<uint32_t*>(dst + r * row_bytes) =
-        encode4<C>(make_float4(finite(f.x) ? f.x / now : nan, finite(f.y) ? f.y / now : nan,
-                               finite(f.z) ? f.z / now : nan, finite(f.w) ? f.w / now : nan));
+    float v[8];
+    one.values(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] / now : nan;
+    *reinterpret_cast<uint2*>(dst + r * row_bytes) = encode8<C>(v);
   }
 }
 
@@ -258,7 +288,7 @@ __global__ void __launch_bounds__(kQThreads) write_scan_kernel(const Q8WriteArgs
     if (threadIdx.x == 0 && blockIdx.y == 0) set_err(a.err, IR_DEVERR_SLOT);
     return;
   }
-  const int64_t blk = s / a.bs, lo = blk * a.bs;
+  const int64_t blk = static_cast<uint32_t>(s) / a.bs, lo = blk * a.bs;
   const int64_t near = before - lo;
   if (near >= 0 && near < a.bs) return;  // its neighbour or an earlier token owns the block
   for (int r = threadIdx.x; r < a.bs; r += kQThreads) src[r] = -1;
@@ -291,27 +321,50 @@ struct Q8Links {
   int* owners;
 };
 
-__global__ void link_runs_kernel(const int64_t* slots, int64_t n, int64_t num_slots, int bs,
-                                 const Q8Links l, int32_t* err) {
+// (a kernel rather than a memset, so that the three grids can overlap their
+// starts: 32768 rows 29.2 us from 29.9)
+__global__ void zero_kernel(int* p, int n) {
+  let_next_grid_start();
   wait_prior_grid();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t s = slots[i];
-  const int64_t p = i > 0 ? slots[i - 1] : -1;
-  if (s < 0) return;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
+}
+
+__global__ void __launch_bounds__(kQThreads)
+    link_runs_kernel(const int64_t* slots, int64_t n, int64_t num_slots, int bs, const Q8Links l,
+                     int32_t* err) {
+  __shared__ int found[kQWarps], base;
+  let_next_grid_start();
+  wait_prior_grid();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kQThreads + threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t s = i < n ? slots[i] : -1;
+  const int64_t p = i > 0 && i < n ? slots[i - 1] : -1;
+  bool owner = false;
   if (s >= num_slots) {
     set_err(err, IR_DEVERR_SLOT);
-    return;
+  } else if (s >= 0) {
+    const int64_t blk = static_cast<uint32_t>(s) / bs;
+    const int64_t off = p - blk * bs;
+    if (off < 0 || off >= bs) {  // the first of its run
+      const int prev = atomicExch(&l.head[blk], static_cast<int>(i) + 1);
+      l.next[i] = prev;
+      owner = prev == 0;
+      if (!owner) atomicAdd(l.count + 1, 1);
+    }
   }
-  const int64_t blk = s / bs;
-  const int64_t off = p - blk * bs;
-  if (off >= 0 && off < bs) return;  // not the first of its run
-  const int prev = atomicExch(&l.head[blk], static_cast<int>(i) + 1);
-  l.next[i] = prev;
-  if (prev == 0)
-    l.owners[atomicAdd(l.count, 1)] = static_cast<int>(i);
-  else
-    atomicAdd(l.count + 1, 1);
+  // one addition to the common count per CTA
+  const unsigned m = __ballot_sync(kAll, owner);
+  if (lane == 0) found[warp] = __popc(m);
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kQWarps; ++w) {
+    before += w < warp ? found[w] : 0;
+    all += found[w];
+  }
+  if (threadIdx.x == 0 && all > 0) base = atomicAdd(l.count, all);
+  __syncthreads();
+  if (owner) l.owners[base + before + __popc(m & ((1u << lane) - 1u))] = static_cast<int>(i);
 }
 
 // Calls f(in, offset, token) for the rows of the run that starts at `first`,
@@ -339,7 +392,7 @@ __device__ __forceinline__ void walk_runs(const Q8WriteArgs& a, const Q8Links& l
 // Blocks of up to 32 rows: every warp takes a task of its own, lane r holding
 // the token of row r.
 template <typename T, typename C, bool VEC>
-__global__ void __launch_bounds__(kQThreads) write_runs_kernel(const Q8WriteArgs a,
+__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 3 : 2) write_runs_kernel(const Q8WriteArgs a,
                                                                const Q8Links l) {
   __shared__ int rows[kQWarps][32];
   wait_prior_grid();
@@ -348,25 +401,44 @@ __global__ void __launch_bounds__(kQThreads) write_runs_kernel(const Q8WriteArgs
   const int tasks = 2 * a.Hkv, warps = gridDim.x * kQWarps;
   const int w = blockIdx.x * kQWarps + warp;
   const int step = warps / tasks, task = w % tasks;
+  const int tside = task / a.Hkv, thead = task - tside * a.Hkv;
   const int count = w / tasks < step ? l.count[0] : 0;
   const bool others = l.count[1] != 0;
   int o = w / tasks;
-  int next = o < count ? l.owners[o] : 0;
+  // the next block's first token and slots arrive during the current task
+  int first = o < count ? l.owners[o] : 0;
+  int next = step < count - o ? l.owners[o + step] : 0;
+  auto slots_from = [&](int f) { return f + lane < a.n ? a.slots[f + lane] : -1; };
+  int64_t mine = slots_from(first);
   for (; o < count; o += step) {
-    const int first = next;
-    if (step < count - o) next = l.owners[o + step];  // (arrives during this task)
-    const int64_t s0 = a.slots[first];
-    const int64_t blk = (s0 >> 31) ? s0 / a.bs : static_cast<uint32_t>(s0) / a.bs;
-    rows[warp][lane] = -1;
-    __syncwarp();
-    walk_runs(a, l, blk, others, first, [&](bool in, int off, int j) {
-      if (in) atomicMax(&rows[warp][off], j);
-    });
-    __syncwarp();
-    const int mine = rows[warp][lane];
-    __syncwarp();
-    quantise_task<T, C, VEC>(a, blk, [&](int r) { return __shfl_sync(kAll, mine, r); },
-                             task / a.Hkv, task % a.Hkv);
+    const int64_t coming = slots_from(next);
+    const int after = 2 * step < count - o ? l.owners[o + 2 * step] : 0;
+    const uint32_t s0 = static_cast<uint32_t>(__shfl_sync(kAll, mine, 0));
+    const int64_t blk = s0 / a.bs;
+    const int64_t off = mine - blk * a.bs;
+    // the run: up to its first token of another block
+    const unsigned in = __ballot_sync(kAll, off >= 0 && off < a.bs);
+    const int len = in == kAll ? 32 : __ffs(~in) - 1;
+    const int off0 = __shfl_sync(kAll, static_cast<int>(off), 0);
+    int row;  // token of row `lane`, or -1
+    if (!others && len < 32 && __all_sync(kAll, lane >= len || off == off0 + lane)) {
+      // rows in order
+      row = lane >= off0 && lane < off0 + len ? first + lane - off0 : -1;
+    } else {
+      rows[warp][lane] = -1;
+      __syncwarp();
+      walk_runs(a, l, blk, others, first, [&](bool hit, int r, int j) {
+        if (hit) atomicMax(&rows[warp][r], j);
+      });
+      __syncwarp();
+      row = rows[warp][lane];
+      __syncwarp();
+    }
+    quantise_task<T, C, VEC>(a, blk, [&](int r) { return __shfl_sync(kAll, row, r); }, tside,
+                             thead);
+    first = next;
+    next = after;
+    mine = coming;
   }
 }
 
@@ -381,7 +453,7 @@ __global__ void __launch_bounds__(kQThreads) write_blocks_kernel(const Q8WriteAr
   const int warp = threadIdx.x >> 5;
   for (int o = blockIdx.x; o < count; o += gridDim.x) {
     const int first = l.owners[o];
-    const int64_t blk = a.slots[first] / a.bs;
+    const int64_t blk = static_cast<uint32_t>(a.slots[first]) / a.bs;
     for (int r = threadIdx.x; r < a.bs; r += kQThreads) src[r] = -1;
     __syncthreads();
     if (warp == 0)
@@ -399,98 +471,105 @@ __global__ void __launch_bounds__(kQThreads) write_blocks_kernel(const Q8WriteAr
 // Finite values beyond T's range saturate.
 template <typename T>
 __device__ __forceinline__ float saturate(float x) {
-  if constexpr (std::is_same<T, __half>::value) {
-    if (fabsf(x) > 65504.f && finite(x)) return copysignf(65504.f, x);
-  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const float top = __uint_as_float(0x7f7f0000u);
-    if (fabsf(x) > top && finite(x)) return copysignf(top, x);
-  }
+  // (a code times a scale is finite or NaN unless the scale is not; min and
+  // max would turn NaN into a number, the comparison keeps it)
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  const float top = kHalf ? 65504.f : __uint_as_float(0x7f7f0000u);
+  if constexpr (sizeof(T) == 2) return fabsf(x) > top && finite(x) ? copysignf(top, x) : x;
   return x;
 }
 
-// 8 codes to 8 values of T, multiplied by the scale in fp32 and rounded once.
+// 8 codes to 8 values of T, likewise (out 16-byte aligned).
 template <typename T, typename C>
-__device__ __forceinline__ void store8(T* out, uint2 codes, float s, int vec) {
+__device__ __forceinline__ void store8(T* out, uint2 codes, float s) {
+  const float4 f = decode4<C>(codes.x), g = decode4<C>(codes.y);
+  const float v[8] = {saturate<T>(f.x * s), saturate<T>(f.y * s), saturate<T>(f.z * s),
+                      saturate<T>(f.w * s), saturate<T>(g.x * s), saturate<T>(g.y * s),
+                      saturate<T>(g.z * s), saturate<T>(g.w * s)};
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
+}
+
+// 16 codes to 16 values of T, multiplied by the scale in fp32 and rounded once.
+template <typename T, typename C>
+__device__ __forceinline__ void store16(T* out, uint4 codes, float s, int vec) {
   constexpr float kLargest = std::is_same<C, int8_t>::value ? 127.f : 448.f;
   constexpr float kTop = std::is_same<T, __half>::value ? 65504.f : 3.38e38f;
-  float4 f[2] = {decode4<C>(codes.x), decode4<C>(codes.y)};
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) f[i] = make_float4(f[i].x * s, f[i].y * s, f[i].z * s, f[i].w * s);
+  for (int i = 0; i < 4; ++i) {
+    const float4 f = decode4<C>(w[i]);
+    v[4 * i] = f.x * s, v[4 * i + 1] = f.y * s, v[4 * i + 2] = f.z * s, v[4 * i + 3] = f.w * s;
+  }
   if (sizeof(T) == 2 && fabsf(s) > kTop / kLargest) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      f[i] = make_float4(saturate<T>(f[i].x), saturate<T>(f[i].y), saturate<T>(f[i].z),
-                         saturate<T>(f[i].w));
+    for (int i = 0; i < 16; ++i) v[i] = saturate<T>(v[i]);
   }
   if (!vec) {
-    const float v[8] = {f[0].x, f[0].y, f[0].z, f[0].w, f[1].x, f[1].y, f[1].z, f[1].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = DT<T>::from_f(v[i]);
+    for (int i = 0; i < 16; ++i) out[i] = DT<T>::from_f(v[i]);
   } else if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(out)[0] = f[0];
-    reinterpret_cast<float4*>(out)[1] = f[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<float4*>(out)[i] =
+          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   } else {
-    *reinterpret_cast<uint4*>(out) =
-        make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[0].z, f[0].w), pack2<T>(f[1].x, f[1].y),
-                   pack2<T>(f[1].z, f[1].w));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      reinterpret_cast<uint4*>(out)[i] =
+          make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                     pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
   }
 }
 
-// Threads that cover a row of Hkv * D codes in pieces of 8: `tpr` of them side
-// by side, or all of the CTA in turns; a CTA holds threads() of them.
-__host__ __device__ inline int piece_threads(int pieces) {
-  return pieces >= 256 ? 256 : 256 / pieces * pieces;
-}
+// Threads that cover a row of this many pieces: as many rows side
+// by side as a CTA holds, or the whole CTA in turns.
+inline int piece_threads(int pieces) { return pieces >= 256 ? 256 : 256 / pieces * pieces; }
 
-// Rows by slot; a thread reads the same piece of kRows rows at once, and the
-// slots of its next rows before these arrive.
-constexpr int kRows = 4;
+// Rows by slot; a thread reads the same piece of kRows rows at once.
+constexpr int kRows = 1;
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)
-    gather_q8_kernel(T* out, const uint8_t* pool, const float* scale, const int64_t* slots,
-                     int64_t n, int Hkv, int D, int bs, int shift, int64_t num_slots, int vec,
-                     int32_t* err) {
+    gather_q8_kernel(T* out, const uint8_t* pool, const float* scale, const int64_t* slots, int n,
+                     int Hkv, int D, int bs, int shift, int64_t num_slots, int vec, int32_t* err) {
   wait_prior_grid();
-  const int pieces = Hkv * D / 8;
+  const int pieces = Hkv * D / 16;
   const int tpr = pieces < 256 ? pieces : 256;
   const int side = blockDim.x / tpr;  // rows side by side
   const int c0 = threadIdx.x % tpr;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * side * kRows;
-  int64_t row0 = static_cast<int64_t>(blockIdx.x) * side * kRows + threadIdx.x / tpr;
-  int64_t next[kRows];
-  auto fetch = [&](int64_t from) {
+  const int row0 = blockIdx.x * side * kRows + threadIdx.x / tpr;
+  int64_t s[kRows];
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) next[u] = from + u * side < n ? slots[from + u * side] : 0;
-  };
-  fetch(row0);
-  for (; row0 < n; row0 += step) {
-    int64_t s[kRows];
+  for (int u = 0; u < kRows; ++u) s[u] = row0 + u * side < n ? slots[row0 + u * side] : 0;
+#pragma unroll
+  for (int u = 0; u < kRows; ++u)
+    if (s[u] < 0 || s[u] >= num_slots) {
+      s[u] = -1;
+      if (c0 == 0) set_err(err, IR_DEVERR_SLOT);
+    }
+  for (int c = c0; c < pieces; c += tpr) {
+    const int h = c * 16 / D;
+    uint4 codes[kRows];
+    float sc[kRows];
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
-      s[u] = next[u];
-      if (s[u] < 0 || s[u] >= num_slots) {
-        s[u] = -1;
-        if (c0 == 0) set_err(err, IR_DEVERR_SLOT);
-      }
+      const uint32_t at = s[u] < 0 ? 0u : static_cast<uint32_t>(s[u]);
+      const uint32_t blk = shift >= 0 ? at >> shift : at / bs;
+      codes[u] = reinterpret_cast<const uint4*>(pool)[static_cast<uint64_t>(at) * pieces + c];
+      sc[u] = scale[static_cast<uint64_t>(blk) * Hkv + h];
     }
-    for (int c = c0; c < pieces; c += tpr) {
-      const int h = c * 8 / D;
-      uint2 codes[kRows];
-      float sc[kRows];
 #pragma unroll
-      for (int u = 0; u < kRows; ++u) {
-        const int64_t at = s[u] < 0 ? 0 : s[u];
-        const int64_t blk = shift >= 0 ? at >> shift : at / bs;
-        codes[u] = reinterpret_cast<const uint2*>(pool)[at * pieces + c];
-        sc[u] = scale[blk * Hkv + h];
-      }
-      if (c + tpr >= pieces) fetch(row0 + step);
-#pragma unroll
-      for (int u = 0; u < kRows; ++u) {
-        const int64_t r = row0 + u * side;
-        if (s[u] < 0) codes[u] = make_uint2(0u, 0u), sc[u] = 0.f;
-        if (r < n) store8<T, C>(out + (r * pieces + c) * 8, codes[u], sc[u], vec);
-      }
+    for (int u = 0; u < kRows; ++u) {
+      if (s[u] < 0) codes[u] = make_uint4(0u, 0u, 0u, 0u), sc[u] = 0.f;
+      if (row0 + u * side < n)
+        store16<T, C>(out + (static_cast<int64_t>(row0 + u * side) * pieces + c) * 16, codes[u],
+                      sc[u], vec);
     }
   }
 }
@@ -517,8 +596,8 @@ __global__ void __launch_bounds__(256)
         const int64_t at = (id * bs + r) * pieces + c;
         const uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
         const uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
-        store8<T, C>(kout + at * 8, kc, k, 1);
-        store8<T, C>(vout + at * 8, vc, v, 1);
+        store8<T, C>(kout + at * 8, kc, k);
+        store8<T, C>(vout + at * 8, vc, v);
       }
     }
   }
@@ -569,8 +648,8 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   a.Hkv = Hkv;
   a.D = D;
   a.bs = bs;
-  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % (4 * eb)) == 0 &&
-                   k_stride % 4 == 0 && v_stride % 4 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
+                   (k_stride * eb) % 16 == 0 && (v_stride * eb) % 16 == 0;
   a.err = err;
   const size_t smem = static_cast<size_t>(bs) * 4;
   if (n <= kScanTokens) {
@@ -592,9 +671,11 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   l.head = l.count + 2;
   l.next = reinterpret_cast<int*>(w + heads);
   l.owners = reinterpret_cast<int*>(w + heads + align256(static_cast<size_t>(n) * 4));
-  cudaError_t e = cudaMemsetAsync(w, 0, heads, stream);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  int rc = launch_behind(link_runs_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0,
+  const int words = static_cast<int>(num_blocks + 2);
+  int rc = launch_behind(zero_kernel, dim3(words < 65536 ? (words + 255) / 256 : 256), 256, 0,
+                         stream, l.count, words);
+  if (rc) return rc;
+  rc = launch_behind(link_runs_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0,
                          stream, slots, n, num_slots, bs, l, err);
   if (rc) return rc;
   const int64_t blocks = n < num_blocks ? n : num_blocks;
@@ -602,7 +683,9 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   // (at least one warp for every task of a block)
   const int64_t least = (2 * Hkv + kQWarps - 1) / kQWarps;
   int64_t grid = small ? (blocks * 2 * Hkv + kQWarps - 1) / kQWarps : blocks;
-  if (grid > static_cast<int64_t>(sms) * 8) grid = static_cast<int64_t>(sms) * 8;
+  // (as many CTAs as fit at once)
+  const int64_t most = static_cast<int64_t>(sms) * (dtype == IR_DTYPE_F32 ? 2 : 3);
+  if (grid > most) grid = most;
   if (small && grid < least) grid = least;
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
@@ -618,11 +701,10 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
 
 int launch_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
                            int64_t n, int Hkv, int D, int bs, int64_t num_slots, int dtype,
-                           int fmt, int sms, int32_t* err, cudaStream_t stream) {
-  const int pieces = Hkv * D / 8, threads = piece_threads(pieces);
+                           int fmt, int32_t* err, cudaStream_t stream) {
+  const int pieces = Hkv * D / 16, threads = piece_threads(pieces);
   const int64_t rows = static_cast<int64_t>(pieces < 256 ? threads / pieces : 1) * kRows;
-  int64_t grid = (n + rows - 1) / rows;
-  if (grid > static_cast<int64_t>(sms) * 4) grid = static_cast<int64_t>(sms) * 4;
+  const int64_t grid = (n + rows - 1) / rows;
   const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
   int shift = 0;  // log2(bs), or -1
   while ((1 << shift) < bs && shift < 30) ++shift;
@@ -633,7 +715,7 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
       return launch_behind(gather_q8_kernel<T, decltype(c)>, dim3(static_cast<unsigned>(grid)),
                            threads, 0, stream,
                            static_cast<T*>(out), static_cast<const uint8_t*>(pool), scale, slots,
-                           n, Hkv, D, bs, shift, num_slots, vec, err);
+                           static_cast<int>(n), Hkv, D, bs, shift, num_slots, vec, err);
     });
   });
 }

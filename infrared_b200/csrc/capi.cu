@@ -630,9 +630,8 @@ int check_q8_rows(int64_t n, int hkv, int d, int bs, int64_t num_slots, int dtyp
     return fail(IR_ERR_INVALID_ARG, "bad sizes (num_slots is a positive multiple of block_size)");
   if (d != 64 && d != 128) return fail(IR_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   if (hkv > 4096) return fail(IR_ERR_UNSUPPORTED, "more than 4096 kv heads");
-  if (n > INT32_MAX || num_slots / bs >= INT32_MAX ||
-      n * (static_cast<int64_t>(hkv) * d / 16) > (int64_t{1} << 38))
-    return fail(IR_ERR_UNSUPPORTED, "too many rows or blocks");
+  if (n > INT32_MAX / 2 || num_slots > INT32_MAX)
+    return fail(IR_ERR_UNSUPPORTED, "2^30 rows or 2^31 slots or more");
   return IR_OK;
 }
 
@@ -1159,12 +1158,9 @@ int ir_cache_gather_q8(void* out, const void* pool, const float* scale, const in
   if (num_rows == 0) return IR_OK;
   if (!out || !pool || !scale || !slots) return fail(IR_ERR_INVALID_ARG, "null pointer");
   if (!aligned(pool, 16)) return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
-  int sms = 1;
-  const int e = cached(-1, sm_count_now, 0, &sms);
-  if (e) return cuda_status(e, "device query");
   return cuda_status(irb::launch_cache_gather_q8(out, pool, scale, slots, num_rows, num_kv_heads,
                                                  head_dim, block_size, num_slots, dtype,
-                                                 kv_format, sms, err_flag,
+                                                 kv_format, err_flag,
                                                  static_cast<cudaStream_t>(stream)),
                      "8-bit cache gather launch");
 }

@@ -40,6 +40,8 @@
 //      pairs of two rows become the token pairs of the A operand
 // t() makes every 8- or 16-lane phase of these reads touch each bank once
 // under the 128-byte (D = 128) and the 64-byte (D = 64) swizzle.
+#include <atomic>
+
 #include "decode_common.cuh"
 #include "kernels.h"
 #include "quant.cuh"
@@ -713,9 +715,15 @@ int run_q8(const CallQ8* call) {
   using L = LayoutQ8<D, HG, R, NS, SETS>;
   static_assert(L::kAlloc <= 227 * 1024 && NS >= 3, "shared memory budget");
   auto kern = decode_q8_kernel<T, C, D, HG, R, SETS, NS>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+  // the shared-memory limit is set on a device's first launch (a bit each; those
+  // beyond 63 every time), and once more if a launch fails, since a device
+  // reset takes it back
+  static std::atomic<uint64_t> known{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  bool fresh = !(known.load(std::memory_order_acquire) & bit);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(call->a->Hkv / HG, call->a->G);
   cfg.blockDim = dim3(kThreads);
@@ -726,8 +734,17 @@ int run_q8(const CallQ8* call) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(
-      cudaLaunchKernelEx(&cfg, kern, *call->tmk, *call->tmv, *call->a, call->q_bulk));
+  for (;;) {
+    if (fresh) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      known.fetch_or(bit, std::memory_order_release);
+    }
+    e = cudaLaunchKernelEx(&cfg, kern, *call->tmk, *call->tmv, *call->a, call->q_bulk);
+    if (e == cudaSuccess || fresh) return static_cast<int>(e);
+    cudaGetLastError();  // (not sticky: the launch was refused)
+    fresh = true;
+  }
 }
 
 template <typename T, typename C, int D, int HG, bool SETS>

@@ -104,7 +104,7 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
                           cudaStream_t stream);
 int launch_cache_gather_q8(void* out, const void* pool, const float* scale, const int64_t* slots,
                            int64_t n, int Hkv, int D, int bs, int64_t num_slots, int dtype,
-                           int fmt, int sms, int32_t* err, cudaStream_t stream);
+                           int fmt, int32_t* err, cudaStream_t stream);
 // Every block that a sequence's history covers, as rows of dtype at the same
 // place of the output pools.
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,

@@ -764,6 +764,36 @@ def derive_varlen_metadata(gather_slots: torch.Tensor, mask: torch.Tensor, block
 
 
 # --- 8-bit K/V cache ----------------------------------------------------------
+#
+# A call's checks depend on its tensors' shapes, strides, types and devices
+# alone, so each entry point keeps the outcome (the shape structs and sizes it
+# passes on) under a key of these: a repeated call, such as every layer of
+# every step makes, skips the checks. No plan holds a tensor or an address.
+
+
+class _Plans(dict):
+    """Validated call plans, bounded."""
+
+    def keep(self, key, plan):
+        if len(self) > 512:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+_write_plans, _gather_plans, _decode_q8_plans, _prefill_q8_plans, _norm_plans = \
+    (_Plans() for _ in range(5))
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _stream
+
+
+def _issue(dev: int, fn, *args) -> None:
+    """One library call on device ``dev``'s current stream (its last argument)."""
+    if dev == torch.cuda.current_device():
+        check(fn(*args, _raw_stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _raw_stream(dev)))
 
 
 def kv_format(dtype: torch.dtype) -> int:
@@ -803,7 +833,14 @@ def _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size) -> int:
     return fmt
 
 
-@_on_tensor_device
+def _pools_key(k_pool, v_pool, k_scale, v_scale, block_size):
+    return (k_pool.shape, k_pool.dtype, k_pool.is_contiguous(), k_pool.get_device(),
+            v_pool.shape, v_pool.dtype, v_pool.is_contiguous(), v_pool.get_device(),
+            k_scale.shape, k_scale.dtype, k_scale.is_contiguous(), k_scale.get_device(),
+            v_scale.shape, v_scale.dtype, v_scale.is_contiguous(), v_scale.get_device(),
+            block_size)
+
+
 def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
                    v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                    slot_mapping: torch.Tensor, block_size: int) -> None:
@@ -816,56 +853,69 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
     rescaled when it grows; a write that holds a block's first row begins the
     block afresh (``ir_cache_write_q8``). Negative slots skip their rows.
     """
-    dev = _dev_index(k_pool)
-    fmt = _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size)
-    n = slot_mapping.numel()
-    hkv, d = k_pool.shape[1], k_pool.shape[2]
-    k = k.reshape(n, hkv, d)
-    v = v.reshape(n, hkv, d)
-    for t, nm in ((k, "k"), (v, "v")):
-        if t.dtype != k.dtype or t.device != k_pool.device:
-            raise ValueError(f"{nm} must match k's dtype and the pool's device")
-        if n and (t.stride(2) != 1 or t.stride(1) != d):
-            raise ValueError(f"{nm} rows must be [Hkv, D] contiguous")
-    slots = slot_mapping.reshape(-1)
-    if slots.dtype != torch.int64 or not slots.is_contiguous() or slots.device != k_pool.device:
-        raise ValueError("slot_mapping must be a contiguous int64 tensor on the pool's device")
-    code = dtype_code(k.dtype)
+    key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype,
+           v.get_device(), slot_mapping.shape, slot_mapping.dtype,
+           slot_mapping.is_contiguous(), slot_mapping.get_device(),
+           _pools_key(k_pool, v_pool, k_scale, v_scale, block_size))
+    plan = _write_plans.get(key)
+    if plan is None:
+        dev = _dev_index(k_pool)
+        fmt = _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size)
+        n = slot_mapping.numel()
+        hkv, d = k_pool.shape[1], k_pool.shape[2]
+        if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or \
+                slot_mapping.device != k_pool.device:
+            raise ValueError("slot_mapping must be a contiguous int64 tensor on the pool's device")
+        strides = []
+        for t, nm in ((k, "k"), (v, "v")):
+            if t.dtype != k.dtype or t.device != k_pool.device:
+                raise ValueError(f"{nm} must match k's dtype and the pool's device")
+            r = t.reshape(n, hkv, d)
+            if n and (r.stride(2) != 1 or r.stride(1) != d or r.data_ptr() != t.data_ptr()):
+                raise ValueError(f"{nm} rows must be [Hkv, D] contiguous")
+            strides.append(_row_stride(r, hkv * d))
+        code = dtype_code(k.dtype)
+        lib = _lib.load()
+        nbytes = lib.ir_cache_write_q8_workspace_size(n, k_pool.shape[0], block_size)
+        plan = _write_plans.keep(key, (dev, lib.ir_cache_write_q8, *strides, n, hkv, d,
+                                       k_pool.shape[0], code, fmt, nbytes))
+    dev, fn, ks, vs, n, hkv, d, num_slots, code, fmt, nbytes = plan
     if n == 0:
         return
-    lib = _lib.load()
-    nbytes = lib.ir_cache_write_q8_workspace_size(n, k_pool.shape[0], block_size)
+    # (of this call alone: PyTorch's allocator orders its reuse on the stream)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=k_pool.device) if nbytes else None
-    check(lib.ir_cache_write_q8(
-        k.data_ptr(), v.data_ptr(), _row_stride(k, hkv * d), _row_stride(v, hkv * d),
-        k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), n, hkv, d,
-        block_size, k_pool.shape[0], code, fmt, _ptr(ws), nbytes, error_flag(dev).data_ptr(),
-        _stream(dev)))
+    _issue(dev, fn, k.data_ptr(), v.data_ptr(), ks, vs, k_pool.data_ptr(), v_pool.data_ptr(),
+           k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), n, hkv, d, block_size,
+           num_slots, code, fmt, _ptr(ws), nbytes, error_flag(dev).data_ptr())
 
 
-@_on_tensor_device
 def cache_gather_q8(pool: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor,
                     block_size: int, dtype: torch.dtype) -> torch.Tensor:
     """Rows of an 8-bit pool as values of ``dtype``: a 1-D or 2-D int64 slot tensor
     -> ``[*slots.shape, Hkv, D]`` (finite values beyond the dtype saturate)."""
-    dev = _dev_index(pool)
-    fmt = _check_pool_q8(pool, scale, block_size, "pool")
-    flat = slots.reshape(-1)
-    if flat.dtype != torch.int64 or flat.device != pool.device:
-        raise ValueError("slots must be int64 on the pool's device")
-    flat = flat.contiguous()
-    code = dtype_code(dtype)
-    out = torch.empty((*slots.shape, pool.shape[1], pool.shape[2]), dtype=dtype,
-                      device=pool.device)
-    if flat.numel():
-        check(_lib.load().ir_cache_gather_q8(
-            out.data_ptr(), pool.data_ptr(), scale.data_ptr(), flat.data_ptr(), flat.numel(),
-            pool.shape[1], pool.shape[2], block_size, pool.shape[0], code, fmt,
-            error_flag(dev).data_ptr(), _stream(dev)))
+    key = (pool.shape, pool.dtype, pool.is_contiguous(), pool.get_device(), scale.shape,
+           scale.dtype, scale.is_contiguous(), scale.get_device(), slots.shape, slots.dtype,
+           slots.get_device(), block_size, dtype)
+    plan = _gather_plans.get(key)
+    if plan is None:
+        dev = _dev_index(pool)
+        fmt = _check_pool_q8(pool, scale, block_size, "pool")
+        if slots.dtype != torch.int64 or slots.device != pool.device:
+            raise ValueError("slots must be int64 on the pool's device")
+        plan = _gather_plans.keep(key, (dev, _lib.load().ir_cache_gather_q8, slots.numel(),
+                                        (*slots.shape, pool.shape[1], pool.shape[2]),
+                                        pool.shape, dtype_code(dtype), fmt))
+    dev, fn, n, shape, (num_slots, hkv, d), code, fmt = plan
+    out = torch.empty(shape, dtype=dtype, device=pool.device)
+    if n:
+        slots = slots if slots.is_contiguous() else slots.contiguous()
+        _issue(dev, fn, out.data_ptr(), pool.data_ptr(), scale.data_ptr(), slots.data_ptr(), n, hkv,
+               d, block_size, num_slots, code, fmt, error_flag(dev).data_ptr())
     return out
 
 
-def _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, block_size):
+def _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
+                     block_size):
     _dev_index(q)
     fmt = _check_pools_q8(k_pool, v_pool, k_scale, v_scale, block_size)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
@@ -880,25 +930,32 @@ def _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_
     for t in (k_pool, block_tables, context_lens):
         if t.device != q.device:
             raise ValueError("all tensors must be on the same device")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or
+                            out.stride(1) != q.shape[2] or out.device != q.device):
+        raise ValueError("out must be of q's shape, dtype and device with [H, D] contiguous rows")
     return fmt
 
 
-def _scratch(ws: torch.Tensor | None, nbytes: int, device) -> torch.Tensor:
+def _decode_q8_key(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out, scale,
+                   block_size):
+    return (q.shape, q.stride(), q.dtype, q.get_device(), block_tables.shape,
+            block_tables.stride(), block_tables.dtype, block_tables.get_device(),
+            context_lens.shape, context_lens.dtype, context_lens.is_contiguous(),
+            context_lens.get_device(), scale,
+            None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()),
+            _pools_key(k_pool, v_pool, k_scale, v_scale, block_size))
+
+
+def _scratch(ws: torch.Tensor | None, nbytes: int, q: torch.Tensor) -> torch.Tensor:
     """The caller's workspace, or one of this call alone: it needs no initial
     state, and PyTorch's allocator orders its reuse on the current stream and
     inside a graph capture, so calls on other streams and replayed graphs
     never share it."""
     if ws is None:
-        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-    if ws.numel() * ws.element_size() < nbytes or ws.device != device or not ws.is_contiguous():
+        return torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if ws.numel() * ws.element_size() < nbytes or ws.device != q.device or not ws.is_contiguous():
         raise ValueError(f"workspace must be {nbytes} contiguous bytes on q's device")
     return ws
-
-
-def _check_out(out, q):
-    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
-            out.stride(1) != q.shape[2] or out.device != q.device:
-        raise ValueError("out must be of q's shape, dtype and device with [H, D] contiguous rows")
 
 
 def decode_plan_q8(q, k_pool, block_tables, block_size, scale=1.0):
@@ -911,7 +968,6 @@ def decode_plan_q8(q, k_pool, block_tables, block_size, scale=1.0):
     return path.value, g.value, lib.ir_paged_decode_q8_workspace_size(s, fmt)
 
 
-@_on_tensor_device
 def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                     k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                     context_lens: torch.Tensor, scale: float, block_size: int,
@@ -919,30 +975,36 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                     ws: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`paged_decode` over an 8-bit cache (:func:`cache_write_q8`):
     ``q [B, H, D]`` (any dtype of the framework) -> ``[B, H, D]``."""
+    key = _decode_q8_key(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
+                         scale, block_size)
+    plan = _decode_q8_plans.get(key)
+    if plan is None:
+        fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
+                               block_size)
+        if block_tables.shape[0] != q.shape[0] or context_lens.numel() != q.shape[0]:
+            raise ValueError("batch sizes of q, block_tables and context_lens differ")
+        dev = _dev_index(q)
+        row = q.shape[1] * q.shape[2]
+        s = _shape(q, k_pool, block_tables, block_size, scale,
+                   row if out is None else _row_stride(out, row))
+        s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            nbytes = lib.ir_paged_decode_q8_workspace_size(s, fmt)
+            if nbytes == 0:
+                check(lib.ir_paged_decode_q8_plan(s, fmt, None, None))
+        plan = _decode_q8_plans.keep(key, (dev, lib.ir_paged_decode_q8, s, fmt, nbytes))
+    dev, fn, s, fmt, nbytes = plan
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens,
-                           block_size)
-    if block_tables.shape[0] != q.shape[0] or context_lens.numel() != q.shape[0]:
-        raise ValueError("batch sizes of q, block_tables and context_lens differ")
-    _check_out(out, q)
-    dev = _dev_index(q)
-    lib = _lib.load()
-    row = q.shape[1] * q.shape[2]
-    s = _shape(q, k_pool, block_tables, block_size, scale, _row_stride(out, row))
-    s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
-    nbytes = lib.ir_paged_decode_q8_workspace_size(s, fmt)
-    if nbytes == 0:
-        check(lib.ir_paged_decode_q8_plan(s, fmt, None, None))
-    ws = _scratch(ws, nbytes, q.device)
-    check(lib.ir_paged_decode_q8(
-        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), fmt, block_tables.data_ptr(), context_lens.data_ptr(), s,
-        ws.data_ptr(), ws.numel() * ws.element_size(), error_flag(dev).data_ptr(), _stream(dev)))
+    ws = _scratch(ws, nbytes, q)
+    _issue(dev, fn, out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+           k_scale.data_ptr(), v_scale.data_ptr(), fmt, block_tables.data_ptr(),
+           context_lens.data_ptr(), s, ws.data_ptr(), ws.numel() * ws.element_size(),
+           error_flag(dev).data_ptr())
     return out
 
 
-@_on_tensor_device
 def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                      k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                      context_lens: torch.Tensor, q_start: torch.Tensor, scale: float,
@@ -950,36 +1012,44 @@ def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
                      ws: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`paged_prefill` over an 8-bit cache (:func:`cache_write_q8`). Its
     workspace holds one layer's pool in q's dtype (``ir_paged_prefill_q8``)."""
-    fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens,
-                           block_size)
-    if q_start.dtype != torch.int32 or not q_start.is_contiguous() or q_start.device != q.device:
-        raise ValueError("q_start must be a contiguous int32 tensor on q's device")
-    nseq = q_start.numel() - 1
-    if nseq < 0 or block_tables.shape[0] != nseq or context_lens.numel() != nseq:
-        raise ValueError("q_start must have one more entry than block_tables / context_lens")
+    key = (_decode_q8_key(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
+                          scale, block_size),
+           q_start.shape, q_start.dtype, q_start.is_contiguous(), q_start.get_device())
+    plan = _prefill_q8_plans.get(key)
+    if plan is None:
+        fmt = _check_decode_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
+                               block_size)
+        if q_start.dtype != torch.int32 or not q_start.is_contiguous() or \
+                q_start.device != q.device:
+            raise ValueError("q_start must be a contiguous int32 tensor on q's device")
+        nseq = q_start.numel() - 1
+        if nseq < 0 or block_tables.shape[0] != nseq or context_lens.numel() != nseq:
+            raise ValueError("q_start must have one more entry than block_tables / context_lens")
+        row = q.shape[1] * q.shape[2]
+        s = _prefill_shape(q, k_pool, block_tables, q_start, block_size, scale,
+                           row if out is None else _row_stride(out, row))
+        s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
+        plan = _prefill_q8_plans.keep(key, (_dev_index(q), _lib.load(), s, fmt))
+    dev, lib, s, fmt = plan
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check_out(out, q)
-    dev = _dev_index(q)
-    row = q.shape[1] * q.shape[2]
-    s = _prefill_shape(q, k_pool, block_tables, q_start, block_size, scale,
-                       _row_stride(out, row))
-    s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
-    lib = _lib.load()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    # (asked each time: it depends on the path chosen by set_prefill_path)
     nbytes = lib.ir_paged_prefill_q8_workspace_size(s)
-    ws = _scratch(ws, nbytes, q.device)
-    check(lib.ir_paged_prefill_q8(
-        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), fmt, block_tables.data_ptr(), context_lens.data_ptr(),
-        q_start.data_ptr(), s, ws.data_ptr(), ws.numel() * ws.element_size(),
-        error_flag(dev).data_ptr(), _stream(dev)))
+    ws = _scratch(ws, max(nbytes, 256), q)
+    _issue(dev, lib.ir_paged_prefill_q8, out.data_ptr(), q.data_ptr(), k_pool.data_ptr(),
+           v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), fmt,
+           block_tables.data_ptr(), context_lens.data_ptr(), q_start.data_ptr(), s, ws.data_ptr(),
+           ws.numel() * ws.element_size(), error_flag(dev).data_ptr())
     return out
 
 
 # --- q/k norm with rotation ---------------------------------------------------
 
 
-@_on_tensor_device
+def _like(t):
+    return (t.shape, t.stride(), t.dtype, t.get_device())
+
+
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, w_q: torch.Tensor | None,
                  w_k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, eps: float,
                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
@@ -988,29 +1058,49 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, w_q: torch.Tensor | None,
     ``cos`` / ``sin [N, D]``, in one kernel; returns ``(q_out, k_out)``.
 
     Computed in fp32 and rounded once. ``q`` and ``k`` may be row views of one
-    QKV projection; ``q_out`` / ``k_out`` may be ``q`` / ``k`` themselves.
+    QKV projection; ``q_out`` / ``k_out`` may be ``q`` / ``k`` themselves, but
+    no other memory that overlaps them.
     """
-    dev = _dev_index(q)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError("q must be [N, H, D] and k [N, Hkv, D]")
-    n, h, d = q.shape
-    hkv = k.shape[1]
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype,
+           k.get_device(), cos.shape, cos.stride(), cos.dtype, cos.get_device(), sin.shape,
+           sin.stride(), sin.dtype, sin.get_device(), w_q is None or _like(w_q),
+           w_k is None or _like(w_k), q_out is None or _like(q_out),
+           k_out is None or _like(k_out))
+    plan = _norm_plans.get(key)
+    if plan is None:
+        dev = _dev_index(q)
+        if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+            raise ValueError("q must be [N, H, D] and k [N, Hkv, D]")
+        n, h, d = q.shape
+        hkv = k.shape[1]
+        strides = []
+        for name, t, like in (("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)):
+            row = like.shape[1] * d
+            if t is None:
+                strides.append(row)
+                continue
+            if t.dtype != q.dtype or t.device != q.device or t.shape != like.shape:
+                raise ValueError(f"{name} must match q's dtype and device and its input's shape")
+            if t.numel() and (t.stride(2) != 1 or t.stride(1) != d):
+                raise ValueError(f"{name} rows must be [heads, D] contiguous")
+            strides.append(_row_stride(t, row))
+        for name, t in (("w_q", w_q), ("w_k", w_k)):
+            if t is not None and (t.numel() != d or t.dtype != q.dtype or not t.is_contiguous()
+                                  or t.device != q.device):
+                raise ValueError(f"{name} must be a contiguous [D] weight of q's dtype")
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype != torch.float32 or t.device != q.device or tuple(t.shape) != (n, d) or \
+                    (n and t.stride(1) != 1):
+                raise ValueError(f"{name} must be fp32 [N, D] rows on q's device")
+        if _row_stride(cos, d) != _row_stride(sin, d):
+            raise ValueError("cos and sin must have the same row stride")
+        plan = _norm_plans.keep(key, (dev, _lib.load().ir_qk_norm_rope, strides,
+                                      _row_stride(cos, d), n, h, hkv, d, dtype_code(q.dtype)))
+    dev, fn, strides, rs, n, h, hkv, d, code = plan
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    for name, t, like in (("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)):
-        if t.dtype != q.dtype or t.device != q.device or t.shape != like.shape:
-            raise ValueError(f"{name} must match q's dtype and device and its input's shape")
-        if t.stride(2) != 1 or t.stride(1) != d:
-            raise ValueError(f"{name} rows must be [heads, D] contiguous")
-    for name, t in (("w_q", w_q), ("w_k", w_k)):
-        if t is not None and (t.numel() != d or t.dtype != q.dtype or not t.is_contiguous()
-                              or t.device != q.device):
-            raise ValueError(f"{name} must be a contiguous [D] weight of q's dtype")
-    cos, sin = _rope_rows(cos, sin, n, d, q.device)
-    check(_lib.load().ir_qk_norm_rope(
-        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), _row_stride(q, h * d),
-        _row_stride(k, hkv * d), _row_stride(q_out, h * d), _row_stride(k_out, hkv * d),
-        _ptr(w_q), _ptr(w_k), cos.data_ptr(), sin.data_ptr(), _row_stride(cos, d), float(eps), n, h, hkv, d, dtype_code(q.dtype), _stream(dev)))
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    _issue(dev, fn, q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *strides,
+           _ptr(w_q), _ptr(w_k), cos.data_ptr(), sin.data_ptr(), rs, eps, n, h, hkv, d, code)
     return q_out, k_out
