@@ -22,8 +22,9 @@ Three hand-written sm_100a CUDA paths behind a C ABI
   embedding in the same pass.
 
 ``PagedKVPool``, ``PagedContext`` and ``paged_attention`` keep the
-reference engine's interface; ``shim.install()`` routes infrared's own
-decode calls here; ``dist`` shards the work over the GPUs of one node.
+reference engine's interface (``PagedKVPoolQ8`` is the pool in 8 bits);
+``shim.install()`` routes infrared's own decode calls here; ``dist`` shards
+the work over the GPUs of one node.
 """
 
 from ._lib import InfraredB200Error, UnsupportedShape
@@ -33,10 +34,11 @@ from .ops import (DeviceError, cache_gather, cache_gather_q8, cache_write, cache
                   paged_decode, paged_decode_lse, paged_decode_q8, paged_decode_rope,
                   paged_decode_rope_write, paged_decode_write, paged_prefill, paged_prefill_q8,
                   qk_norm_rope)
-from .paged_kv_cache import PagedContext, PagedKVPool
+from .paged_kv_cache import PagedContext, PagedKVPool, PagedKVPoolQ8
 
 __all__ = [
-    "DeviceError", "InfraredB200Error", "PagedContext", "PagedKVPool", "UnsupportedShape",
+    "DeviceError", "InfraredB200Error", "PagedContext", "PagedKVPool",
+    "PagedKVPoolQ8", "UnsupportedShape",
     "cache_gather", "cache_gather_q8", "cache_write", "cache_write_q8", "check_device_errors",
     "derive_block_metadata", "kv_proj_rope_write", "lse_merge", "paged_attention",
     "paged_decode", "paged_decode_lse", "paged_decode_q8", "paged_decode_rope",

@@ -24,6 +24,7 @@ import threading
 import torch
 
 from . import ops
+from .paged_kv_cache import PagedKVPoolQ8
 
 _cache_lock = threading.Lock()
 _cache: dict = {}
@@ -63,6 +64,10 @@ def prefill_frame(q: torch.Tensor, paged, mask: torch.Tensor, layer_idx: int,
     pool = paged.pool
     bt, ctx, q_start = varlen_metadata(paged, mask)
     out = torch.empty((1, nq, h, d), dtype=q.dtype, device=q.device)
+    if isinstance(pool, PagedKVPoolQ8):
+        ops.paged_prefill_q8(q.reshape(nq, h, d), *pool.layer(layer_idx), bt, ctx, q_start, scale,
+                             pool.block_size, out=out.view(nq, h, d))
+        return out
     ops.paged_prefill(q.reshape(nq, h, d), pool.k[layer_idx], pool.v[layer_idx], bt, ctx,
                       q_start, scale, pool.block_size, out=out.view(nq, h, d))
     return out
@@ -83,7 +88,8 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, paged,
     True runs the fused write + decode kernel (``ir_paged_decode_write``;
     the write slot of each row must be the slot of its last history
     position, which the engine's decode step guarantees), False runs the
-    cache write and the decode as two launches.
+    cache write and the decode as two launches. With a ``PagedKVPoolQ8`` the
+    rows are quantised as they are written and read as 8-bit codes.
     """
     b, sq, h, d = q.shape
     hkv = k.shape[-2]
@@ -101,7 +107,12 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, paged,
     bt, ctx = block_metadata(paged, mask)
     q3 = q.reshape(b, h, d)
     out = torch.empty((b, 1, h, d), dtype=q.dtype, device=q.device)
-    if paged.use_triton:
+    if isinstance(pool, PagedKVPoolQ8):
+        pool.write(layer_idx, k.reshape(-1, hkv, d), v.reshape(-1, hkv, d),
+                   paged.write_slots)
+        ops.paged_decode_q8(q3, *pool.layer(layer_idx), bt, ctx, scale, pool.block_size,
+                            out=out.view(b, h, d))
+    elif paged.use_triton:
         ops.paged_decode_write(q3, k.reshape(b, hkv, d), v.reshape(b, hkv, d),
                                pool.k[layer_idx], pool.v[layer_idx], paged.write_slots,
                                bt, ctx, scale, pool.block_size, out=out.view(b, h, d))

@@ -630,8 +630,8 @@ int check_q8_rows(int64_t n, int hkv, int d, int bs, int64_t num_slots, int dtyp
     return fail(IR_ERR_INVALID_ARG, "bad sizes (num_slots is a positive multiple of block_size)");
   if (d != 64 && d != 128) return fail(IR_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   if (hkv > 4096) return fail(IR_ERR_UNSUPPORTED, "more than 4096 kv heads");
-  if (n > INT32_MAX / 2 || num_slots > INT32_MAX)
-    return fail(IR_ERR_UNSUPPORTED, "2^30 rows or 2^31 slots or more");
+  if (n > INT32_MAX / 2 || num_slots > INT32_MAX - 64)
+    return fail(IR_ERR_UNSUPPORTED, "2^30 rows or about 2^31 slots or more");
   return IR_OK;
 }
 

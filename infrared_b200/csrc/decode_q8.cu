@@ -83,22 +83,22 @@ struct LayoutQ8 {
   static constexpr int kTileBytes = 2 * kSide;
   static constexpr int kStage = W * kTileBytes;
   static constexpr int kScales = W * NB * 2 * HG;  // floats per stage
-  static constexpr int kSteps = 5;                 // barriers of a combination
   static constexpr int off_scale = NS * kStage;
   static constexpr int off_desc = off_scale + NS * kScales * 4;
-  // full[NS], empty[NS], qfree[2], then kSteps per pair
+  // full[NS], empty[NS], qfree[2], then one per consumer warp (see the flush)
   static constexpr int off_bar = off_desc + NS * 16;
-  static constexpr int off_misc = (off_bar + (2 * NS + 2 + kRows * kSteps) * 8 + 15) / 16 * 16;
-  // misc: RangeInfo (64 B) + block-scan scratch; then (m, l) of every warp, twice
+  static constexpr int off_misc = (off_bar + (2 * NS + 2 + kConsumers) * 8 + 15) / 16 * 16;
+  // misc: RangeInfo (64 B) + block-scan scratch; then (m, l) of every warp
   static constexpr int off_ml = off_misc + 64 + (kConsumers + 1) * 8 + 8;
-  static constexpr int kMl = kConsumers * 8 * 2;  // floats of one copy
+  static constexpr int kMl = kConsumers * 8 * 2;
   static constexpr int kPart = 8 * D;             // floats of one warp's O
-  static constexpr int off_part = (off_ml + 2 * kMl * 4 + 15) / 16 * 16;
+  static constexpr int off_part = (off_ml + kMl * 4 + 15) / 16 * 16;
   static constexpr int kParts = kRows * (WT / 2);
-  static constexpr int kQBuf = HG * (SETS ? 16 : 8) * D * 2;
   static constexpr int off_q = (off_part + kParts * kPart * 4 + 127) / 128 * 128;
-  static constexpr int kBytes = off_q + 2 * kQBuf;
-  static constexpr int kAlloc = kBytes + 1024;  // slack for 1 KB alignment
+  // q rows of the current and the next segment: the group's own size, so that
+  // the merge kernel's CTAs mostly find room beside this kernel's
+  static constexpr int kAlloc = off_q + 2 * HG * (SETS ? 16 : 8) * D * 2;  // at most
+  static int bytes(int n_rep) { return off_q + 2 * HG * n_rep * D * 2; }
 };
 
 // Stages that fit in one CTA's shared memory beside the other buffers.
@@ -137,16 +137,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = LayoutQ8<D, HG, R, NS, SETS>;
   constexpr int W = L::W, NB = L::NB, WT = L::WT, kPair = L::kPair;
   constexpr int KS = D / 16;  // k-steps of Q.K, m-tiles of P.V
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // (the swizzles count from here)
   const int hgrp = blockIdx.x, g = blockIdx.y;
   const int kv0 = hgrp * HG;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::off_bar);
   uint64_t* empty = full + NS;
   uint64_t* qfree = empty + NS;
-  uint64_t* hbar = qfree + 2;  // kSteps per (head, query set): the warps of a row's state
+  uint64_t* hbar = qfree + 2;  // one per consumer warp
   RangeInfo* ri = reinterpret_cast<RangeInfo*>(smem + L::off_misc);
   static_assert(sizeof(RangeInfo) <= 64, "RangeInfo fits its shared-memory slot");
   int64_t* sm_scan = reinterpret_cast<int64_t*>(smem + L::off_misc + 64);
@@ -160,22 +158,72 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&qfree[0], kConsumers);
     mbar_init(&qfree[1], kConsumers);
-    for (int i = 0; i < L::kRows; ++i) {
-      mbar_init(&hbar[i * L::kSteps], WT);  // (m, l) of every warp written
-      for (int k = 1; k < L::kSteps; ++k)   // step k: half of the rest wrote its O
-        mbar_init(&hbar[i * L::kSteps + k], (WT >> k) > 0 ? WT >> k : 1);
-    }
+    // a state's first warp: its buffers are free; the others: its O is written
+    for (int i = 0; i < kConsumers; ++i) mbar_init(&hbar[i], i % WT == 0 && WT > 1 ? WT / 2 : 1);
     fence_mbar_init();
   }
   if (threadIdx.x == 32) {
     prefetch_tensormap(&tmk);
     prefetch_tensormap(&tmv);
   }
+  __syncthreads();  // the barriers are set up
+  const int q_buf = HG * a.n_rep * D * 2;  // bytes of one q buffer
   wait_prerequisites();
-  find_share<kThreads, T>(a, g, kv0, HG, ri, sm_scan);  // includes __syncthreads
   launch_dependents();
-  const int64_t start = ri->start, end = ri->end;
-  if (start >= end) return;
+  // The share of this CTA. Batches of up to 256 sequences: by the producer
+  // alone, 8 sequences a lane, without a block-wide scan (the merge kernel sums
+  // the tile prefix itself then); the rows of empty sequences by the others.
+  constexpr int kEach = 8;
+  if (a.B <= 32 * kEach) {
+    if (warp == 0) {
+      int64_t sum = 0;
+      int n[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int sb = lane * kEach + i;
+        n[i] = sb < a.B ? a.context_lens[sb] : 0;
+      }
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int c = clamp_ctx(n[i], a);
+        bad = bad || c != n[i];
+        n[i] = (c + kTile - 1) / kTile;
+        sum += n[i];
+      }
+      if (bad) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
+      int64_t incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const int64_t total = __shfl_sync(kFull, incl, 31);
+      const int G = shares_used(total, a.G);
+      const int64_t from = g < G ? share_start(g, total, G) : total;
+      const int64_t to = g < G ? share_start(g + 1, total, G) : total;
+      int64_t p = incl - sum;
+      if (sum > 0 && p <= from && from < incl) {  // one lane, where the share is not empty
+        int i = 0;
+#pragma unroll
+        for (int k = 0; k < kEach - 1; ++k)
+          if (i == k && from >= p + n[k]) p += n[k], ++i;
+        ri->b_first = lane * kEach + i;
+        ri->p_first = p;
+      }
+      if (lane == 0) ri->start = from, ri->end = to;
+      __syncwarp();
+    } else if (g == 0) {
+      for (int sb = warp - 1; sb < a.B; sb += kConsumers) {
+        if (clamp_ctx(a.context_lens[sb], a) != 0) continue;
+        T* o = reinterpret_cast<T*>(a.out) + sb * a.out_stride +
+               static_cast<int64_t>(kv0) * a.n_rep * D;
+        for (int i = lane; i < HG * a.n_rep * D; i += 32) o[i] = DT<T>::from_f(0.f);
+      }
+    }
+  } else {
+    find_share<kThreads, T>(a, g, kv0, HG, ri, sm_scan);
+  }
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -184,9 +232,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // first lane; then, item by item, the lanes of an item issue their own
     // copies and store their own scales, so that little is left to do between
     // a stage falling free and its copies.
-    int b = ri->b_first;
-    int64_t pb = ri->p_first;
-    int nb = tiles_of(a, b);
+    const int64_t start = ri->start, end = ri->end;
+    int b = 0, nb = 0;
+    int64_t pb = 0;
+    if (start < end) {
+      b = ri->b_first;
+      pb = ri->p_first;
+      nb = tiles_of(a, b);
+    }
     int seg = -1;  // segments started before this batch, less one
     uint32_t slot = 0, par = 1;
     bool abort = false;
@@ -279,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == k) {
             desc[slot] = it;
             if (q_bulk && seg_start)
-              bulk_load(smem + L::off_q + (kseg & 1) * L::kQBuf,
+              bulk_load(smem + L::off_q + (kseg & 1) * q_buf,
                         reinterpret_cast<const T*>(a.q) + lb * a.q_stride +
                             static_cast<int64_t>(kv0 * a.n_rep) * D,
                         qrows, &full[slot]);
@@ -354,97 +407,79 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t flushes = 0;
 
   // Combine the WT states of the finished segment and write its rows: the
-  // output (whole sequences) or a normalised fp32 piece. (m, l) are exchanged
-  // first, so every warp brings its O to the common scale itself; then in each
-  // step the upper half of the remaining warps hands its O to the lower half
-  // through the buffer it last read (the first step: the reader's own).
+  // output (whole sequences) or a normalised fp32 piece. In each step the
+  // upper half of the remaining warps hands its (m, l) and O to the lower half
+  // and is done; the buffer it writes is the one it last read (in the first
+  // step the reader's own, once its readers of the last segment are through).
   auto flush = [&]() {
-    uint64_t* bar = hbar + row * L::kSteps;
+    uint64_t* bar = hbar + first;
+    float2* ml = reinterpret_cast<float2*>(smem + L::off_ml) + first * 8 + qd;
+    // 16-byte pieces of a lane's D / 8 columns, rotated by its rows against bank conflicts
+    float* parts = reinterpret_cast<float*>(smem + L::off_part) + row * (WT / 2) * L::kPart +
+                   qd * D + pc * (D / 8);
+    auto piece = [&](int i) { return ((i / 2) ^ (qq & (D / 32 - 1))) * 4; };
     const uint32_t par = flushes & 1u;
-    float2* ml = reinterpret_cast<float2*>(smem + L::off_ml) + (flushes & 1u) * (L::kMl / 2);
-    ++flushes;
-    float f[2], lse[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       l[j] += __shfl_xor_sync(kFull, l[j], 4);
       l[j] += __shfl_xor_sync(kFull, l[j], 8);
       l[j] += __shfl_xor_sync(kFull, l[j], 16);
-      if (WT > 1 && grp == 0) ml[(first + part) * 8 + qd + j] = make_float2(m[j], l[j]);
     }
-    if (WT > 1) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[0]);
-      if (!__all_sync(kFull, mbar_wait_bounded(&bar[0], par))) return false;
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float M = m[j], Ls = 0.f;
-      if (WT > 1) {
-        M = -INFINITY;
-#pragma unroll 4
-        for (int i = 0; i < WT; ++i) M = fmaxf(M, ml[(first + i) * 8 + qd + j].x);
-      }
-      const float use = M == -INFINITY ? 0.f : M;
-      if (WT > 1) {
-#pragma unroll 4
-        for (int i = 0; i < WT; ++i) {
-          const float2 p = ml[(first + i) * 8 + qd + j];
-          Ls += p.y * ex2(p.x - use);
-        }
-      } else {
-        Ls = l[j] * ex2(m[j] - use);
-      }
-      // nothing attended: zero (a NaN sum is not nothing)
-      f[j] = Ls == 0.f ? 0.f : ex2(m[j] - use) / Ls;
-      lse[j] = Ls == 0.f ? -INFINITY : use + log2f(Ls) - kPShift;
-    }
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      acc[i][0] *= f[0];
-      acc[i][1] *= f[1];
-      acc[i][2] *= f[0];
-      acc[i][3] *= f[1];
-    }
-    // 16-byte pieces of a lane's D / 8 columns, rotated by its rows against bank conflicts
-    float* parts = reinterpret_cast<float*>(smem + L::off_part) + row * (WT / 2) * L::kPart +
-                   qd * D + pc * (D / 8);
-    auto piece = [&](int i) { return ((i / 2) ^ (qq & (D / 32 - 1))) * 4; };
     int mine = part >= WT / 2 ? part - WT / 2 : part;  // buffer of this warp
-    int step = 1;
-    for (int h = WT / 2; h > 0; h >>= 1, ++step) {
+    if (WT > 1 && part >= WT / 2 && flushes > 0 &&
+        !__all_sync(kFull, mbar_wait_bounded(&bar[0], par ^ 1u)))
+      return false;
+    ++flushes;
+    for (int h = WT / 2; h > 0; h >>= 1) {
       if (part >= h) {
         float* o = parts + mine * L::kPart;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
+          if (grp == 0) ml[part * 8 + j] = make_float2(m[j], l[j]);
 #pragma unroll
           for (int i = 0; i < KS; i += 2)
             *reinterpret_cast<float4*>(o + j * D + piece(i)) =
                 make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar[step]);
+        if (lane == 0) {
+          mbar_arrive(&bar[part]);
+          if (part < WT / 2) mbar_arrive(&bar[0]);  // (a reader of the steps before)
+        }
         break;
       }
-      if (!__all_sync(kFull, mbar_wait_bounded(&bar[step], par))) return false;
-      // warp part + h wrote the buffer it last read: its own place's in the
-      // first step, then the one it read in the step before
+      if (!__all_sync(kFull, mbar_wait_bounded(&bar[part + h], par))) return false;
       mine = h == WT / 2 ? part : mine + h;
       const float* o = parts + mine * L::kPart;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        const float2 other = ml[(part + h) * 8 + j];
+        const float M = fmaxf(m[j], other.x);
+        const float use = M == -INFINITY ? 0.f : M;
+        const float f = ex2(m[j] - use), e = ex2(other.x - use);
+        l[j] = l[j] * f + other.y * e;
+        m[j] = M;
 #pragma unroll
         for (int i = 0; i < KS; i += 2) {
           const float4 x = *reinterpret_cast<const float4*>(o + j * D + piece(i));
-          acc[i][j] += x.x;
-          acc[i][j + 2] += x.y;
-          acc[i + 1][j] += x.z;
-          acc[i + 1][j + 2] += x.w;
+          acc[i][j] = acc[i][j] * f + x.x * e;
+          acc[i][j + 2] = acc[i][j + 2] * f + x.y * e;
+          acc[i + 1][j] = acc[i + 1][j] * f + x.z * e;
+          acc[i + 1][j + 2] = acc[i + 1][j + 2] * f + x.w * e;
         }
+      }
     }
     if (part == 0) {
+      if (WT > 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[0]);
+      }
       const int64_t pslot = static_cast<int64_t>(kvh) * a.ws_slots + seg_unit + seg_b;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int n = n0 + qd + j;
+        // nothing attended: zero (a NaN sum is not nothing)
+        const float f = l[j] == 0.f ? 0.f : 1.f / l[j];
         if (qd + j >= nq) continue;
         if (seg_whole) {
           T* dst = reinterpret_cast<T*>(a.out) + seg_b * a.out_stride +
@@ -452,17 +487,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < KS; i += 4)
             *reinterpret_cast<uint4*>(dst + 2 * i) =
-                make_uint4(pack2<T>(acc[i][j], acc[i][j + 2]),
-                           pack2<T>(acc[i + 1][j], acc[i + 1][j + 2]),
-                           pack2<T>(acc[i + 2][j], acc[i + 2][j + 2]),
-                           pack2<T>(acc[i + 3][j], acc[i + 3][j + 2]));
+                make_uint4(pack2<T>(acc[i][j] * f, acc[i][j + 2] * f),
+                           pack2<T>(acc[i + 1][j] * f, acc[i + 1][j + 2] * f),
+                           pack2<T>(acc[i + 2][j] * f, acc[i + 2][j + 2] * f),
+                           pack2<T>(acc[i + 3][j] * f, acc[i + 3][j + 2] * f));
         } else {
           float* dst = a.ws_o + (pslot * a.n_rep + n) * D + pc * (D / 8);
 #pragma unroll
           for (int i = 0; i < KS; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) =
-                make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
-          if (grp == 0) a.ws_lse[pslot * a.n_rep + n] = lse[j];
+                make_float4(acc[i][j] * f, acc[i][j + 2] * f, acc[i + 1][j] * f,
+                            acc[i + 1][j + 2] * f);
+          if (grp == 0)
+            a.ws_lse[pslot * a.n_rep + n] =
+                l[j] == 0.f ? -INFINITY : m[j] + log2f(l[j]) - kPShift;
         }
       }
     }
@@ -499,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (hr < a.n_rep) {
         if (q_bulk) {
           const uint4* src = reinterpret_cast<const uint4*>(
-              smem + L::off_q + buf * L::kQBuf + (head * a.n_rep + hr) * D * 2);
+              smem + L::off_q + buf * q_buf + (head * a.n_rep + hr) * D * 2);
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -545,17 +583,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&qfree[buf]);
       }
     }
-    // this warp's neighbouring tiles of the item
+    // this warp's tiles of the item (short items are spread over the warps)
     int nv[kPair];
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
-      const int w = part * kPair + u;
+      const int w = u * WT + part;
       nv[u] = ((it.flags >> w) & 1) ? max(0, min(kTile, it.ntok - w * kTile)) : 0;
     }
     if (nv[0] | nv[kPair - 1]) {
-      const uint32_t base = smem_u32(smem + slot * L::kStage + part * (kPair * L::kTileBytes)) +
+      const uint32_t base = smem_u32(smem + slot * L::kStage + part * L::kTileBytes) +
                             head * L::kRegion;
-      const float* sc = scales + slot * L::kScales + part * (kPair * NB * 2 * HG) + head;
+      constexpr int kApart = WT * L::kTileBytes;  // from one of its tiles to the next
+      const float* sc = scales + slot * L::kScales + part * (NB * 2 * HG) + head;
       // scales of each tile's first and second 8 tokens (0 where there are none)
       float ks[kPair][2], vs[kPair][2];
 #pragma unroll
@@ -563,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const bool any = nv[u] > (NB == 2 ? 8 * i : 0);
-          const float* q = sc + (u * NB + (NB == 2 ? i : 0)) * 2 * HG;
+          const float* q = sc + (u * WT * NB + (NB == 2 ? i : 0)) * 2 * HG;
           ks[u][i] = any ? q[0] : 0.f;
           vs[u][i] = any ? q[HG] : 0.f;
         }
@@ -578,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < D / 64; ++c)
 #pragma unroll
         for (int u = 0; u < kPair; ++u) {
-          const uint32_t kb = base + u * L::kTileBytes + koff[c];
+          const uint32_t kb = base + u * kApart + koff[c];
           const uint4 x = lds128(kb), y = lds128(kb + kHalf);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -596,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t vw[kPair][4][VW];
 #pragma unroll
       for (int u = 0; u < kPair; ++u) {
-        const uint32_t vb0 = base + u * L::kTileBytes + L::kSide;
+        const uint32_t vb0 = base + u * kApart + L::kSide;
         const uint32_t at[4] = {vb0 + va, vb0 + vb, vb0 + kHalf + va, vb0 + kHalf + vb};
         const int tk[4] = {ta, tb, ta + 8, tb + 8};
 #pragma unroll
@@ -727,7 +766,7 @@ int run_q8(const CallQ8* call) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(call->a->Hkv / HG, call->a->G);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = L::kAlloc;
+  cfg.dynamicSmemBytes = L::bytes(call->a->n_rep);
   cfg.stream = call->s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -179,6 +179,7 @@ def set_decode_path(path: int) -> None:
     3 = TMA kernel with one copy per (kv head, column half)."""
     check(_lib.load().ir_set_decode_path(path))
     _plans.clear()   # cached workspace sizes depend on the kernel choice
+    _decode_q8_plans.clear()
 
 
 # --- pool scatter / gather ----------------------------------------------------

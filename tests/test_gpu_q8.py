@@ -562,3 +562,181 @@ def test_prompt_then_decode_steps(fmt):
     back = irb.cache_gather_q8(kp, ks, dev(slots), bs, torch.float32)
     unit = ks.max().item() * (0.5 if fmt == "int8" else 16)
     assert (back - k.float()).abs().max().item() <= 2 * unit
+
+
+# ---------------------------------------------------------------- pool, seam, streams, graphs
+
+
+@pytest.mark.parametrize("kv", [torch.float8_e4m3fn, torch.int8])
+def test_pool_class_and_paged_attention(kv):
+    """``paged_attention`` on a two-layer 8-bit pool: a packed frame, then a decode
+    step, as the direct calls on the same codes give them."""
+    from oracle import paged_attention_np as orc
+
+    rng = np.random.default_rng(4)
+    h, hkv, d, bs, nb = 14, 2, 64, 16, 20
+    dt = torch.bfloat16
+    pool = irb.PagedKVPoolQ8(2, nb, bs, hkv, d, dt, kv)
+    assert pool.k.dtype == kv and pool.num_slots == nb * bs
+    starts, qls = [0, 0], [20, 37]
+    bt = rng.permutation(nb)[:8].reshape(2, 4).astype(np.int32)
+    fr = orc.varlen_frame(bt, starts, qls, bs)
+    n = sum(qls)
+    q = dev(rng.normal(size=(1, n, h, d))).to(dt)
+    k, v = (dev(rng.normal(size=(1, n, hkv, d))).to(dt) for _ in range(2))
+    gs = dev(fr["gather_slots"]).reshape(1, -1)
+    ws = dev(fr["write_slots"])
+    mask = dev(orc.varlen_mask(fr["q_seq_ids"], fr["q_pos"], fr["k_seq_ids"], fr["k_pos"]))
+    paged = irb.PagedContext(pool, ws, gs)
+    out = irb.paged_attention(q, k, v, paged, mask, 1, d ** -0.5, h // hkv)
+    q_start = dev(np.array([0, 20, 57], np.int32))
+    ctx = dev(np.array(qls, np.int32))
+    want = irb.paged_prefill_q8(q[0], *pool.layer(1), dev(bt), ctx, q_start, d ** -0.5, bs)
+    assert torch.equal(out[0], want)
+    back = pool.gather(1, gs)
+    assert back[0].shape == (1, n, hkv, d) and back[0].dtype == dt
+    assert not pool.k[0].view(torch.int8).any()   # the other layer is untouched
+    # each row is off by its quantisation alone: half a code unit
+    kf = k[0].float()
+    unit = 2.0 ** -4 * kf.abs() + 2.0 ** -10 * pool.k_scale[1].max() if kv != torch.int8 else \
+        pool.k_scale[1].max() / 2
+    rows = irb.cache_gather_q8(pool.k[1], pool.k_scale[1], ws, bs, torch.float32)
+    assert ((rows - kf).abs() <= unit).all()
+    # a decode step for both sequences
+    ctx1 = np.array(qls, np.int32) + 1
+    t = int(ctx1.max())
+    gs1 = dev(orc.gather_slots_from_tables(bt, ctx1, bs, t))
+    m1 = dev(orc.decode_mask(ctx1, t))
+    ws1 = dev(wl.tail_slots(bt, ctx1, bs))
+    q1 = dev(rng.normal(size=(2, 1, h, d))).to(dt)
+    k1, v1 = (dev(rng.normal(size=(2, 1, hkv, d))).to(dt) for _ in range(2))
+    got = irb.paged_attention(q1, k1, v1, irb.PagedContext(pool, ws1, gs1), m1, 1, d ** -0.5,
+                              h // hkv)
+    want = irb.paged_decode_q8(q1[:, 0], *pool.layer(1), dev(bt), dev(ctx1), d ** -0.5, bs)
+    assert torch.equal(got[:, 0], want)
+
+
+def test_pool_class_refusals():
+    with pytest.raises(ValueError):
+        irb.PagedKVPoolQ8(1, 2, 16, 2, 64, torch.bfloat16, device="cpu")
+    with pytest.raises(irb.UnsupportedShape):
+        irb.PagedKVPoolQ8(1, 2, 16, 2, 64, torch.bfloat16, torch.uint8)
+    with pytest.raises(irb.UnsupportedShape):
+        irb.PagedKVPoolQ8(1, 2, 16, 2, 64, torch.float64)
+
+
+def test_python_refusals():
+    rng = np.random.default_rng(0)
+    codes, scale = make_pool(rng, 4, 16, 2, 64, "e4m3")
+    p, sc = codes_to(codes, "e4m3"), dev(scale.astype(np.float32))
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=DEV)
+    slots = dev(np.arange(3))
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    bt, ctx = torch.zeros(2, 2, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    qs = dev(np.array([0, 1, 2], np.int32))
+    write = lambda **o: irb.cache_write_q8(*{**dict(k=k, v=k, kp=p, vp=p, ks=sc, vs=sc, s=slots,  # noqa: E731
+                                                    bs=16), **o}.values())
+    decode = lambda **o: irb.paged_decode_q8(*{**dict(q=q, kp=p, vp=p, ks=sc, vs=sc, bt=bt, c=ctx,  # noqa: E731
+                                                      f=0.1, bs=16), **o}.values())
+    for bad in (dict(ks=sc.double()), dict(ks=sc[:2]), dict(vs=sc.t().contiguous()), dict(bs=12),
+                dict(bs=0), dict(vp=codes_to(codes, "int8")), dict(kp=p[:, :1]), dict(vp=p[:48])):
+        with pytest.raises((ValueError, irb.InfraredB200Error)):
+            write(**bad)
+        with pytest.raises((ValueError, irb.InfraredB200Error)):
+            decode(**bad)
+    for bad in (dict(k=k.half()), dict(s=slots.int()), dict(s=dev(np.arange(4))), dict(k=k.double()),
+                dict(k=k.transpose(1, 2).contiguous().transpose(1, 2)), dict(s=slots.cpu())):
+        with pytest.raises((ValueError, RuntimeError)):
+            write(**bad)
+    for bad in (dict(q=q[:1]), dict(q=q[0]), dict(bt=bt.long()), dict(c=ctx[:1]), dict(q=q.double()),
+                dict(q=torch.zeros(2, 3, 64, dtype=q.dtype, device=DEV)), dict(bt=bt.cpu())):
+        with pytest.raises((ValueError, irb.InfraredB200Error)):
+            decode(**bad)
+    with pytest.raises(ValueError):
+        irb.paged_decode_q8(q, p, p, sc, sc, bt, ctx, 0.1, 16, out=torch.empty(2, 4, 65, device=DEV))
+    with pytest.raises(ValueError):
+        irb.paged_decode_q8(q, p, p, sc, sc, bt, ctx, 0.1, 16,
+                            ws=torch.empty(16, dtype=torch.uint8, device=DEV))
+    with pytest.raises(ValueError):
+        irb.paged_prefill_q8(q, p, p, sc, sc, bt, ctx, qs[:2], 0.1, 16)
+    with pytest.raises(ValueError):
+        irb.cache_gather_q8(p, sc, slots.int(), 16, torch.float32)
+
+
+def test_kernel_choice_can_change_between_equal_calls():
+    """The same call with the CUDA-core kernel asked for in between."""
+    w = _with_lengths(5, [600, 33, 1], 14, 2, 64, 16)
+    a = check_decode(w, "e4m3", torch.bfloat16, 2)
+    ops.set_decode_path(1)
+    try:
+        b = check_decode(w, "e4m3", torch.bfloat16, 1)
+    finally:
+        ops.set_decode_path(0)
+    c = check_decode(w, "e4m3", torch.bfloat16, 2)
+    assert torch.equal(a, c) and a.shape == b.shape
+
+
+@pytest.mark.parametrize("n", [9, 1500])
+def test_write_and_gather_on_a_side_stream_and_in_a_graph(n):
+    rng = np.random.default_rng(n)
+    codes, scale, rows, slots = _write_case(rng, n, 2, 64, 16, 100, "e4m3", torch.bfloat16)
+    want, ws = codes.copy(), scale.copy()
+    q8.write(want, ws, host(rows[0]), slots, 16, "e4m3")
+    s = dev(slots.astype(np.int64))
+
+    def fresh():
+        return (codes_to(codes, "e4m3"), codes_to(codes, "e4m3"),
+                dev(scale.astype(np.float32)), dev(scale.astype(np.float32)))
+
+    side = torch.cuda.Stream()
+    kp, vp, ks, vs = fresh()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        irb.cache_write_q8(rows[0], rows[1], kp, vp, ks, vs, s, 16)
+        got = irb.cache_gather_q8(kp, ks, s, 16, torch.float32)
+    side.synchronize()
+    np.testing.assert_array_equal(host(kp), want)
+    np.testing.assert_array_equal(host(got), q8.values(want, ws, 16)[slots])
+    # captured, with other rows replayed through the same buffers
+    kp, vp, ks, vs = fresh()
+    k2, v2 = torch.zeros_like(rows[0]), torch.zeros_like(rows[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        irb.cache_write_q8(k2, v2, kp, vp, ks, vs, s, 16)
+        got = irb.cache_gather_q8(kp, ks, s, 16, torch.float32)
+    kp.view(torch.int8).copy_(fresh()[0].view(torch.int8))
+    ks.copy_(fresh()[2])
+    for rep in range(2):   # the second replay finds the scales grown and changes nothing
+        k2.copy_(rows[0])
+        v2.copy_(rows[1])
+        g.replay()
+        torch.cuda.synchronize()
+        if rep == 0:
+            np.testing.assert_array_equal(host(kp), want)
+            np.testing.assert_array_equal(host(ks), ws)
+        np.testing.assert_array_equal(host(got), q8.values(want, ws, 16)[slots])
+
+
+def test_a_long_table_passes_32_bits_of_bytes():
+    """Codes beyond 2^31 bytes into the pool, and rows of the expanded pool beyond it."""
+    hkv, d, bs = 8, 128, 16
+    nb = (2 ** 31 // (hkv * d)) // bs + 40   # the last blocks lie past 2^31 bytes
+    kp = torch.zeros(nb * bs, hkv, d, dtype=torch.int8, device=DEV).view(torch.float8_e4m3fn)
+    vp = torch.zeros_like(kp.view(torch.int8)).view(torch.float8_e4m3fn)
+    ks, vs = torch.zeros(nb, hkv, device=DEV), torch.zeros(nb, hkv, device=DEV)
+    rng = np.random.default_rng(1)
+    n = 100
+    bt = np.array([[nb - 1, nb - 9, nb - 4, 3, nb - 2, nb - 30, nb - 7]], np.int32)
+    p = np.arange(n)
+    slots = bt[0, p // bs].astype(np.int64) * bs + p % bs
+    k, v = (dev(rng.normal(size=(n, hkv, d))).to(torch.bfloat16) for _ in range(2))
+    irb.cache_write_q8(k, v, kp, vp, ks, vs, dev(slots), bs)
+    kf = irb.cache_gather_q8(kp, ks, dev(slots), bs, torch.float32)
+    vf = irb.cache_gather_q8(vp, vs, dev(slots), bs, torch.float32)
+    assert ((kf - k.float()).abs() <= 2.0 ** -4 * k.float().abs() + 2.0 ** -10 * ks.max()).all()
+    q = dev(rng.normal(size=(1, 16, d))).to(torch.bfloat16)
+    ctx = dev(np.array([n], np.int32))
+    out = irb.paged_decode_q8(q, kp, vp, ks, vs, dev(bt), ctx, d ** -0.5, bs)
+    want, weighted, size = q8.attend(host(q[0]), host(kf), host(vf), d ** -0.5)
+    assert (np.abs(host(out[0]) - want) <=
+            attend_tolerance(want, weighted, size, n, d, torch.bfloat16, True)).all()
