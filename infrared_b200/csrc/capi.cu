@@ -432,7 +432,9 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
     if (!make_pool_map_q8(&tmk, k_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg) ||
         !make_pool_map_q8(&tmv, v_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg))
       return fail(IR_ERR_CUDA, "cuTensorMapEncodeTiled failed");
-    e = irb::launch_decode_q8(tmk, tmv, a, s->dtype, fmt, stream);
+    // (launches its merge itself)
+    return cuda_status(irb::launch_decode_q8(tmk, tmv, a, s->dtype, fmt, stream),
+                       "8-bit decode kernel launch");
   } else if (plan.path == 2) {
     CUtensorMap tmk, tmv;
     const int rows = s->block_size == 8 ? 8 : 16;

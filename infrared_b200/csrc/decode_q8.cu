@@ -739,6 +739,141 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- merge
+//
+// The pieces of a row (query head of a sequence) that several CTAs hold,
+// combined by W warps, every warp loading up to U pieces at once and lane i
+// columns 4 i .. 4 i + 3. The grid should be resident while the decode CTAs
+// still run, so that nothing but the pieces' round trip remains after them:
+// beside a decode CTA an SM has a quarter of its registers and 2-4 KB of
+// shared memory left. Hence rows of one group in one CTA without shared
+// memory where a row has few pieces (W = 1), and four warps a row otherwise.
+// Which pieces a row has follows from the context lengths, summed by every
+// warp before the wait for batches of up to 256 (else the decode grid's prefix).
+template <typename T, int W, int U>
+__global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) merge_q8_kernel(const DecodeArgs a) {
+  launch_dependents();
+  constexpr int kSide = W > 1 ? W : 1;
+  __shared__ float4 s_acc[W > 1 ? W : 1][W > 1 ? 32 : 1];
+  __shared__ float2 s_ms[kSide];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x, kvh = blockIdx.y;
+  const bool early = a.B <= 256;
+  int64_t total = 0, pb = 0, nb = 0;
+  int glo = 0, parts = 0;
+  auto units = [&]() {
+    if (nb > 0) piece_range(pb, nb, total, shares_used(total, a.G), &glo, &parts);
+  };
+  if (early) {
+    for (int i = lane; i < a.B; i += 32) {
+      const int64_t t = tiles_of(a, i);
+      total += t;
+      if (i < b) pb += t;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(kFull, total, o);
+      pb += __shfl_xor_sync(kFull, pb, o);
+    }
+    nb = tiles_of(a, b);
+    units();
+  }
+  wait_prerequisites();
+  if (!early) {
+    pb = a.ws_prefix[b];
+    nb = a.ws_prefix[b + 1] - pb;
+    total = a.ws_prefix[a.B];
+    units();
+  }
+  if (nb <= 0 || parts == 1) return;  // empty, or written whole by its CTA
+  const bool active = lane * 4 < a.D;
+  // W = 1: a warp per row of the group in turns; else the CTA's row is in z
+  const int step = W == 1 ? blockDim.x >> 5 : a.n_rep;
+  for (int n = W == 1 ? warp : blockIdx.z; n < a.n_rep; n += step) {
+    const int64_t base = static_cast<int64_t>(kvh) * a.ws_slots + glo + b;
+    const float* lse = a.ws_lse + base * a.n_rep + n;
+    const float* o = a.ws_o + (base * a.n_rep + n) * a.D + lane * 4;
+    const int64_t ostride = static_cast<int64_t>(a.n_rep) * a.D;
+    float M = -INFINITY, S = 0.f;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = W == 1 ? 0 : warp; i0 < parts; i0 += W * U) {
+      float li[U];
+      float4 oi[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * W;
+        li[u] = -INFINITY;
+        oi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < parts) {
+          li[u] = __ldcg(lse + static_cast<int64_t>(i) * a.n_rep);
+          if (active) oi[u] = __ldcg(reinterpret_cast<const float4*>(o + i * ostride));
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, li[u]);
+      const float use = top == -INFINITY ? 0.f : top;
+      const float c = ex2(M - use);
+      S *= c;
+      r.x *= c, r.y *= c, r.z *= c, r.w *= c;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = ex2(li[u] - use);  // (0 for a piece with nothing attended)
+        S += w;
+        r.x += w * oi[u].x, r.y += w * oi[u].y, r.z += w * oi[u].z, r.w += w * oi[u].w;
+      }
+      M = top;
+    }
+    if (W > 1) {
+      s_acc[warp][lane] = r;
+      if (lane == 0) s_ms[warp] = make_float2(M, S);
+      __syncthreads();
+      if (warp != 0) return;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ms[w].x);
+      const float use = top == -INFINITY ? 0.f : top;
+      S = 0.f;
+      r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float c = ex2(s_ms[w].x - use);
+        const float4 x = s_acc[w][lane];
+        S += c * s_ms[w].y;
+        r.x += c * x.x, r.y += c * x.y, r.z += c * x.z, r.w += c * x.w;
+      }
+    }
+    if (active) {
+      const float f = S == 0.f ? 0.f : 1.f / S;  // (a NaN sum is not nothing)
+      T* dst = reinterpret_cast<T*>(a.out) + b * a.out_stride +
+               static_cast<int64_t>(kvh * a.n_rep + n) * a.D + lane * 4;
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(pack2<T>(r.x * f, r.y * f), pack2<T>(r.z * f, r.w * f));
+    }
+  }
+}
+
+template <typename T>
+int launch_merge_q8(const DecodeArgs& a, cudaStream_t s) {
+  // a sequence of average length spans about G / B shares (+ 1)
+  const int pieces = a.G / (a.B > 0 ? a.B : 1) + 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = s;
+  if (pieces <= 8) {
+    cfg.gridDim = dim3(a.B, a.Hkv);
+    cfg.blockDim = dim3(32 * (a.n_rep < 8 ? a.n_rep : 8));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, merge_q8_kernel<T, 1, 4>, a));
+  }
+  cfg.gridDim = dim3(a.B, a.Hkv, a.n_rep);
+  cfg.blockDim = dim3(32 * 4);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, merge_q8_kernel<T, 4, 10>, a));
+}
+
 // ---------------------------------------------------------------- dispatch
 
 struct CallQ8 {
@@ -829,8 +964,10 @@ int launch_decode_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, const Decod
   // q rows of a head group move as one bulk copy when 16-byte aligned
   const int q_bulk = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && (a.q_stride * 2) % 16 == 0;
   const CallQ8 call{&tmk, &tmv, &a, q_bulk, stream};
-  return dtype == IR_DTYPE_BF16 ? by_code<__nv_bfloat16>(fmt, &call)
-                                : by_code<__half>(fmt, &call);
+  const bool bf16 = dtype == IR_DTYPE_BF16;
+  const int e = bf16 ? by_code<__nv_bfloat16>(fmt, &call) : by_code<__half>(fmt, &call);
+  if (e) return e;
+  return bf16 ? launch_merge_q8<__nv_bfloat16>(a, stream) : launch_merge_q8<__half>(a, stream);
 }
 
 }  // namespace irb

@@ -90,7 +90,8 @@ int decode_generic_occupancy(int dtype, int D, int fmt);
 // decode_q8.cu: 8-bit pools, 16-bit q, D in {64, 128}, group <= 16, bs == 8 or
 // bs % 16 == 0. One CTA (per SM) covers q8_head_group(Hkv, group) kv heads; the
 // maps view a pool as (D bytes, slots, Hkv) with boxes {D, min(bs, 16), head
-// group} and a swizzle as wide as the row.
+// group} and a swizzle as wide as the row. The merge of split rows is launched
+// behind.
 int q8_head_group(int num_kv_heads, int n_rep);
 int launch_decode_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, const DecodeArgs& a,
                      int dtype, int fmt, cudaStream_t stream);

@@ -788,13 +788,26 @@ _write_plans, _gather_plans, _decode_q8_plans, _prefill_q8_plans, _norm_plans = 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _stream
 
 
-def _issue(dev: int, fn, *args) -> None:
-    """One library call on device ``dev``'s current stream (its last argument)."""
-    if dev == torch.cuda.current_device():
-        check(fn(*args, _raw_stream(dev)))
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_err_ptrs: dict[int, int] = {}   # device -> address of its error word (allocated once)
+
+
+def _issue(dev: int, fn, args) -> None:
+    """One library call on device ``dev``; ``args`` end with its stream."""
+    if dev == _current_device():
+        rc = fn(*args)
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, _raw_stream(dev)))
+            rc = fn(*args)
+    if rc:
+        check(rc)
+
+
+def _err_ptr(dev: int) -> int:
+    p = _err_ptrs.get(dev)
+    if p is None:
+        p = _err_ptrs[dev] = error_flag(dev).data_ptr()
+    return p
 
 
 def kv_format(dtype: torch.dtype) -> int:
@@ -885,9 +898,10 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
         return
     # (of this call alone: PyTorch's allocator orders its reuse on the stream)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=k_pool.device) if nbytes else None
-    _issue(dev, fn, k.data_ptr(), v.data_ptr(), ks, vs, k_pool.data_ptr(), v_pool.data_ptr(),
-           k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), n, hkv, d, block_size,
-           num_slots, code, fmt, _ptr(ws), nbytes, error_flag(dev).data_ptr())
+    _issue(dev, fn, (k.data_ptr(), v.data_ptr(), ks, vs, k_pool.data_ptr(), v_pool.data_ptr(),
+                     k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), n, hkv, d,
+                     block_size, num_slots, code, fmt, _ptr(ws), nbytes, _err_ptr(dev),
+                     _raw_stream(dev)))
 
 
 def cache_gather_q8(pool: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor,
@@ -910,8 +924,9 @@ def cache_gather_q8(pool: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor
     out = torch.empty(shape, dtype=dtype, device=pool.device)
     if n:
         slots = slots if slots.is_contiguous() else slots.contiguous()
-        _issue(dev, fn, out.data_ptr(), pool.data_ptr(), scale.data_ptr(), slots.data_ptr(), n, hkv,
-               d, block_size, num_slots, code, fmt, error_flag(dev).data_ptr())
+        _issue(dev, fn, (out.data_ptr(), pool.data_ptr(), scale.data_ptr(), slots.data_ptr(), n,
+                         hkv, d, block_size, num_slots, code, fmt, _err_ptr(dev),
+                         _raw_stream(dev)))
     return out
 
 
@@ -999,10 +1014,10 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ws = _scratch(ws, nbytes, q)
-    _issue(dev, fn, out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-           k_scale.data_ptr(), v_scale.data_ptr(), fmt, block_tables.data_ptr(),
-           context_lens.data_ptr(), s, ws.data_ptr(), ws.numel() * ws.element_size(),
-           error_flag(dev).data_ptr())
+    _issue(dev, fn, (out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                     k_scale.data_ptr(), v_scale.data_ptr(), fmt, block_tables.data_ptr(),
+                     context_lens.data_ptr(), s, ws.data_ptr(), ws.numel() * ws.element_size(),
+                     _err_ptr(dev), _raw_stream(dev)))
     return out
 
 
@@ -1037,10 +1052,11 @@ def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     # (asked each time: it depends on the path chosen by set_prefill_path)
     nbytes = lib.ir_paged_prefill_q8_workspace_size(s)
     ws = _scratch(ws, max(nbytes, 256), q)
-    _issue(dev, lib.ir_paged_prefill_q8, out.data_ptr(), q.data_ptr(), k_pool.data_ptr(),
-           v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), fmt,
-           block_tables.data_ptr(), context_lens.data_ptr(), q_start.data_ptr(), s, ws.data_ptr(),
-           ws.numel() * ws.element_size(), error_flag(dev).data_ptr())
+    _issue(dev, lib.ir_paged_prefill_q8,
+           (out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), fmt, block_tables.data_ptr(),
+            context_lens.data_ptr(), q_start.data_ptr(), s, ws.data_ptr(),
+            ws.numel() * ws.element_size(), _err_ptr(dev), _raw_stream(dev)))
     return out
 
 
@@ -1102,6 +1118,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, w_q: torch.Tensor | None,
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k_out is None:
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    _issue(dev, fn, q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *strides,
-           _ptr(w_q), _ptr(w_k), cos.data_ptr(), sin.data_ptr(), rs, eps, n, h, hkv, d, code)
+    _issue(dev, fn, (q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *strides,
+                     _ptr(w_q), _ptr(w_k), cos.data_ptr(), sin.data_ptr(), rs, eps, n, h, hkv, d,
+                     code, _raw_stream(dev)))
     return q_out, k_out
