@@ -509,13 +509,21 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
                        const ir_decode_shape* shape, void* workspace, size_t workspace_bytes,
                        int32_t* err_flag, ir_stream_t stream);
 
-/* ir_paged_prefill over an 8-bit pool. The blocks of the sequences' histories
- * are expanded once into a pool of shape->dtype in the workspace (two launches
- * in all), which the prefill kernel then attends over: a block's conversion is
- * paid once, not once per 128 query rows and head. In bf16 and fp32 the
- * expanded values are exact for power-of-two scales. The workspace holds one
- * layer's pool of shape->dtype and can serve every layer. */
-size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape);
+/* ir_paged_prefill over an 8-bit pool, by one of
+ *   2 (3: its CTA-pair form) 16-bit q with 16-byte aligned rows: the blocks of
+ *     the sequences' histories are expanded once into rows of shape->dtype in
+ *     the workspace, which the tensor-core kernel attends over: a block's
+ *     conversion is paid once, not once per 128 query rows and head. Exact in
+ *     bf16 for power-of-two scales. The workspace holds the histories (or one
+ *     layer's pool) in shape->dtype and can serve every layer;
+ *   4 everything else: fp32 tiles on the CUDA cores, codes read directly;
+ *   1 as 4 for at most 4 query rows per sequence: every row decoded as its own
+ *     sequence (ir_paged_decode_q8).
+ * Values of K or V at positions that a row does not attend change nothing in it,
+ * NaN included. ir_set_prefill_path(2 or 3) asks for the tensor cores, 1 for
+ * the others. */
+size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape, int kv_format);
+int ir_paged_prefill_q8_plan(const ir_prefill_shape* shape, int kv_format, int* path);
 int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
                         const float* k_scale, const float* v_scale, int kv_format,
                         const int32_t* block_tables, const int32_t* context_lens,

@@ -24,7 +24,8 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "libinfrared_b200.so"
 
 SOURCES = ["capi.cu", "cache_ops.cu", "decode_generic.cu", "decode_tma.cu", "prefill_tc.cu",
-           "peer_exchange.cu", "kv_proj.cu", "cache_q8.cu", "decode_q8.cu", "qk_norm_rope.cu"]
+           "peer_exchange.cu", "kv_proj.cu", "cache_q8.cu", "decode_q8.cu", "prefill_q8.cu",
+           "qk_norm_rope.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

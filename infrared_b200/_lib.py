@@ -165,7 +165,8 @@ _SIGNATURES = {
     "ir_paged_decode_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_int, c_void_p, c_void_p, POINTER(DecodeShape), c_void_p,
                                    c_size_t, c_void_p, c_void_p]),
-    "ir_paged_prefill_q8_workspace_size": (c_size_t, [POINTER(PrefillShape)]),
+    "ir_paged_prefill_q8_workspace_size": (c_size_t, [POINTER(PrefillShape), c_int]),
+    "ir_paged_prefill_q8_plan": (c_int, [POINTER(PrefillShape), c_int, POINTER(c_int)]),
     "ir_paged_prefill_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_int, c_void_p, c_void_p, c_void_p, POINTER(PrefillShape),
                                     c_void_p, c_size_t, c_void_p, c_void_p]),

@@ -479,6 +479,12 @@ __device__ __forceinline__ float saturate(float x) {
   return x;
 }
 
+// Whether any of four e4m3 codes is NaN (0x7f or 0xff).
+__device__ __forceinline__ bool has_nan(uint32_t w) {
+  // 0x7f + 1 carries into a byte's top bit, and nothing below it does
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
+}
+
 // 8 codes to 8 values of T, likewise (out 16-byte aligned).
 template <typename T, typename C>
 __device__ __forceinline__ void store8(T* out, uint2 codes, float s) {
@@ -574,33 +580,58 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Blocks of the sequences' histories, each to its own place in a pool of T.
+// The blocks of the sequences' histories as rows of T: with `table` null, each
+// in its own place of a pool laid out as the codes are; else sequence by
+// sequence (cap rows each), with the block table of that order. CTA (s, y) takes
+// blocks y, y + gridDim.y, ... of sequence s and writes to flags[] whether it met
+// a V that is not finite.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)
     expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp, const float* ks,
                          const float* vs, const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
-                         int max_blocks, int64_t num_blocks, int Hkv, int D, int bs) {
+                         int max_blocks, int64_t num_blocks, int Hkv, int D, int bs,
+                         int32_t* table, int64_t cap, int table_block, int* flags, int32_t* err) {
   wait_prior_grid();
   const int sq = blockIdx.x;
   const int64_t c0 = ctx[sq];
   const int pieces = Hkv * D / 8;
   const int tpr = pieces < 256 ? pieces : 256;
   const int side = blockDim.x / tpr;
+  bool nan = false;
+  if (threadIdx.x == 0 && blockIdx.y == 0 && c0 > static_cast<int64_t>(max_blocks) * bs)
+    set_err(err, IR_DEVERR_CONTEXT_LEN);
   for (int j = blockIdx.y; j < max_blocks && static_cast<int64_t>(j) * bs < c0; j += gridDim.y) {
-    const int64_t id = bt[sq * bt_stride + j];
-    if (id < 0 || id >= num_blocks) continue;  // the attention kernel reports it
+    int64_t id = bt[sq * bt_stride + j];
+    bool ok = id >= 0 && id < num_blocks;
+    if (!ok) {
+      // in place the attention kernel reports it and reads zeros
+      if (table == nullptr) continue;
+      if (threadIdx.x == 0) set_err(err, IR_DEVERR_BLOCK_ID);
+      id = 0;
+    }
+    const int64_t to = table ? sq * cap + static_cast<int64_t>(j) * bs : id * bs;
     for (int c = threadIdx.x % tpr; c < pieces; c += tpr) {
-      const float k = ks[id * Hkv + c * 8 / D], v = vs[id * Hkv + c * 8 / D];
+      const float k = ok ? ks[id * Hkv + c * 8 / D] : 0.f, v = ok ? vs[id * Hkv + c * 8 / D] : 0.f;
 #pragma unroll 4
       for (int r = threadIdx.x / tpr; r < bs; r += side) {
-        const int64_t at = (id * bs + r) * pieces + c;
-        const uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
-        const uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
-        store8<T, C>(kout + at * 8, kc, k);
-        store8<T, C>(vout + at * 8, vc, v);
+        const int64_t at = (id * bs + r) * pieces + c, dst = (to + r) * pieces + c;
+        uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
+        uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
+        if (!ok) kc = vc = make_uint2(0u, 0u);
+        if (std::is_same<C, e4m3_t>::value && (has_nan(vc.x) || has_nan(vc.y)) &&
+            static_cast<int64_t>(j) * bs + r < c0)
+          nan = true;
+        store8<T, C>(kout + dst * 8, kc, k);
+        store8<T, C>(vout + dst * 8, vc, v);
       }
+      nan = nan || !finite(v);
     }
   }
+  if (table != nullptr && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < cap / table_block; i += blockDim.x)
+      table[sq * (cap / table_block) + i] = static_cast<int32_t>(sq * (cap / table_block) + i);
+  nan = __syncthreads_or(nan);
+  if (threadIdx.x == 0) flags[static_cast<int64_t>(sq) * gridDim.y + blockIdx.y] = nan ? 1 : 0;
 }
 
 template <typename F>
@@ -720,14 +751,20 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
   });
 }
 
+int expand_flags(int S, int max_blocks, int sms) {
+  // CTAs of a sequence: eight per SM in all
+  const int y = S > 0 ? 8 * sms / S : 1;
+  return S * (y < 1 ? 1 : (y > max_blocks ? max_blocks : y));
+}
+
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
                          int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
                          int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
-                         cudaStream_t stream) {
-  if (S == 0 || max_blocks == 0) return 0;
+                         int32_t* table, int64_t cap, int table_block, int* flags, int sms,
+                         int32_t* err, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(S),
-                  static_cast<unsigned>(max_blocks < 4096 ? max_blocks : 4096));
+                  static_cast<unsigned>(expand_flags(S, max_blocks, sms) / S));
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
       using T = decltype(t);
@@ -735,7 +772,8 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
                            piece_threads(Hkv * D / 8), 0, stream, static_cast<T*>(k_out),
                            static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
                            static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride,
-                           ctx, max_blocks, num_blocks, Hkv, D, bs);
+                           ctx, max_blocks, num_blocks, Hkv, D, bs, table, cap, table_block, flags,
+                           err);
     });
   });
 }

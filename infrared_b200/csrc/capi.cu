@@ -637,10 +637,67 @@ int check_q8_rows(int64_t n, int hkv, int d, int bs, int64_t num_slots, int dtyp
   return IR_OK;
 }
 
-// Bytes of one side of the expanded pool of ir_paged_prefill_q8.
-size_t expanded_pool_bytes(const ir_prefill_shape* s) {
-  return align256(static_cast<size_t>(s->num_slots) * s->num_kv_heads * s->head_dim *
-                  elem_bytes(s->dtype));
+// How ir_paged_prefill_q8 goes about a shape.
+struct PrefillQ8Plan {
+  int path;        // 1 rows as decode rows, 2 / 3 expansion + tensor cores, 4 fp32 tiles
+  bool dense;      // the expansion lays the histories out sequence by sequence
+  int64_t cap;     // rows of a sequence there
+  int sms, flags;
+  // workspace: K, V, table, flags, or the rows path's tables and contexts
+  size_t pool, table_off, flags_off, rows_table, rows_ctx, bytes;
+};
+
+constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy per key tile
+
+// The tensor-core kernel reads an expanded pool, so the layout is free: dense
+// where that takes at most twice the pool's rows (or, for block sizes that the
+// kernel cannot read in place, up to 8 GiB), else in the blocks' own places.
+// Measured, dense against in place (blocks of 16): 4 prompts of 2048 rows 223 us
+// against 235, six sequences of up to 300 rows 36 us against 40. fp32 rows go to
+// the fp32 tile kernel, unless there are a few rows per sequence: these split
+// over the SMs as decode rows do (six single rows over 1000 keys: 44 us).
+int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
+  int rc = check_prefill_shape(s);
+  if (rc) return rc;
+  if (s->num_slots < s->block_size || s->num_slots % s->block_size != 0)
+    return fail(IR_ERR_INVALID_ARG, "num_slots must be a positive multiple of block_size");
+  *p = PrefillQ8Plan{};
+  const int e = cached(-1, sm_count_now, 0, &p->sms);
+  if (e) return cuda_status(e, "device query");
+  const int bs = s->block_size;
+  const bool half = s->dtype != IR_DTYPE_F32;
+  const bool rows_ok = half && (s->q_stride * 2) % 16 == 0 && (s->out_stride * 2) % 16 == 0;
+  p->cap = (static_cast<int64_t>(s->max_blocks) * bs + kDenseBlock - 1) / kDenseBlock * kDenseBlock;
+  const int64_t dense_rows = p->cap * s->num_seqs;
+  const int64_t row_bytes = static_cast<int64_t>(s->num_kv_heads) * s->head_dim * 2;
+  const bool in_place = bs >= 8 && (bs & (bs - 1)) == 0 && s->num_slots < INT32_MAX;
+  const bool fits = dense_rows <= 2 * s->num_slots + 4096 ||
+                    (!in_place && dense_rows <= (int64_t{8} << 30) / (2 * row_bytes));
+  p->dense = dense_rows > 0 && dense_rows < INT32_MAX && fits;
+  const bool tc = rows_ok && s->max_blocks > 0 && (p->dense || in_place);
+  if (g_prefill_path >= 2 && !(tc && (g_prefill_path == 2 || s->head_dim == 128)))
+    return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but shape not eligible");
+  const bool few = s->total_q <= 4 * static_cast<int64_t>(s->num_seqs) &&
+                   s->num_heads / s->num_kv_heads <= 16;
+  p->path = tc && g_prefill_path != 1 ? (g_prefill_path == 3 ? 3 : 2) : (few ? 1 : 4);
+  if (p->path == 2 || p->path == 3) {
+    const int64_t rows = p->dense ? dense_rows : s->num_slots;
+    p->pool = align256(static_cast<size_t>(rows) * row_bytes);
+    p->table_off = 2 * p->pool;
+    p->flags_off = p->table_off +
+                   (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
+    p->flags = s->num_seqs > 0 ? irb::expand_flags(s->num_seqs, s->max_blocks, p->sms) : 0;
+    p->bytes = p->flags_off + align256(static_cast<size_t>(p->flags) * 4);
+  } else if (p->path == 1) {
+    ir_decode_shape d = rows_shape(s);
+    Plan plan;
+    rc = make_plan(&d, &plan, fmt);
+    if (rc) return rc;
+    p->rows_table = align256(static_cast<size_t>(s->total_q) * s->max_blocks * 4);
+    p->rows_ctx = align256(static_cast<size_t>(s->total_q) * 4);
+    p->bytes = p->rows_table + p->rows_ctx + plan.bytes;
+  }
+  return IR_OK;
 }
 
 }  // namespace
@@ -1195,9 +1252,19 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
                      err_flag, stream, nullptr, nullptr, 0, kv_format, k_scale, v_scale);
 }
 
-size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape) {
-  if (check_prefill_shape(shape)) return 0;
-  return 2 * expanded_pool_bytes(shape) + align256(ir_paged_prefill_workspace_size(shape));
+size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape, int kv_format) {
+  PrefillQ8Plan p;
+  if (!kv_format_ok(kv_format) || plan_prefill_q8(shape, kv_format, &p)) return 0;
+  return p.bytes;
+}
+
+int ir_paged_prefill_q8_plan(const ir_prefill_shape* shape, int kv_format, int* path) {
+  if (!kv_format_ok(kv_format)) return fail(IR_ERR_INVALID_ARG, "unknown kv_format");
+  PrefillQ8Plan p;
+  int rc = plan_prefill_q8(shape, kv_format, &p);
+  if (rc) return rc;
+  if (path) *path = p.path;
+  return IR_OK;
 }
 
 int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
@@ -1209,27 +1276,87 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
   int rc = check_prefill_shape(s);
   if (rc) return rc;
   if (s->num_seqs == 0 || s->total_q == 0) return IR_OK;
-  if (s->num_slots < s->block_size || s->num_slots % s->block_size != 0)
-    return fail(IR_ERR_INVALID_ARG, "num_slots must be a positive multiple of block_size");
   if (!out || !q || !k_pool || !v_pool || !k_scale || !v_scale || !context_lens || !q_start ||
       (s->max_blocks > 0 && !block_tables))
     return fail(IR_ERR_INVALID_ARG, "null pointer");
   if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
     return fail(IR_ERR_INVALID_ARG, "8-bit pools must be 16-byte aligned");
-  if (!workspace || workspace_bytes < ir_paged_prefill_q8_workspace_size(s))
+  PrefillQ8Plan p;
+  rc = plan_prefill_q8(s, kv_format, &p);
+  if (rc) return rc;
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(IR_ERR_WORKSPACE, "workspace smaller than ir_paged_prefill_q8_workspace_size");
-  if (!aligned(workspace, 256))
+  if (p.bytes && !aligned(workspace, 256))
     return fail(IR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  const size_t pool = expanded_pool_bytes(s);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int e = irb::launch_expand_blocks(ws, ws + pool, k_pool, v_pool, k_scale, v_scale,
-                                          block_tables, s->bt_stride, context_lens, s->num_seqs,
-                                          s->max_blocks, s->num_slots / s->block_size,
-                                          s->num_kv_heads, s->head_dim, s->block_size, s->dtype,
-                                          kv_format, static_cast<cudaStream_t>(stream));
+  if ((p.path == 2 || p.path == 3) && !(aligned(q, 16) && aligned(out, 16))) {
+    if (g_prefill_path >= 2)
+      return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but pointers misaligned");
+    p.path = 4;
+  }
+  int e;
+  if (p.path == 1) {
+    int32_t* row_bt = reinterpret_cast<int32_t*>(ws);
+    int32_t* row_ctx = reinterpret_cast<int32_t*>(ws + p.rows_table);
+    e = irb::launch_prefill_rows(block_tables, s->bt_stride, context_lens, q_start, s->num_seqs,
+                                 s->total_q, s->max_blocks, s->max_blocks * s->block_size, row_bt,
+                                 row_ctx, err_flag, st);
+    if (e) return cuda_status(e, "prefill row tables");
+    ir_decode_shape d = rows_shape(s);
+    const size_t off = p.rows_table + p.rows_ctx;
+    return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr,
+                       0, nullptr, row_bt, row_ctx, &d, ws + off, workspace_bytes - off, err_flag,
+                       st, nullptr, nullptr, 0, kv_format, k_scale, v_scale);
+  }
+  irb::PrefillArgs a{};
+  a.q = q;
+  a.q_stride = s->q_stride;
+  a.out = out;
+  a.out_stride = s->out_stride;
+  a.block_tables = block_tables;
+  a.bt_stride = s->bt_stride;
+  a.context_lens = context_lens;
+  a.q_start = q_start;
+  a.S = s->num_seqs;
+  a.total_q = s->total_q;
+  a.H = s->num_heads;
+  a.Hkv = s->num_kv_heads;
+  a.n_rep = s->num_heads / s->num_kv_heads;
+  a.D = s->head_dim;
+  a.bs = s->block_size;
+  a.max_blocks = s->max_blocks;
+  a.num_slots = s->num_slots;
+  a.num_blocks = s->num_slots / s->block_size;
+  a.scale_log2 = s->scale * irb::kLog2e;
+  a.err = err_flag;
+  if (p.path == 4) {
+    e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, nullptr,
+                               0, p.sms, st);
+    return cuda_status(e, "8-bit prefill launch");
+  }
+  int32_t* table = p.dense ? reinterpret_cast<int32_t*>(ws + p.table_off) : nullptr;
+  int* flags = reinterpret_cast<int*>(ws + p.flags_off);
+  e = irb::launch_expand_blocks(ws, ws + p.pool, k_pool, v_pool, k_scale, v_scale, block_tables,
+                                s->bt_stride, context_lens, s->num_seqs, s->max_blocks,
+                                a.num_blocks, s->num_kv_heads, s->head_dim, s->block_size,
+                                s->dtype, kv_format, table, p.cap, kDenseBlock, flags, p.sms,
+                                err_flag, st);
   if (e) return cuda_status(e, "8-bit block expansion launch");
-  return ir_paged_prefill(out, q, ws, ws + pool, block_tables, context_lens, q_start, s,
-                          ws + 2 * pool, workspace_bytes - 2 * pool, err_flag, stream);
+  ir_prefill_shape x = *s;
+  if (p.dense) {
+    x.block_size = kDenseBlock;
+    x.max_blocks = static_cast<int>(p.cap / kDenseBlock);
+    x.bt_stride = x.max_blocks;
+    x.num_slots = p.cap * s->num_seqs;
+  }
+  rc = ir_paged_prefill(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
+                        q_start, &x, nullptr, 0, err_flag, stream);
+  if (rc) return rc;
+  // (does nothing unless the expansion flagged a V that is not finite)
+  e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, flags,
+                             p.flags, p.sms, st);
+  return cuda_status(e, "8-bit prefill launch");
 }
 
 // ---------------------------------------------------------------- q/k norm + rotation

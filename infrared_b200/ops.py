@@ -1021,13 +1021,25 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     return out
 
 
+def prefill_plan_q8(q, k_pool, block_tables, q_start, block_size, scale=1.0):
+    """``(path, workspace_bytes)`` of :func:`paged_prefill_q8` for these shapes."""
+    s = _prefill_shape(q, k_pool, block_tables, q_start, block_size, scale,
+                       q.shape[1] * q.shape[2])
+    fmt = kv_format(k_pool.dtype)
+    lib = _lib.load()
+    path = _lib.c_int()
+    check(lib.ir_paged_prefill_q8_plan(s, fmt, path))
+    return path.value, lib.ir_paged_prefill_q8_workspace_size(s, fmt)
+
+
 def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                      k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                      context_lens: torch.Tensor, q_start: torch.Tensor, scale: float,
                      block_size: int, out: torch.Tensor | None = None,
                      ws: torch.Tensor | None = None) -> torch.Tensor:
-    """:func:`paged_prefill` over an 8-bit cache (:func:`cache_write_q8`). Its
-    workspace holds one layer's pool in q's dtype (``ir_paged_prefill_q8``)."""
+    """:func:`paged_prefill` over an 8-bit cache (:func:`cache_write_q8`). With
+    16-bit q its workspace holds the histories, or the pool, in q's dtype
+    (``ir_paged_prefill_q8``)."""
     key = (_decode_q8_key(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out,
                           scale, block_size),
            q_start.shape, q_start.dtype, q_start.is_contiguous(), q_start.get_device())
@@ -1050,7 +1062,10 @@ def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     # (asked each time: it depends on the path chosen by set_prefill_path)
-    nbytes = lib.ir_paged_prefill_q8_workspace_size(s)
+    nbytes = lib.ir_paged_prefill_q8_workspace_size(s, fmt)
+    if nbytes == 0:
+        with torch.cuda.device(dev):
+            check(lib.ir_paged_prefill_q8_plan(s, fmt, None))
     ws = _scratch(ws, max(nbytes, 256), q)
     _issue(dev, lib.ir_paged_prefill_q8,
            (out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),

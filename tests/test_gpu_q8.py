@@ -461,25 +461,35 @@ def test_decode_is_deterministic_and_replays():
 # ---------------------------------------------------------------- prefill
 
 
-@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("h,hkv,d,bs,spans", [
-    (28, 4, 128, 16, [(0, 130), (17, 1), (50, 40)]), (14, 2, 64, 16, [(3, 5), (0, 1), (0, 200)]),
-    (4, 4, 128, 12, [(20, 30), (0, 7)]), (16, 1, 64, 8, [(9, 33)]),
-])
-def test_prefill(h, hkv, d, bs, spans, dtype, fmt):
-    """Against 64 bits: the tensor-core kernel rounds P to the type (half a unit each)."""
+def check_prefill(h, hkv, d, bs, spans, dtype, fmt, path, q=None, out=None, width=0, spread=1.0,
+                  dirty=False):
+    """Every row of a packed frame against 64 bits; `width`: extra table columns;
+    `dirty`: NaN in the workspace and in pool rows that no row attends."""
     rng = np.random.default_rng(h + d)
     f = wl.prefill_frame("t", 3, [s for s, _ in spans], [n for _, n in spans], h, hkv, d, bs)
-    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, fmt, spread)
     vc, vs = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
-    q = dev(rng.normal(size=(f.total_q, h, d))).to(dtype)
-    got = host(irb.paged_prefill_q8(q, codes_to(kc, fmt), codes_to(vc, fmt),
-                                    dev(ks.astype(np.float32)), dev(vs.astype(np.float32)),
-                                    dev(f.block_tables), dev(f.context_lens), dev(f.q_start),
-                                    f.scale, bs))
+    if q is None:
+        q = dev(rng.normal(size=(f.total_q, h, d))).to(dtype)
+    table = np.pad(f.block_tables, ((0, 0), (0, width)))
+    kd, vd, ksd, vsd = kc.copy(), vc.copy(), ks.copy(), vs.copy()
+    if dirty:
+        used = np.zeros(f.num_blocks * bs, bool)
+        for i, n in enumerate(f.context_lens):
+            p = np.arange(n)
+            used[f.block_tables[i, p // bs] * bs + p % bs] = True
+        kd[~used] = vd[~used] = np.nan if fmt == "e4m3" else 127
+    kp, vp = codes_to(kd, fmt), codes_to(vd, fmt)
+    bt, ctx, qs = dev(table), dev(f.context_lens), dev(f.q_start)
+    got_path, nbytes = ops.prefill_plan_q8(q, kp, bt, qs, bs)
+    assert got_path == path
+    ws = torch.full((max(nbytes, 256),), 0xff, dtype=torch.uint8, device=DEV) if dirty else None
+    got = host(irb.paged_prefill_q8(q, kp, vp, dev(ksd.astype(np.float32)),
+                                    dev(vsd.astype(np.float32)), bt, ctx, qs, f.scale, bs, out=out,
+                                    ws=ws))
     kv, vv = q8.values(kc, ks, bs), q8.values(vc, vs, bs)
-    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    low = path in (2, 3)
+    half = torch.finfo(dtype).eps / 2
     for i, (start, n) in enumerate(spans):
         for r in range(0, n, 1 if n < 50 else 13):
             t = start + r + 1
@@ -487,18 +497,132 @@ def test_prefill(h, hkv, d, bs, spans, dtype, fmt):
             want, weighted, size = q8.attend(host(q[row]),
                                              q8.history(kv, f.block_tables[i], t, bs),
                                              q8.history(vv, f.block_tables[i], t, bs), f.scale)
-            tol = attend_tolerance(want, weighted, size, t, d, dtype, False)
-            # weights rounded to the type; in fp16 a weight below 2^-14 (of a
-            # largest of 1) is rounded to a multiple of 2^-24, so it is off by
-            # up to 2^-25 whatever its size: t of them move sum p v / sum p,
-            # whose denominator is at least 1, by up to t 2^-25 max |v|. Rows of
-            # the expanded pool below fp16's normal range: 2^-25 each likewise
-            tol = tol + 2 * half * weighted
-            if dtype == torch.float16:
-                vmax = np.abs(q8.history(vv, f.block_tables[i], t, bs)).max()
-                tol = tol + t * 2.0 ** -25 * vmax + 2.0 ** -24
+            tol = attend_tolerance(want, weighted, size, t, d, dtype, path == 1 and dtype !=
+                                   torch.float32)
+            if low:
+                # weights rounded to the type; in fp16 a weight below 2^-14 (of a
+                # largest of 1) is rounded to a multiple of 2^-24, so it is off by
+                # up to 2^-25 whatever its size: t of them move sum p v / sum p,
+                # whose denominator is at least 1, by up to t 2^-25 max |v|. Rows of
+                # the expanded pool below fp16's normal range: 2^-25 each likewise
+                tol = tol + 2 * half * weighted
+                if dtype == torch.float16:
+                    vmax = np.abs(q8.history(vv, f.block_tables[i], t, bs)).max()
+                    tol = tol + t * 2.0 ** -25 * vmax + 2.0 ** -24
             err = np.abs(got[row] - want)
             assert (err <= tol).all(), (i, r, float((err - tol).max()))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("h,hkv,d,bs,spans", [
+    (28, 4, 128, 16, [(0, 130), (17, 1), (50, 40)]), (14, 2, 64, 16, [(3, 5), (0, 1), (0, 200)]),
+    (4, 4, 128, 12, [(20, 30), (0, 7)]), (16, 1, 64, 8, [(9, 33)]),
+    (40, 2, 64, 16, [(0, 9), (70, 20)]),   # a group of 20
+])
+def test_prefill(h, hkv, d, bs, spans, dtype, fmt):
+    path = 4 if dtype == torch.float32 else 2
+    check_prefill(h, hkv, d, bs, spans, dtype, fmt, path)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bs,width", [(16, 0), (16, 4000), (12, 0), (1, 7), (256, 0)])
+def test_prefill_layouts(bs, width, dtype):
+    """Dense and in-place expansion (a wide table), blocks of any size, and
+    nothing read that no row attends."""
+    check_prefill(8, 2, 64, bs, [(0, 70), (33, 2), (0, 1), (260, 140)], dtype, "e4m3",
+                  2 if dtype == torch.bfloat16 else 4, width=width, dirty=True)
+    check_prefill(8, 2, 64, bs, [(0, 70), (33, 20)], dtype, "int8",
+                  2 if dtype == torch.bfloat16 else 4, width=width)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prefill_few_rows_and_forced_paths(dtype):
+    spans = [(100, 1), (0, 1), (33, 4), (500, 2)]
+    check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 2 if dtype == torch.bfloat16 else 1)
+    ops.set_prefill_path(1)
+    try:
+        check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 1)
+        check_prefill(28, 4, 128, 16, [(3, 70), (10, 9)], dtype, "int8", 4, spread=4.0)
+    finally:
+        ops.set_prefill_path(0)
+
+
+def test_prefill_unaligned_rows():
+    rng = np.random.default_rng(4)
+    n, h, d = 29, 8, 64
+    for off, stride, path in ((1, h * d + 3, 4), (1, h * d + 8, 2), (0, h * d + 64, 2)):
+        flat = dev(rng.normal(size=n * (h * d + 64) + 16)).to(torch.bfloat16)
+        q = flat[off:].as_strided((n, h, d), (stride, d, 1), off)
+        check_prefill(h, 2, d, 16, [(20, 20), (0, 9)], torch.bfloat16, "e4m3", path, q=q)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prefill_nan_reaches_the_rows_that_attend_it(dtype, fmt):
+    """A NaN in K or V at one position: rows before it keep their values."""
+    rng = np.random.default_rng(2)
+    h, hkv, d, bs, n = 8, 2, 64, 16, 90
+    f = wl.prefill_frame("t", 3, [10, 0], [n, 30], h, hkv, d, bs)
+    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    vc, vs = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    q = dev(rng.normal(size=(f.total_q, h, d))).to(dtype)
+    bt, ctx, qs = dev(f.block_tables), dev(f.context_lens), dev(f.q_start)
+
+    def run(kc, ks, vc, vs):
+        return irb.paged_prefill_q8(q, codes_to(kc, fmt), codes_to(vc, fmt),
+                                    dev(ks.astype(np.float32)), dev(vs.astype(np.float32)), bt,
+                                    ctx, qs, f.scale, bs)
+
+    clean = run(kc, ks, vc, vs)
+    at = 64   # a block's first position, so that an int8 scale begins there
+    slot = f.block_tables[0, at // bs] * bs + at % bs
+    for side in "vk":
+        k2, v2, ks2, vs2 = kc.copy(), vc.copy(), ks.copy(), vs.copy()
+        if fmt == "e4m3":
+            (v2 if side == "v" else k2)[slot, 1, 5] = np.nan
+        else:
+            (vs2 if side == "v" else ks2)[slot // bs, 1] = np.nan
+        out = run(k2, ks2, v2, vs2)
+        bad = torch.isnan(out)
+        want = torch.zeros_like(bad)
+        rows = slice(at - 10, n)
+        if side == "v" and fmt == "e4m3":
+            want[rows, 4:, 5] = True
+        else:
+            want[rows, 4:] = True
+        assert torch.equal(bad, want)
+        err = (out.float() - clean.float()).abs()[~want]
+        # (the rows may come from the fp32 kernel now: both are off by the bound)
+        assert err.max().item() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prefill_bad_metadata_is_flagged(dtype):
+    rng = np.random.default_rng(2)
+    f = wl.prefill_frame("t", 3, [10, 0], [40, 30], 8, 2, 64, 16)
+    kc, ks = make_pool(rng, f.num_blocks, 16, 2, 64, "e4m3")
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    q = dev(rng.normal(size=(70, 8, 64))).to(dtype)
+    run = lambda bt, ctx: irb.paged_prefill_q8(q, pool, pool, sc, sc, dev(bt), dev(ctx),  # noqa: E731
+                                               dev(f.q_start), f.scale, 16)
+    good = run(f.block_tables, f.context_lens)
+    bt = f.block_tables.copy()
+    bt[0, 1] = f.num_blocks
+    out = run(bt, f.context_lens)
+    with pytest.raises(irb.DeviceError, match="BLOCK_ID"):
+        irb.check_device_errors()
+    assert torch.equal(out[40:], good[40:])
+    for c in (np.array([30, 30], np.int32), np.array([16 * 4 + 1, 30], np.int32)):
+        out = run(f.block_tables, c)
+        with pytest.raises(irb.DeviceError, match="CONTEXT_LEN"):
+            irb.check_device_errors()
+        assert torch.equal(out[40:], good[40:])
+    # rows behind the last sequence stay as they were
+    out = torch.full_like(q, 7.0)
+    irb.paged_prefill_q8(q, pool, pool, sc, sc, dev(f.block_tables[:1]), dev(f.context_lens[:1]),
+                         dev(f.q_start[:2]), f.scale, 16, out=out)
+    assert (out[40:] == 7.0).all() and torch.equal(out[:40], good[:40])
 
 
 def test_prefill_row_is_the_decode_row():

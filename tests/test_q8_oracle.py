@@ -112,8 +112,7 @@ def test_prefill_q8_and_norm_refusals():
         None)
     assert call(5) == _lib.IR_ERR_INVALID_ARG
     assert call(1) == _lib.IR_ERR_INVALID_ARG                     # null pointers
-    # both sides of the pool in 16 bits
-    assert lib.ir_paged_prefill_q8_workspace_size(ctypes.byref(s)) >= 2 * 64 * 2 * 64 * 2
+    assert lib.ir_paged_prefill_q8_plan(ctypes.byref(s), 7, None) == _lib.IR_ERR_INVALID_ARG
     s.num_slots = 70
     assert call(1) == _lib.IR_ERR_INVALID_ARG
 
