@@ -515,7 +515,8 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *     the workspace, which the tensor-core kernel attends over: a block's
  *     conversion is paid once, not once per 128 query rows and head. Exact in
  *     bf16 for power-of-two scales. The workspace holds the histories (or one
- *     layer's pool) in shape->dtype and can serve every layer;
+ *     layer's pool) in shape->dtype and can serve every layer. A NaN in V makes
+ *     its whole head NaN in the rows that attend it;
  *   4 everything else: fp32 tiles on the CUDA cores, codes read directly;
  *   1 as 4 for at most 4 query rows per sequence: every row decoded as its own
  *     sequence (ir_paged_decode_q8).

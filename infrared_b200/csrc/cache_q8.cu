@@ -582,22 +582,23 @@ __global__ void __launch_bounds__(256)
 
 // The blocks of the sequences' histories as rows of T: with `table` null, each
 // in its own place of a pool laid out as the codes are; else sequence by
-// sequence (cap rows each), with the block table of that order. CTA (s, y) takes
-// blocks y, y + gridDim.y, ... of sequence s and writes to flags[] whether it met
-// a V that is not finite.
+// sequence (cap rows each), with the block table of that order. The tensor
+// cores multiply the masked weights of a key tile too, and 0 * NaN is NaN: a V
+// that is not finite would reach rows that do not attend it. So it becomes 0,
+// and its head's K NaN instead: the score of a row that attends it is NaN, and
+// a masked score is never used.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)
     expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp, const float* ks,
                          const float* vs, const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
                          int max_blocks, int64_t num_blocks, int Hkv, int D, int bs,
-                         int32_t* table, int64_t cap, int table_block, int* flags, int32_t* err) {
+                         int32_t* table, int64_t cap, int table_block, int32_t* err) {
   wait_prior_grid();
   const int sq = blockIdx.x;
   const int64_t c0 = ctx[sq];
   const int pieces = Hkv * D / 8;
   const int tpr = pieces < 256 ? pieces : 256;
   const int side = blockDim.x / tpr;
-  bool nan = false;
   if (threadIdx.x == 0 && blockIdx.y == 0 && c0 > static_cast<int64_t>(max_blocks) * bs)
     set_err(err, IR_DEVERR_CONTEXT_LEN);
   for (int j = blockIdx.y; j < max_blocks && static_cast<int64_t>(j) * bs < c0; j += gridDim.y) {
@@ -618,20 +619,20 @@ __global__ void __launch_bounds__(256)
         uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
         uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
         if (!ok) kc = vc = make_uint2(0u, 0u);
-        if (std::is_same<C, e4m3_t>::value && (has_nan(vc.x) || has_nan(vc.y)) &&
-            static_cast<int64_t>(j) * bs + r < c0)
-          nan = true;
-        store8<T, C>(kout + dst * 8, kc, k);
-        store8<T, C>(vout + dst * 8, vc, v);
+        float kr = k, vr = v;
+        if (!finite(v) || (std::is_same<C, e4m3_t>::value && (has_nan(vc.x) || has_nan(vc.y)))) {
+          kr = __uint_as_float(0x7fc00000u);
+          vr = 0.f;
+          vc = make_uint2(0u, 0u);
+        }
+        store8<T, C>(kout + dst * 8, kc, kr);
+        store8<T, C>(vout + dst * 8, vc, vr);
       }
-      nan = nan || !finite(v);
     }
   }
   if (table != nullptr && blockIdx.y == 0)
     for (int i = threadIdx.x; i < cap / table_block; i += blockDim.x)
       table[sq * (cap / table_block) + i] = static_cast<int32_t>(sq * (cap / table_block) + i);
-  nan = __syncthreads_or(nan);
-  if (threadIdx.x == 0) flags[static_cast<int64_t>(sq) * gridDim.y + blockIdx.y] = nan ? 1 : 0;
 }
 
 template <typename F>
@@ -751,20 +752,15 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
   });
 }
 
-int expand_flags(int S, int max_blocks, int sms) {
-  // CTAs of a sequence: eight per SM in all
-  const int y = S > 0 ? 8 * sms / S : 1;
-  return S * (y < 1 ? 1 : (y > max_blocks ? max_blocks : y));
-}
-
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
                          int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
                          int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
-                         int32_t* table, int64_t cap, int table_block, int* flags, int sms,
-                         int32_t* err, cudaStream_t stream) {
+                         int32_t* table, int64_t cap, int table_block, int32_t* err,
+                         cudaStream_t stream) {
+  if (S == 0 || max_blocks == 0) return 0;
   const dim3 grid(static_cast<unsigned>(S),
-                  static_cast<unsigned>(expand_flags(S, max_blocks, sms) / S));
+                  static_cast<unsigned>(max_blocks < 4096 ? max_blocks : 4096));
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
       using T = decltype(t);
@@ -772,8 +768,7 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
                            piece_threads(Hkv * D / 8), 0, stream, static_cast<T*>(k_out),
                            static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
                            static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride,
-                           ctx, max_blocks, num_blocks, Hkv, D, bs, table, cap, table_block, flags,
-                           err);
+                           ctx, max_blocks, num_blocks, Hkv, D, bs, table, cap, table_block, err);
     });
   });
 }

@@ -642,9 +642,8 @@ struct PrefillQ8Plan {
   int path;        // 1 rows as decode rows, 2 / 3 expansion + tensor cores, 4 fp32 tiles
   bool dense;      // the expansion lays the histories out sequence by sequence
   int64_t cap;     // rows of a sequence there
-  int sms, flags;
-  // workspace: K, V, table, flags, or the rows path's tables and contexts
-  size_t pool, table_off, flags_off, rows_table, rows_ctx, bytes;
+  // workspace: K, V, table, or the rows path's tables and contexts
+  size_t pool, table_off, rows_table, rows_ctx, bytes;
 };
 
 constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy per key tile
@@ -662,8 +661,6 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   if (s->num_slots < s->block_size || s->num_slots % s->block_size != 0)
     return fail(IR_ERR_INVALID_ARG, "num_slots must be a positive multiple of block_size");
   *p = PrefillQ8Plan{};
-  const int e = cached(-1, sm_count_now, 0, &p->sms);
-  if (e) return cuda_status(e, "device query");
   const int bs = s->block_size;
   const bool half = s->dtype != IR_DTYPE_F32;
   const bool rows_ok = half && (s->q_stride * 2) % 16 == 0 && (s->out_stride * 2) % 16 == 0;
@@ -684,10 +681,8 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
     const int64_t rows = p->dense ? dense_rows : s->num_slots;
     p->pool = align256(static_cast<size_t>(rows) * row_bytes);
     p->table_off = 2 * p->pool;
-    p->flags_off = p->table_off +
-                   (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
-    p->flags = s->num_seqs > 0 ? irb::expand_flags(s->num_seqs, s->max_blocks, p->sms) : 0;
-    p->bytes = p->flags_off + align256(static_cast<size_t>(p->flags) * 4);
+    p->bytes = p->table_off +
+               (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
   } else if (p->path == 1) {
     ir_decode_shape d = rows_shape(s);
     Plan plan;
@@ -1331,17 +1326,14 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
   a.scale_log2 = s->scale * irb::kLog2e;
   a.err = err_flag;
   if (p.path == 4) {
-    e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, nullptr,
-                               0, p.sms, st);
+    e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, st);
     return cuda_status(e, "8-bit prefill launch");
   }
   int32_t* table = p.dense ? reinterpret_cast<int32_t*>(ws + p.table_off) : nullptr;
-  int* flags = reinterpret_cast<int*>(ws + p.flags_off);
   e = irb::launch_expand_blocks(ws, ws + p.pool, k_pool, v_pool, k_scale, v_scale, block_tables,
                                 s->bt_stride, context_lens, s->num_seqs, s->max_blocks,
                                 a.num_blocks, s->num_kv_heads, s->head_dim, s->block_size,
-                                s->dtype, kv_format, table, p.cap, kDenseBlock, flags, p.sms,
-                                err_flag, st);
+                                s->dtype, kv_format, table, p.cap, kDenseBlock, err_flag, st);
   if (e) return cuda_status(e, "8-bit block expansion launch");
   ir_prefill_shape x = *s;
   if (p.dense) {
@@ -1350,13 +1342,8 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     x.bt_stride = x.max_blocks;
     x.num_slots = p.cap * s->num_seqs;
   }
-  rc = ir_paged_prefill(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
-                        q_start, &x, nullptr, 0, err_flag, stream);
-  if (rc) return rc;
-  // (does nothing unless the expansion flagged a V that is not finite)
-  e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, flags,
-                             p.flags, p.sms, st);
-  return cuda_status(e, "8-bit prefill launch");
+  return ir_paged_prefill(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
+                          q_start, &x, nullptr, 0, err_flag, stream);
 }
 
 // ---------------------------------------------------------------- q/k norm + rotation

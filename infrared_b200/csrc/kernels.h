@@ -108,21 +108,20 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
                            int fmt, int32_t* err, cudaStream_t stream);
 // Every block that a sequence's history covers, as rows of dtype: at the same
 // place of the output pools (table null), or sequence by sequence, cap rows
-// each, with the block table [S, cap / table_block] of that order. flags
-// [expand_flags()] tell where V is not finite. max_blocks > 0.
-int expand_flags(int S, int max_blocks, int sms);
+// each, with the block table [S, cap / table_block] of that order. Where a V is
+// not finite it becomes 0 and its K NaN.
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
                          int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
                          int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
-                         int32_t* table, int64_t cap, int table_block, int* flags, int sms,
-                         int32_t* err, cudaStream_t stream);
+                         int32_t* table, int64_t cap, int table_block, int32_t* err,
+                         cudaStream_t stream);
 
 // prefill_q8.cu: packed rows over an 8-bit pool in fp32 on the CUDA cores
-// (args as in PrefillArgs); with flags, only where one of them is set.
+// (args as in PrefillArgs)
 int launch_prefill_q8(const PrefillArgs& a, const void* k_pool, const void* v_pool,
                       const float* k_scale, const float* v_scale, int dtype, int fmt,
-                      const int* flags, int num_flags, int sms, cudaStream_t s);
+                      cudaStream_t s);
 
 // qk_norm_rope.cu
 struct NormRopeArgs {

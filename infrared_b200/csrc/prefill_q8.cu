@@ -1,9 +1,6 @@
 // Causal attention of packed query rows over an 8-bit pool in fp32 on the CUDA
 // cores: for q of 32 bits, and for 16-bit calls that the tensor-core path
-// cannot take (rows that are not 16-byte aligned, or asked for). It also
-// follows every tensor-core call, to do nothing unless the expansion met a V
-// that is not finite: there the masked weights of a tile multiply such a V as
-// 0 * NaN, and rows before it would read NaN; here they are left out.
+// cannot take (rows that are not 16-byte aligned, or asked for).
 //
 // A CTA takes 64 rows of one kv head, a row being a (query token, head of the
 // group) pair, and walks the sequence's keys 64 at a time: the codes of a tile
@@ -12,7 +9,8 @@
 // block's scale, and each of 256 threads computes 4 x 4 scores and 4 x D / 16
 // outputs from registers, with an online softmax whose statistics live in the
 // 16 lanes that share a row. Bound by FMA issue: 8 FMAs per 16-byte
-// shared-memory read.
+// shared-memory read. 6 sequences of up to 300 rows over 700 more keys, 12 heads
+// of 128, fp32: 283 us a call (5.8 GFLOP), where decoding every row takes 1500.
 #include "kernels.h"
 #include "quant.cuh"
 
@@ -73,22 +71,15 @@ __device__ __forceinline__ bool find_tile(const int32_t* q_start, int S, int tot
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(kT, 2)
     prefill_q8_kernel(const PrefillArgs a, const uint8_t* kp, const uint8_t* vp, const float* ks,
-                      const float* vs, const int* flags, int num_flags) {
+                      const float* vs) {
   extern __shared__ __align__(16) uint8_t raw[];
   SmemQ8P<D>& sm = *reinterpret_cast<SmemQ8P<D>*>(raw);
   __shared__ int s_seq, s_tile, s_tiles, s_nan;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int kvh = blockIdx.y;
-  if (flags != nullptr) {
-    int any = 0;
-    for (int i = tid; i < num_flags; i += kT) any |= flags[i];
-    if (!__syncthreads_or(any)) return;
-  }
-  for (int index = blockIdx.x;; index += gridDim.x) {
-  __syncthreads();  // the tile before is done
   if (tid < 32) {
     int seq = -1, tile = 0, tiles = 0;
-    if (!find_tile(a.q_start, a.S, a.total_q, a.n_rep, index, &seq, &tile, &tiles)) seq = -1;
+    if (!find_tile(a.q_start, a.S, a.total_q, a.n_rep, blockIdx.x, &seq, &tile, &tiles)) seq = -1;
     if (tid == 0) s_seq = seq, s_tile = tile, s_tiles = tiles;
   }
   __syncthreads();
@@ -101,7 +92,7 @@ __global__ void __launch_bounds__(kT, 2)
   if (ctx < q_len || ctx > static_cast<int64_t>(a.max_blocks) * a.bs ||
       q0 + static_cast<int64_t>(q_len) > a.total_q) {
     if (tid == 0) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
-    continue;
+    return;
   }
   const int64_t m0 = static_cast<int64_t>(tile) * kM;
   const int64_t rows = static_cast<int64_t>(q_len) * a.n_rep;
@@ -289,48 +280,44 @@ __global__ void __launch_bounds__(kT, 2)
 #pragma unroll
     for (int c = 0; c < CO; ++c) dst[64 * (c / 4) + tx * 4 + c % 4] = DT<T>::from_f(o[i][c] * f);
   }
-  }  // tiles
 }
 
 template <typename T, typename C, int D>
 int launch_p(const PrefillArgs& a, const void* kp, const void* vp, const float* ks,
-             const float* vs, const int* flags, int num_flags, int sms, cudaStream_t s) {
+             const float* vs, cudaStream_t s) {
   auto kern = prefill_q8_kernel<T, C, D>;
   constexpr int bytes = static_cast<int>(sizeof(SmemQ8P<D>));
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return static_cast<int>(e);
   // at most this many tiles: every sequence's last one may be short
-  int64_t tiles = (static_cast<int64_t>(a.total_q) * a.n_rep + kM - 1) / kM + a.S;
-  // (a call that mostly has nothing to do: as few CTAs as fill the GPU)
-  const int64_t most = flags ? (2 * sms + a.Hkv - 1) / a.Hkv : INT32_MAX / 2;
-  if (tiles > most) tiles = most;
+  const int64_t tiles = (static_cast<int64_t>(a.total_q) * a.n_rep + kM - 1) / kM + a.S;
+  if (tiles > INT32_MAX) return static_cast<int>(cudaErrorInvalidConfiguration);
   kern<<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.Hkv)), kT, bytes, s>>>(
-      a, static_cast<const uint8_t*>(kp), static_cast<const uint8_t*>(vp), ks, vs, flags,
-      num_flags);
+      a, static_cast<const uint8_t*>(kp), static_cast<const uint8_t*>(vp), ks, vs);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, typename C>
 int by_d(const PrefillArgs& a, const void* kp, const void* vp, const float* ks, const float* vs,
-         const int* flags, int num_flags, int sms, cudaStream_t s) {
-  return a.D == 128 ? launch_p<T, C, 128>(a, kp, vp, ks, vs, flags, num_flags, sms, s)
-                    : launch_p<T, C, 64>(a, kp, vp, ks, vs, flags, num_flags, sms, s);
+         cudaStream_t s) {
+  return a.D == 128 ? launch_p<T, C, 128>(a, kp, vp, ks, vs, s)
+                    : launch_p<T, C, 64>(a, kp, vp, ks, vs, s);
 }
 
 template <typename T>
 int by_c(int fmt, const PrefillArgs& a, const void* kp, const void* vp, const float* ks,
-         const float* vs, const int* flags, int num_flags, int sms, cudaStream_t s) {
-  return fmt == IR_KV_INT8 ? by_d<T, int8_t>(a, kp, vp, ks, vs, flags, num_flags, sms, s)
-                           : by_d<T, e4m3_t>(a, kp, vp, ks, vs, flags, num_flags, sms, s);
+         const float* vs, cudaStream_t s) {
+  return fmt == IR_KV_INT8 ? by_d<T, int8_t>(a, kp, vp, ks, vs, s)
+                           : by_d<T, e4m3_t>(a, kp, vp, ks, vs, s);
 }
 
 }  // namespace
 
 int launch_prefill_q8(const PrefillArgs& a, const void* k_pool, const void* v_pool,
                       const float* k_scale, const float* v_scale, int dtype, int fmt,
-                      const int* flags, int num_flags, int sms, cudaStream_t s) {
+                      cudaStream_t s) {
   auto run = [&](auto by) {
-    return by(fmt, a, k_pool, v_pool, k_scale, v_scale, flags, num_flags, sms, s);
+    return by(fmt, a, k_pool, v_pool, k_scale, v_scale, s);
   };
   switch (dtype) {
     case IR_DTYPE_F32: return run(by_c<float>);
