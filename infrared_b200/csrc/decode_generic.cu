@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(kGenThreads)
   // banks
   __shared__ __align__(16) float q_s[kMaxGroup][D];
   __shared__ __align__(16) float k_s[kTile][D + 4];
-  __shared__ float v_s[kTile][D];
-  __shared__ float p_s[kMaxGroup][kTile];
+  __shared__ __align__(16) float v_s[kTile][D];
+  __shared__ __align__(16) float p_s[kMaxGroup][kTile];
   __shared__ float m_s[kMaxGroup], l_s[kMaxGroup], alpha_s[kMaxGroup];
   __shared__ RangeInfo ri;
   __shared__ int64_t sm_scan[kGenThreads / 32];
@@ -132,12 +132,20 @@ __global__ void __launch_bounds__(kGenThreads)
       if (i >= NCH) continue;
       const int r = i / CPR, cc = i % CPR;
       if constexpr (kQ8) {
-        const C* kc = reinterpret_cast<const C*>(&kr[k]);
-        const C* vc = reinterpret_cast<const C*>(&vr[k]);
+        // four values at a time, each lane starting at another of the chunk's
+        // quarters: neighbouring lanes' chunks are 64 bytes apart
+        const uint32_t* kw = reinterpret_cast<const uint32_t*>(&kr[k]);
+        const uint32_t* vw = reinterpret_cast<const uint32_t*>(&vr[k]);
 #pragma unroll
-        for (int e = 0; e < EPC; ++e) {
-          k_s[r][cc * EPC + e] = DT<C>::to_f(kc[e]) * ksc[k];
-          v_s[r][cc * EPC + e] = DT<C>::to_f(vc[e]) * vsc[k];
+        for (int e = 0; e < 4; ++e) {
+          const int p = (e + lane) & 3;
+          const uint32_t a4 = p == 0 ? kw[0] : p == 1 ? kw[1] : p == 2 ? kw[2] : kw[3];
+          const uint32_t b4 = p == 0 ? vw[0] : p == 1 ? vw[1] : p == 2 ? vw[2] : vw[3];
+          const float4 x = decode4<C>(a4), y = decode4<C>(b4);
+          *reinterpret_cast<float4*>(&k_s[r][cc * EPC + 4 * p]) =
+              make_float4(x.x * ksc[k], x.y * ksc[k], x.z * ksc[k], x.w * ksc[k]);
+          *reinterpret_cast<float4*>(&v_s[r][cc * EPC + 4 * p]) =
+              make_float4(y.x * vsc[k], y.y * vsc[k], y.z * vsc[k], y.w * vsc[k]);
         }
         continue;
       }
@@ -264,13 +272,31 @@ __global__ void __launch_bounds__(kGenThreads)
       }
     }
     __syncthreads();
+    float vcol[kQ8 ? kTile : 1];
+    if constexpr (kQ8) {
+#pragma unroll
+      for (int r = 0; r < kTile; ++r) vcol[r] = v_s[r][d];
+    }
 #pragma unroll
     for (int k = 0; k < NH; ++k) {
       const int n = hg + k * HPT;
       if (n < a.n_rep) {
         float x = acc[k] * alpha_s[n];
+        if constexpr (kQ8) {
+          // (the same products in the same order, the weights read four at a time
+          // and the column once for all heads)
 #pragma unroll
-        for (int r = 0; r < kTile; ++r) x = fmaf(p_s[n][r], v_s[r][d], x);
+          for (int r = 0; r < kTile; r += 4) {
+            const float4 p = *reinterpret_cast<const float4*>(&p_s[n][r]);
+            x = fmaf(p.x, vcol[r], x);
+            x = fmaf(p.y, vcol[r + 1], x);
+            x = fmaf(p.z, vcol[r + 2], x);
+            x = fmaf(p.w, vcol[r + 3], x);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < kTile; ++r) x = fmaf(p_s[n][r], v_s[r][d], x);
+        }
         acc[k] = x;
       }
     }
