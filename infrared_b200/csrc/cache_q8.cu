@@ -143,14 +143,66 @@ __device__ __forceinline__ uint2 encode8(const float (&v)[8]) {
                     encode4<C>(make_float4(v[4], v[5], v[6], v[7])));
 }
 
+// The scale of a (block, side, head) after the new rows (largest finite
+// magnitude amax; `bad`: one was not finite), written by lane 0.
+template <typename C>
+__device__ __forceinline__ float settle_scale(float amax, bool bad, bool begun, float before,
+                                              float* sp) {
+  constexpr bool kInt = std::is_same<C, int8_t>::value;
+  const float old = begun ? 0.f : before;
+  const float need = scale_for<C>(amax);
+  float now = old > need ? old : need;
+  // int8 has no code for a value that is not finite: its block reads as NaN
+  // until it is begun again
+  if (kInt && (bad || old != old)) now = __uint_as_float(0x7fc00000u);
+  if ((threadIdx.x & 31) == 0) *sp = now;
+  return now;
+}
+
+// The codes that stay, moved from scale `old` to `now`.
+template <typename C, typename Src>
+__device__ __forceinline__ void rescale_rest(const Q8WriteArgs& a, Src src, uint8_t* dst,
+                                             int row_bytes, int rp, int sub, float old,
+                                             float now) {
+  const float inv = pow2_reciprocal(now);
+  const float ratio = inv != 0.f ? old * inv : old / now;
+  for (int base = 0; base < a.bs; base += rp) {
+    const int r = base + sub;
+    const int t = src(r < a.bs ? r : 0);
+    if (r >= a.bs || t >= 0) continue;
+    uint2* p = reinterpret_cast<uint2*>(dst + r * row_bytes);
+    const uint2 c = *p;
+    const float4 f = decode4<C>(c.x), g = decode4<C>(c.y);
+    const float v[8] = {f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio,
+                        g.x * ratio, g.y * ratio, g.z * ratio, g.w * ratio};
+    *p = encode8<C>(v);
+  }
+}
+
+constexpr int kPass = 8;  // passes of rows that a warp holds at once
+
+// Codes of the new rows held in x (bit u of have: pass u is one), all finite;
+// `row` is this lane's place in pass 0, `apart` the bytes between passes.
+template <typename T, typename C>
+__device__ __forceinline__ void encode_rows(const Eight<T> (&x)[kPass], uint32_t have, float inv,
+                                            uint8_t* row, int apart) {
+#pragma unroll
+  for (int u = 0; u < kPass; ++u) {
+    float v[8];
+    x[u].values(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    const uint2 c = encode8<C>(v);
+    if ((have >> u) & 1u) *reinterpret_cast<uint2*>(row + u * apart) = c;
+  }
+}
+
 // One (side, kv head) of block `blk`, by one warp. Lanes cover D in groups of
 // 8 elements, 256 / D rows at a time, kPass such passes at once. src(r) is
 // called by all lanes of the warp together.
 template <typename T, typename C, bool VEC, typename Src>
 __device__ __forceinline__ void quantise_task(const Q8WriteArgs& a, int64_t blk, Src src, int side,
                                               int h) {
-  constexpr bool kInt = std::is_same<C, int8_t>::value;
-  constexpr int kPass = 8;
   const int lane = threadIdx.x & 31;
   const int sh = a.D == 128 ? 4 : 3;  // log2 of the lanes per row
   const int rp = 32 >> sh;            // rows per pass
@@ -210,44 +262,15 @@ __device__ __forceinline__ void quantise_task(const Q8WriteArgs& a, int64_t blk,
   // (bits of magnitudes are in their order)
   amax = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(amax)));
 
-  const float old = begun ? 0.f : before;
-  const float need = scale_for<C>(amax);
-  float now = old > need ? old : need;
-  // int8 has no code for a value that is not finite: its block reads as NaN
-  // until it is begun again
-  if (kInt && (bad || old != old)) now = __uint_as_float(0x7fc00000u);
+  const float now = settle_scale<C>(amax, bad, begun, before, sp);
   const float inv = pow2_reciprocal(now);
-  if (lane == 0) *sp = now;
-
-  if (!begun && now != old && now == now) {
-    // rescale the codes that stay
-    const float ratio = inv != 0.f ? old * inv : old / now;
-    for (int base = 0; base < a.bs; base += rp) {
-      const int r = base + sub;
-      const int t = src(r < a.bs ? r : 0);
-      if (r >= a.bs || t >= 0) continue;
-      uint2* p = reinterpret_cast<uint2*>(dst + r * row_bytes);
-      const uint2 c = *p;
-      const float4 f = decode4<C>(c.x), g = decode4<C>(c.y);
-      const float v[8] = {f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio,
-                          g.x * ratio, g.y * ratio, g.z * ratio, g.w * ratio};
-      *p = encode8<C>(v);
-    }
-  }
+  if (!begun && now != before && now == now)
+    rescale_rest<C>(a, src, dst, row_bytes, rp, sub, before, now);
   if (!bad && inv != 0.f) {
     // every value finite and the scale a power of two: no case to tell apart
     for (int base = 0; base < a.bs; base += chunk) {
       if (chunk < a.bs) load(base);
-      uint8_t* row = dst + (base + sub) * row_bytes;
-#pragma unroll
-      for (int u = 0; u < kPass; ++u) {
-        float v[8];
-        x[u].values(v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inv;
-        const uint2 c = encode8<C>(v);
-        if ((have >> u) & 1u) *reinterpret_cast<uint2*>(row + u * rp * row_bytes) = c;
-      }
+      encode_rows<T, C>(x, have, inv, dst + (base + sub) * row_bytes, rp * row_bytes);
     }
     return;
   }
@@ -439,6 +462,143 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 3 : 2) write_runs_
     first = next;
     next = after;
     mine = coming;
+  }
+}
+
+// A task with a value that is not finite, kept out of the common path's
+// registers (row: token of block row `lane`).
+template <typename T, typename C>
+__device__ __noinline__ void quantise_apart(const Q8WriteArgs& a, int64_t blk, int row, int side,
+                                            int h) {
+  quantise_task<T, C, true>(a, blk, [&](int r) { return __shfl_sync(kAll, row, r & 31); }, side,
+                            h);
+}
+
+// The same for 16-bit rows where a task's rows are at most one load of the
+// warp (bs * D <= 2048): the rows of the next task are copied to shared memory
+// while the current one is computed, so that a warp's reads never pause; every
+// lane copies and reads its own pieces. Two CTAs fill an SM's registers (32768
+// rows of 4 heads of 128, bf16, the three grids together: 24.4 us = 4.1 TB/s, against 29.2
+// with the rows in registers; a device copy of as many bytes takes 35).
+template <typename T, typename C>
+__global__ void __launch_bounds__(kQThreads, 2) write_stream_kernel(const Q8WriteArgs a,
+                                                                    const Q8Links l) {
+  __shared__ int rows[kQWarps][32];
+  extern __shared__ __align__(16) uint4 stage[];  // [warp][2][kPass][32]
+  wait_prior_grid();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tasks = 2 * a.Hkv, warps = gridDim.x * kQWarps;
+  const int w = blockIdx.x * kQWarps + warp;
+  const int step = warps / tasks, task = w % tasks;
+  const int side = task / a.Hkv, h = task - side * a.Hkv;
+  int o = w / tasks;
+  const int count = o < step ? l.count[0] : 0;
+  const bool others = l.count[1] != 0;
+  if (o >= count) return;
+  const int sh = a.D == 128 ? 4 : 3;  // log2 of the lanes per row
+  const int rp = 32 >> sh;
+  const int sub = lane >> sh, col = (lane & ((1 << sh) - 1)) * 8;
+  const T* in = reinterpret_cast<const T*>(a.src[side]) + h * a.D + col;
+  const int row_bytes = a.Hkv * a.D;
+  uint4* mine = stage + warp * (2 * kPass * 32) + lane;
+
+  struct Task {
+    int64_t blk;
+    int row;        // token of row `lane`, or -1
+    float before;   // the scale
+    uint32_t have;
+  };
+  auto slots_from = [&](int f) { return f + lane < a.n ? a.slots[f + lane] : -1; };
+  // resolves a task and starts its copies into buffer `buf`
+  auto start = [&](int first, int64_t slot, int buf) {
+    Task t;
+    t.blk = static_cast<uint32_t>(__shfl_sync(kAll, slot, 0)) / a.bs;
+    t.before = a.scale[side][t.blk * a.Hkv + h];
+    const int64_t off = slot - t.blk * a.bs;
+    const unsigned inside = __ballot_sync(kAll, off >= 0 && off < a.bs);
+    const int len = inside == kAll ? 32 : __ffs(~inside) - 1;
+    const int off0 = __shfl_sync(kAll, static_cast<int>(off), 0);
+    if (!others && len < 32 && __all_sync(kAll, lane >= len || off == off0 + lane)) {
+      t.row = lane >= off0 && lane < off0 + len ? first + lane - off0 : -1;  // rows in order
+    } else {
+      rows[warp][lane] = -1;
+      __syncwarp();
+      walk_runs(a, l, t.blk, others, first, [&](bool hit, int r, int j) {
+        if (hit) atomicMax(&rows[warp][r], j);
+      });
+      __syncwarp();
+      t.row = rows[warp][lane];
+      __syncwarp();
+    }
+    const int some = __reduce_max_sync(kAll, t.row);
+    t.have = 0;
+#pragma unroll
+    for (int u = 0; u < kPass; ++u) {
+      const int r = u * rp + sub;
+      int tok = __shfl_sync(kAll, t.row, r & 31);
+      if (r < a.bs && tok >= 0)
+        t.have |= 1u << u;
+      else
+        tok = some;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       smem_u32(mine + (buf * kPass + u) * 32)),
+                   "l"(in + static_cast<int64_t>(tok) * a.stride[side])
+                   : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return t;
+  };
+
+  int first = l.owners[o];
+  int next = step < count - o ? l.owners[o + step] : 0;
+  Task cur = start(first, slots_from(first), 0);
+  int64_t slot = slots_from(next);
+  for (int buf = 0;; buf ^= 1) {
+    const bool more = step < count - o;
+    Task coming;
+    if (more) {
+      coming = start(next, slot, buf ^ 1);
+      next = 2 * step < count - o ? l.owners[o + 2 * step] : 0;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    // (read twice, for the maximum and for the codes, not held in between)
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < kPass; ++u) m = Eight<T>{mine[(buf * kPass + u) * 32]}.top(m);
+    if (more) slot = slots_from(next);
+    auto src = [&](int r) { return __shfl_sync(kAll, cur.row, r & 31); };
+    const float amax = Eight<T>::magnitude(m);
+    if (__any_sync(kAll, !finite(amax))) {
+      quantise_apart<T, C>(a, cur.blk, cur.row, side, h);
+    } else {
+      const float top = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(amax)));
+      const bool begun = src(0) >= 0;
+      const float now = settle_scale<C>(top, false, begun, cur.before,
+                                        a.scale[side] + cur.blk * a.Hkv + h);
+      uint8_t* dst = a.pool[side] + cur.blk * a.bs * row_bytes + (h * a.D + col);
+      const float inv = pow2_reciprocal(now);
+      if (!begun && now != cur.before && now == now)
+        rescale_rest<C>(a, src, dst, row_bytes, rp, sub, cur.before, now);
+      uint8_t* to = dst + sub * row_bytes;
+#pragma unroll 4
+      for (int u = 0; u < kPass; ++u) {
+        float v[8];
+        Eight<T>{mine[(buf * kPass + u) * 32]}.values(v);
+        if (inv != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= inv;
+        } else {  // a scale that is no power of two
+          for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], now);
+        }
+        const uint2 c = encode8<C>(v);
+        if ((cur.have >> u) & 1u) *reinterpret_cast<uint2*>(to + u * rp * row_bytes) = c;
+      }
+    }
+    if (!more) return;
+    cur = coming;
+    o += step;
   }
 }
 
@@ -716,13 +876,25 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   const int64_t least = (2 * Hkv + kQWarps - 1) / kQWarps;
   int64_t grid = small ? (blocks * 2 * Hkv + kQWarps - 1) / kQWarps : blocks;
   // (as many CTAs as fit at once)
-  const int64_t most = static_cast<int64_t>(sms) * (dtype == IR_DTYPE_F32 ? 2 : 3);
+  const bool stream16 = dtype != IR_DTYPE_F32 && vec && small && bs * D <= 2048;
+  const int64_t most = static_cast<int64_t>(sms) * (dtype == IR_DTYPE_F32 || stream16 ? 2 : 3);
   if (grid > most) grid = most;
   if (small && grid < least) grid = least;
   return by_type(dtype, [&](auto t) {
     return by_format(fmt, [&](auto c) {
       using T = decltype(t);
       using C = decltype(c);
+      if constexpr (sizeof(T) == 2) {
+        if (stream16) {
+          auto stream_kern = write_stream_kernel<T, C>;
+          constexpr int kStage = kQWarps * 2 * kPass * 32 * 16;  // 64 KB
+          cudaError_t e = cudaFuncSetAttribute(
+              stream_kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+          if (e != cudaSuccess) return static_cast<int>(e);
+          return launch_behind(stream_kern, dim3(static_cast<unsigned>(grid)), kQThreads, kStage,
+                               stream, a, l);
+        }
+      }
       auto kern = small ? (vec ? write_runs_kernel<T, C, true> : write_runs_kernel<T, C, false>)
                         : (vec ? write_blocks_kernel<T, C, true> : write_blocks_kernel<T, C, false>);
       return launch_behind(kern, dim3(static_cast<unsigned>(grid)), kQThreads, small ? 0 : smem,
