@@ -518,8 +518,9 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *     layer's pool) in shape->dtype and can serve every layer. A NaN in V makes
  *     its whole head NaN in the rows that attend it;
  *   4 everything else: fp32 tiles on the CUDA cores, codes read directly;
- *   1 as 4 for at most 4 query rows per sequence: every row decoded as its own
- *     sequence (ir_paged_decode_q8).
+ *   1 as 4 for at most 2 query rows per sequence (4, up to 64 rows): every row
+ *     decoded as its own sequence (ir_paged_decode_q8).
+ * Rows of q that belong to no sequence leave theirs of out as they are.
  * Values of K or V at positions that a row does not attend change nothing in it,
  * NaN included. ir_set_prefill_path(2 or 3) asks for the tensor cores, 1 for
  * the others. */

@@ -9,9 +9,12 @@
 // rows,
 //   s' = max(s, scale_for(amax))          (s counts as 0 when row 0 is new),
 // rescales the codes that stay if s' > s, and writes the new codes. Nothing
-// is summed, so the result does not depend on the order of the tokens. The
-// warp loads up to 16 rows at once and keeps them in registers between the
-// two steps, so that rows are read once.
+// is summed, so the result does not depend on the order of the tokens. Rows are
+// read from memory once: up to 16 a warp wait in registers, or in shared memory
+// where the next task's are copied meanwhile, between the maximum and the codes.
+//
+// Bound by HBM where calls are large: 32768 rows of 4 heads of 128, bf16, move
+// 101 MB in 24.4 us. Small calls are one launch (64 rows 3.3 us, 777 int8 5.6).
 #include "kernels.h"
 #include "quant.cuh"
 
@@ -21,7 +24,10 @@ namespace {
 
 constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
-// Calls of up to this many tokens find each block's rows by reading all slots.
+// Calls of up to this many tokens find each block's rows by reading all slots:
+// one launch instead of three. 1024 rows of one prompt take 6.9 us so, 6.1 with
+// linked runs, but each launch costs the host 2-3 us more; 1024 rows appended to
+// as many blocks take 11.1 (the scan is quadratic, so not for much longer calls).
 constexpr int64_t kScanTokens = 1024;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -415,8 +421,8 @@ __device__ __forceinline__ void walk_runs(const Q8WriteArgs& a, const Q8Links& l
 // Blocks of up to 32 rows: every warp takes a task of its own, lane r holding
 // the token of row r.
 template <typename T, typename C, bool VEC>
-__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 3 : 2) write_runs_kernel(const Q8WriteArgs a,
-                                                               const Q8Links l) {
+__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 3 : 2)
+    write_runs_kernel(const Q8WriteArgs a, const Q8Links l) {
   __shared__ int rows[kQWarps][32];
   wait_prior_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -628,15 +634,15 @@ __global__ void __launch_bounds__(kQThreads) write_blocks_kernel(const Q8WriteAr
   }
 }
 
-// Finite values beyond T's range saturate.
+// code * s beyond T's range saturates; a NaN code and a scale that is not finite
+// keep their value.
 template <typename T>
-__device__ __forceinline__ float saturate(float x) {
-  // (a code times a scale is finite or NaN unless the scale is not; min and
-  // max would turn NaN into a number, the comparison keeps it)
-  constexpr bool kHalf = std::is_same<T, __half>::value;
-  const float top = kHalf ? 65504.f : __uint_as_float(0x7f7f0000u);
-  if constexpr (sizeof(T) == 2) return fabsf(x) > top && finite(x) ? copysignf(top, x) : x;
-  return x;
+__device__ __forceinline__ float saturate(float x, float s) {
+  constexpr float kTop = std::is_same<T, __half>::value ? 65504.f
+                         : sizeof(T) == 2               ? 0x1.fep127f
+                                                        : 0x1.fffffep127f;
+  // (min and max would turn NaN into a number, the comparison keeps it)
+  return fabsf(x) > kTop && finite(s) ? copysignf(kTop, x) : x;
 }
 
 // Whether any of four e4m3 codes is NaN (0x7f or 0xff).
@@ -649,9 +655,10 @@ __device__ __forceinline__ bool has_nan(uint32_t w) {
 template <typename T, typename C>
 __device__ __forceinline__ void store8(T* out, uint2 codes, float s) {
   const float4 f = decode4<C>(codes.x), g = decode4<C>(codes.y);
-  const float v[8] = {saturate<T>(f.x * s), saturate<T>(f.y * s), saturate<T>(f.z * s),
-                      saturate<T>(f.w * s), saturate<T>(g.x * s), saturate<T>(g.y * s),
-                      saturate<T>(g.z * s), saturate<T>(g.w * s)};
+  const float v[8] = {saturate<T>(f.x * s, s), saturate<T>(f.y * s, s),
+                      saturate<T>(f.z * s, s), saturate<T>(f.w * s, s),
+                      saturate<T>(g.x * s, s), saturate<T>(g.y * s, s),
+                      saturate<T>(g.z * s, s), saturate<T>(g.w * s, s)};
   if constexpr (sizeof(T) == 4) {
     reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -673,9 +680,9 @@ __device__ __forceinline__ void store16(T* out, uint4 codes, float s, int vec) {
     const float4 f = decode4<C>(w[i]);
     v[4 * i] = f.x * s, v[4 * i + 1] = f.y * s, v[4 * i + 2] = f.z * s, v[4 * i + 3] = f.w * s;
   }
-  if (sizeof(T) == 2 && fabsf(s) > kTop / kLargest) {
+  if (fabsf(s) > kTop / kLargest) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = saturate<T>(v[i]);
+    for (int i = 0; i < 16; ++i) v[i] = saturate<T>(v[i], s);
   }
   if (!vec) {
 #pragma unroll
@@ -698,7 +705,9 @@ __device__ __forceinline__ void store16(T* out, uint4 codes, float s, int vec) {
 // by side as a CTA holds, or the whole CTA in turns.
 inline int piece_threads(int pieces) { return pieces >= 256 ? 256 : 256 / pieces * pieces; }
 
-// Rows by slot; a thread reads the same piece of kRows rows at once.
+// Rows by slot; a thread reads the same piece of kRows rows at once (with more
+// CTAs in flight one does best: both sides of 32768 rows of 4 heads of 128 to
+// bf16, 101 MB, 23.7 us = 4.3 TB/s; 2 and 4 rows 24.2 and 25.5). Bound by HBM.
 constexpr int kRows = 1;
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)

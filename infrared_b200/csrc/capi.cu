@@ -331,7 +331,8 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
                 void* workspace, size_t workspace_bytes, int32_t* err,
                 cudaStream_t stream, const float* rope_cos = nullptr,
                 const float* rope_sin = nullptr, int64_t rope_stride = 0, int fmt = 0,
-                const float* k_scale = nullptr, const float* v_scale = nullptr) {
+                const float* k_scale = nullptr, const float* v_scale = nullptr,
+                bool keep_empty = false) {
   Plan plan;
   int rc = make_plan(s, &plan, fmt);
   if (rc) return rc;
@@ -423,6 +424,7 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
   a.err = err;
   a.k_scale = k_scale;
   a.v_scale = v_scale;
+  a.keep_empty = keep_empty ? 1 : 0;
 
   int e;
   if (plan.path == 2 && fmt) {
@@ -653,8 +655,12 @@ constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy pe
 // kernel cannot read in place, up to 8 GiB), else in the blocks' own places.
 // Measured, dense against in place (blocks of 16): 4 prompts of 2048 rows 223 us
 // against 235, six sequences of up to 300 rows 36 us against 40. fp32 rows go to
-// the fp32 tile kernel, unless there are a few rows per sequence: these split
-// over the SMs as decode rows do (six single rows over 1000 keys: 44 us).
+// the fp32 tile kernel, unless there are so few per sequence that most of a tile
+// would be empty: these split over the SMs as decode rows do. Decoded against
+// tiles, 28 / 4 heads of 128: 64 single rows over 300 keys 52 us against 95, 256
+// over 1000 441 against 972, 8 x 4 rows over 1000 71 against 161; 64 x 4 rows 438
+// against 283, 256 rows of one prompt 93 against 54 (which a frame padded to one
+// sequence per row still pays: only the device knows its real number).
 int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
@@ -674,7 +680,7 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   const bool tc = rows_ok && s->max_blocks > 0 && (p->dense || in_place);
   if (g_prefill_path >= 2 && !(tc && (g_prefill_path == 2 || s->head_dim == 128)))
     return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but shape not eligible");
-  const bool few = s->total_q <= 4 * static_cast<int64_t>(s->num_seqs) &&
+  const bool few = s->total_q <= (s->total_q <= 64 ? 4 : 2) * static_cast<int64_t>(s->num_seqs) &&
                    s->num_heads / s->num_kv_heads <= 16;
   p->path = tc && g_prefill_path != 1 ? (g_prefill_path == 3 ? 3 : 2) : (few ? 1 : 4);
   if (p->path == 2 || p->path == 3) {
@@ -1300,9 +1306,10 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     if (e) return cuda_status(e, "prefill row tables");
     ir_decode_shape d = rows_shape(s);
     const size_t off = p.rows_table + p.rows_ctx;
+    // (rows of no sequence have an empty context and stay as they are)
     return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr,
                        0, nullptr, row_bt, row_ctx, &d, ws + off, workspace_bytes - off, err_flag,
-                       st, nullptr, nullptr, 0, kv_format, k_scale, v_scale);
+                       st, nullptr, nullptr, 0, kv_format, k_scale, v_scale, true);
   }
   irb::PrefillArgs a{};
   a.q = q;

@@ -79,6 +79,7 @@ struct DecodeArgs {
   // 8-bit pools: fp32 scales [num_blocks, Hkv] (null: pools of the dtype)
   const float* k_scale;
   const float* v_scale;
+  int keep_empty;  // 1: rows of empty contexts keep what `out` holds
 };
 
 __device__ __forceinline__ int clamp_ctx(int c, const DecodeArgs& a) {
@@ -236,6 +237,7 @@ __device__ void find_share(const DecodeArgs& a, int g, int kv0, int nkv,
   const bool publish = (g == 0 && kv0 == 0);
   auto empty_rows = [&](int b) {
     // empty context: zero rows (and lse = -inf) of this CTA's heads
+    if (a.keep_empty) return;
     for (int i = 0; i < nkv * a.n_rep * a.D; ++i) {
       const int h = kv0 * a.n_rep + i / a.D, d = i % a.D;
       if (a.lse_mode) {

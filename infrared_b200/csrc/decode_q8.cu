@@ -2,19 +2,25 @@
 // block and kv head): TMA-fed, warp-specialised, half the bytes of the 16-bit
 // kernel per token.
 //
-// Work partition, pieces and merge are the 16-bit kernel's (decode_common.cuh).
-// A CTA owns HG kv heads and one share of the 16-token tiles. The producer
-// warp resolves 32 tiles at a time and sends items of up to W = 8 / HG
-// neighbouring tiles of one sequence through a ring of stages; its lanes issue
-// the tiles' tensor copies (one box per block and side: [HG][rows][D] bytes)
-// and copy the blocks' scales with 4-byte asynchronous copies that complete on
-// the same barrier. Two sets of 8 consumer warps take the items in turn, warp
-// (head, w) of a set tile w of the item: the work on a tile is a chain of
-// dependent steps, so the warps of an SM hide one another's latency (8 warps
-// alone: 43 us for 64 sequences of 512-4096 tokens, against 33 us). For
-// groups of 9-16 query heads both sets take every item, each for 8 of the
-// heads. At the end of a segment the warps of a head combine their states
-// through shared memory, in halves.
+// Work partition and pieces are the 16-bit kernel's (decode_common.cuh). A CTA
+// owns HG kv heads and one share of the 16-token tiles. The producer warp
+// resolves 32 tiles at a time, a lane each: sequence, block and scales. Items
+// are up to W neighbouring tiles of one sequence and travel through a ring of
+// stages; a tile's lane issues its tensor copies (one box per block and side:
+// [HG][rows][D] bytes) and stores its scales beside them. 8 consumer warps share
+// an item: WT = 8 / HG of them hold a state of each head (8 / (2 HG) for groups
+// of 9-16 query heads, which make two sets of 8 with states of their own), and a
+// warp takes tiles w and w + WT of the W = 2 WT together, since the work on a
+// tile is a chain of dependent steps (blocks of 8 rows: one, a second set of
+// scales takes the registers). 16 warps of half the registers spilled and were
+// slower. At the end of a segment the warps of a state are combined through
+// shared memory, in halves.
+//
+// Bound by HBM and by fixed costs: 64 sequences of 512-4096 tokens, 28 / 4 heads
+// of 128, e4m3 (163 MB): 38.1 us = 4.3 TB/s; 4 of 32768, int8 (134 MB): 31.3 us.
+// Without the arithmetic the same copies take 35.1 and a device copy of 100 MB
+// takes 35. Around the stream stand finding the share (1.3), the first tiles'
+// tables (2.4), the first bytes (4.8), the last flush (1.4) and the merge (2.5).
 //
 // Mathematics of a tile (16 tokens, one kv head, 8 query heads):
 //   S^T[16 x 8] = K[16 x D] . Q^T     (codes as fp16, q as fp16)
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (lane == 0) ri->start = from, ri->end = to;
       __syncwarp();
-    } else if (g == 0) {
+    } else if (g == 0 && !a.keep_empty) {
       for (int sb = warp - 1; sb < a.B; sb += kConsumers) {
         if (clamp_ctx(a.context_lens[sb], a) != 0) continue;
         T* o = reinterpret_cast<T*>(a.out) + sb * a.out_stride +
@@ -363,7 +369,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           set_err(a.err, IR_DEVERR_TIMEOUT);
         }
       }
+      abort = !__all_sync(kFull, good);
     }
+    // (given up: the copies under way still need this shared memory)
+    if (abort)
+      for (int i = 0; i < NS; ++i)
+        mbar_wait_bounded(&full[i], static_cast<uint32_t>(i) < slot ? par ^ 1u : par);
     return;
   }
 

@@ -124,7 +124,9 @@ int launch_norm_t(const NormRopeArgs& a, int vec, int sms, cudaStream_t s) {
   constexpr int kTok = kNormThreads / (D / 8);  // tokens per CTA
   const int64_t gx = (a.n + kTok - 1) / kTok;
   const int heads = a.H + a.Hkv;
-  // pieces of heads: whole tokens where these fill the GPU, else one batch
+  // pieces of heads: whole tokens where these fill the GPU (cos, sin and the
+  // weights are read once), else one batch, which is what runs side by side (64
+  // rows of 28 + 4 heads: 8 CTAs a token group, 2.4 us)
   NormRopeArgs b = a;
   b.hpg = gx >= 2 * sms ? heads : kBatch;
   cudaLaunchConfig_t cfg = {};

@@ -80,7 +80,8 @@ class PagedKVPoolQ8:
         self.k, self.v = (torch.zeros(shape, dtype=torch.int8, device=device).view(kv_dtype)
                           for _ in range(2))
         self.k_scale, self.v_scale = (
-            torch.zeros((num_layers, num_blocks, num_kv_heads), device=device) for _ in range(2))
+            torch.zeros((num_layers, num_blocks, num_kv_heads), dtype=torch.float32, device=device)
+            for _ in range(2))
 
     def layer(self, layer_idx: int):
         """``(k, v, k_scale, v_scale)`` of one layer, as the ``*_q8`` calls take them."""

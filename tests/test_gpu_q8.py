@@ -222,6 +222,25 @@ def test_gather_bad_slots_give_zero_rows():
     np.testing.assert_array_equal(host(got[1]), q8.values(codes, scale, 16)[5])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_largest_values(dtype):
+    """The largest value of the type comes back as its code does, saturated where
+    the rounded code times its scale (2^128 for 32 exponents more) is beyond it."""
+    top = torch.finfo(dtype).max
+    for fmt in ("e4m3", "int8"):
+        x = torch.full((16, 1, 64), top, dtype=dtype, device="cuda")
+        x[1] = -top
+        pool = codes_to(np.zeros((16, 1, 64)), fmt)
+        sc = torch.zeros(1, 1, device="cuda")
+        irb.cache_write_q8(x, x, pool, pool.clone(), sc, sc.clone(), torch.arange(16, device="cuda"), 16)
+        codes, scale = np.zeros((16, 1, 64)), np.zeros((1, 1))
+        q8.write(codes, scale, x.double().cpu().numpy(), range(16), 16, fmt)
+        assert float(sc) == scale[0, 0]
+        got = irb.cache_gather_q8(pool, sc, torch.arange(16, device="cuda"), 16, dtype)
+        want = torch.from_numpy(q8.values(codes, scale, 16)).clamp(-top, top).to(dtype)
+        assert torch.equal(got.cpu(), want) and torch.isfinite(got).all()
+
+
 # ---------------------------------------------------------------- attention
 
 
@@ -623,6 +642,47 @@ def test_prefill_bad_metadata_is_flagged(dtype):
     assert (out[40:] == 7.0).all() and torch.equal(out[:40], good[:40])
 
 
+@pytest.mark.parametrize("path,dtype", [(2, torch.bfloat16), (1, torch.bfloat16),
+                                        (1, torch.float32)])
+def test_prefill_few_rows_leave_the_others_alone(path, dtype):
+    """One or two rows per sequence, with rows of no sequence behind them."""
+    rng = np.random.default_rng(5)
+    f = wl.prefill_frame("t", 3, [10, 0, 300], [1, 2, 1], 8, 2, 64, 16)
+    kc, ks = make_pool(rng, f.num_blocks, 16, 2, 64, "e4m3")
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    q = dev(rng.normal(size=(9, 8, 64))).to(dtype)
+    args = (pool, pool, sc, sc, dev(f.block_tables), dev(f.context_lens), dev(f.q_start), f.scale,
+            16)
+    ops.set_prefill_path(0 if path == 2 or dtype == torch.float32 else 1)
+    try:
+        assert ops.prefill_plan_q8(q, pool, args[4], args[6], 16)[0] == path
+        good = irb.paged_prefill_q8(q[:4], *args)
+        out = torch.full_like(q, 7.0)
+        irb.paged_prefill_q8(q, *args, out=out)
+    finally:
+        ops.set_prefill_path(0)
+    assert torch.equal(out[:4], good) and (out[4:] == 7.0).all()
+
+
+def test_prefill_overflow_of_later_positions_stays_there():
+    """A V whose code times its scale is beyond the type is held as its largest
+    value: rows before it do not meet an infinity."""
+    rng = np.random.default_rng(6)
+    f = wl.prefill_frame("t", 3, [0], [60], 4, 2, 64, 16)
+    kc, ks = make_pool(rng, f.num_blocks, 16, 2, 64, "e4m3")
+    q = dev(rng.normal(size=(60, 4, 64))).to(torch.bfloat16)
+    run = lambda c, s: irb.paged_prefill_q8(  # noqa: E731
+        q, codes_to(kc, "e4m3"), codes_to(c, "e4m3"), dev(ks.astype(np.float32)),
+        dev(s.astype(np.float32)), dev(f.block_tables), dev(f.context_lens), dev(f.q_start),
+        f.scale, 16)
+    clean = run(kc, ks)
+    vc, vs = kc.copy(), ks.copy()
+    blk = int(f.block_tables[0, 2])            # positions 32 .. 47
+    vc[blk * 16:(blk + 1) * 16] = 448.0
+    vs[blk] = 2.0 ** 120
+    assert torch.equal(run(vc, vs)[:32], clean[:32])
+
+
 def test_prefill_row_is_the_decode_row():
     """A prompt's last row and the decode of the same token agree within both bounds."""
     rng = np.random.default_rng(0)
@@ -687,6 +747,15 @@ def test_prompt_then_decode_steps(fmt):
 
 
 # ---------------------------------------------------------------- pool, seam, streams, graphs
+
+
+def test_pool_scales_are_fp32_under_another_default_type():
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        pool = irb.PagedKVPoolQ8(1, 2, 16, 1, 64, torch.bfloat16)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert pool.k_scale.dtype == pool.v_scale.dtype == torch.float32
 
 
 @pytest.mark.parametrize("kv", [torch.float8_e4m3fn, torch.int8])
