@@ -475,7 +475,8 @@ size_t ir_cache_write_q8_workspace_size(int64_t num_tokens, int64_t num_slots,
  * flagged IR_DEVERR_SLOT; of two rows for one slot the later one counts. The
  * result does not depend on the order of the other rows.
  * k, v: [num_tokens, num_kv_heads, head_dim] of dtype with row strides in
- * elements; head_dim 64 or 128; block_size up to 1024.
+ * elements (below 2^31); head_dim 64 or 128; block_size up to 1024; at most 4096
+ * heads, 2^30 rows and 2^31 - 65 slots (gather: the same).
  */
 int ir_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
                       void* k_pool, void* v_pool, float* k_scale, float* v_scale,
@@ -499,7 +500,8 @@ int ir_cache_gather_q8(void* out, const void* pool, const float* scale, const in
  * shape->flags must be 0. Workspace and plan of the same shape come from the
  * two calls below (path 2: TMA + mma kernel for 16-bit q, block_size 8 or a
  * multiple of 16; path 1: CUDA cores for everything else). Scores, softmax and
- * sums are fp32; scales may have any value. */
+ * sums are fp32; scales may have any value (values of K or V beyond about 2^100
+ * overflow in the sums). */
 size_t ir_paged_decode_q8_workspace_size(const ir_decode_shape* shape, int kv_format);
 int ir_paged_decode_q8_plan(const ir_decode_shape* shape, int kv_format, int* path,
                             int* ctas_per_kv_head);
