@@ -519,13 +519,13 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *     bf16 for power-of-two scales. The workspace holds the histories (or one
  *     layer's pool) in shape->dtype and can serve every layer. A NaN in V makes
  *     its whole head NaN in the rows that attend it;
- *   4 everything else: fp32 tiles on the CUDA cores, codes read directly;
- *   1 as 4 for at most 2 query rows per sequence (4, up to 64 rows): every row
- *     decoded as its own sequence (ir_paged_decode_q8).
+ *   1 at most 8 query rows per sequence on average (fp32: 2, or 16 up to 64
+ *     rows): every row decoded as its own sequence (ir_paged_decode_q8);
+ *   4 everything else: fp32 tiles on the CUDA cores, codes read directly.
  * Rows of q that belong to no sequence leave theirs of out as they are.
  * Values of K or V at positions that a row does not attend change nothing in it,
  * NaN included. ir_set_prefill_path(2 or 3) asks for the tensor cores, 1 for
- * the others. */
+ * paths 1 and 4. */
 size_t ir_paged_prefill_q8_workspace_size(const ir_prefill_shape* shape, int kv_format);
 int ir_paged_prefill_q8_plan(const ir_prefill_shape* shape, int kv_format, int* path);
 int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void* v_pool,

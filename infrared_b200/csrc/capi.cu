@@ -654,13 +654,14 @@ constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy pe
 // where that takes at most twice the pool's rows (or, for block sizes that the
 // kernel cannot read in place, up to 8 GiB), else in the blocks' own places.
 // Measured, dense against in place (blocks of 16): 4 prompts of 2048 rows 223 us
-// against 235, six sequences of up to 300 rows 36 us against 40. fp32 rows go to
-// the fp32 tile kernel, unless there are so few per sequence that most of a tile
-// would be empty: these split over the SMs as decode rows do. Decoded against
-// tiles, 28 / 4 heads of 128: 64 single rows over 300 keys 52 us against 95, 256
-// over 1000 441 against 972, 8 x 4 rows over 1000 71 against 161; 64 x 4 rows 438
-// against 283, 256 rows of one prompt 93 against 54 (which a frame padded to one
-// sequence per row still pays: only the device knows its real number).
+// against 235, six sequences of up to 300 rows 36 us against 40. fp32 rows and
+// unaligned ones go to the fp32 tile kernel. Few rows per sequence are decoded as
+// sequences of their own, from the codes and split over the SMs (28 / 4 heads of
+// 128, decoded against tensor cores): 64 x 2 rows over 512-4096 keys 65 us against
+// 373, 64 x 8 209 against 379, 64 x 16 444 against 400; 1 x 8 over 4096 18 against
+// 42; 4 x 8 over 100 15 against 12. fp32, decoded against tiles: 64 single rows
+// over 300 keys 52 against 95, 64 x 4 over 50 49 against 31, but 4 x 16 over
+// 512-4096 174 against 275.
 int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
@@ -680,9 +681,13 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   const bool tc = rows_ok && s->max_blocks > 0 && (p->dense || in_place);
   if (g_prefill_path >= 2 && !(tc && (g_prefill_path == 2 || s->head_dim == 128)))
     return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but shape not eligible");
-  const bool few = s->total_q <= (s->total_q <= 64 ? 4 : 2) * static_cast<int64_t>(s->num_seqs) &&
-                   s->num_heads / s->num_kv_heads <= 16;
-  p->path = tc && g_prefill_path != 1 ? (g_prefill_path == 3 ? 3 : 2) : (few ? 1 : 4);
+  const int64_t most = half ? 8 : s->total_q <= 64 ? 16 : 2;  // rows per sequence
+  const bool few = s->num_heads / s->num_kv_heads <= 16 &&
+                   s->total_q <= most * static_cast<int64_t>(s->num_seqs);
+  p->path = g_prefill_path >= 2 ? g_prefill_path
+            : few               ? 1
+            : tc && g_prefill_path == 0 ? 2
+                                : 4;
   if (p->path == 2 || p->path == 3) {
     const int64_t rows = p->dense ? dense_rows : s->num_slots;
     p->pool = align256(static_cast<size_t>(rows) * row_bytes);

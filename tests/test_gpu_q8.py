@@ -558,7 +558,13 @@ def test_prefill_layouts(bs, width, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_prefill_few_rows_and_forced_paths(dtype):
     spans = [(100, 1), (0, 1), (33, 4), (500, 2)]
-    check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 2 if dtype == torch.bfloat16 else 1)
+    check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 1)
+    if dtype == torch.bfloat16:
+        ops.set_prefill_path(2)
+        try:
+            check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 2)
+        finally:
+            ops.set_prefill_path(0)
     ops.set_prefill_path(1)
     try:
         check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 1)
@@ -653,7 +659,7 @@ def test_prefill_few_rows_leave_the_others_alone(path, dtype):
     q = dev(rng.normal(size=(9, 8, 64))).to(dtype)
     args = (pool, pool, sc, sc, dev(f.block_tables), dev(f.context_lens), dev(f.q_start), f.scale,
             16)
-    ops.set_prefill_path(0 if path == 2 or dtype == torch.float32 else 1)
+    ops.set_prefill_path(2 if path == 2 else 0)
     try:
         assert ops.prefill_plan_q8(q, pool, args[4], args[6], 16)[0] == path
         good = irb.paged_prefill_q8(q[:4], *args)
