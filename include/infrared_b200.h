@@ -518,7 +518,9 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *     conversion is paid once, not once per 128 query rows and head. Exact in
  *     bf16 for power-of-two scales. The workspace holds the histories (or one
  *     layer's pool) in shape->dtype and can serve every layer. A NaN in V makes
- *     its whole head NaN in the rows that attend it;
+ *     its whole head NaN in the rows that attend it. In frames of at most 64
+ *     rows per sequence on average and long tables, sequences of up to 8 rows are
+ *     decoded as in 1 beside it;
  *   1 at most 8 query rows per sequence on average (fp32: 2, or 16 up to 64
  *     rows): every row decoded as its own sequence (ir_paged_decode_q8);
  *   4 everything else: fp32 tiles on the CUDA cores, codes read directly.

@@ -158,7 +158,7 @@ __global__ void prefill_rows_kernel(const int32_t* __restrict__ bt, int64_t bt_s
                                     const int32_t* __restrict__ ctx,
                                     const int32_t* __restrict__ q_start, int S, int max_blocks,
                                     int max_ctx, int32_t* __restrict__ row_bt,
-                                    int32_t* __restrict__ row_ctx, int32_t* err) {
+                                    int32_t* __restrict__ row_ctx, int32_t* err, int only_short) {
   const int t = blockIdx.x;
   __shared__ int s_seq;
   if (threadIdx.x == 0) {
@@ -181,14 +181,16 @@ __global__ void prefill_rows_kernel(const int32_t* __restrict__ bt, int64_t bt_s
       } else {
         c = cs - ql + (t - q_start[found]) + 1;
       }
+      if (only_short > 0 && ql > only_short) c = 0;
     } else {
       found = -1;
     }
     row_ctx[t] = c;
-    s_seq = found;
+    s_seq = only_short > 0 && c == 0 ? -2 : found;
   }
   __syncthreads();
   const int sq = s_seq;
+  if (sq == -2) return;  // (an empty context's table is not read)
   for (int j = threadIdx.x; j < max_blocks; j += blockDim.x)
     row_bt[static_cast<int64_t>(t) * max_blocks + j] =
         sq >= 0 ? bt[static_cast<int64_t>(sq) * bt_stride + j] : 0;
@@ -413,10 +415,11 @@ int launch_build_decode_inputs(const int32_t* bt, int64_t bt_stride,
 
 int launch_prefill_rows(const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
                         const int32_t* q_start, int S, int total_q, int max_blocks, int max_ctx,
-                        int32_t* row_bt, int32_t* row_ctx, int32_t* err, cudaStream_t stream) {
+                        int32_t* row_bt, int32_t* row_ctx, int32_t* err, cudaStream_t stream,
+                        int only_short) {
   if (total_q == 0) return 0;
   prefill_rows_kernel<<<total_q, 128, 0, stream>>>(bt, bt_stride, ctx, q_start, S, max_blocks,
-                                                   max_ctx, row_bt, row_ctx, err);
+                                                   max_ctx, row_bt, row_ctx, err, only_short);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -760,11 +760,13 @@ template <typename T, typename C>
 __global__ void __launch_bounds__(256)
     expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp, const float* ks,
                          const float* vs, const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
-                         int max_blocks, int64_t num_blocks, int Hkv, int D, int bs,
-                         int32_t* table, int64_t cap, int table_block, int32_t* err) {
+                         const int32_t* q_start, int short_rows, int max_blocks,
+                         int64_t num_blocks, int Hkv, int D, int bs, int32_t* table, int64_t cap,
+                         int table_block, int32_t* err) {
   wait_prior_grid();
   const int sq = blockIdx.x;
-  const int64_t c0 = ctx[sq];
+  // (sequences of few rows are attended from the codes)
+  const int64_t c0 = q_start[sq + 1] - q_start[sq] > short_rows ? ctx[sq] : 0;
   const int pieces = Hkv * D / 8;
   const int tpr = pieces < 256 ? pieces : 256;
   const int side = blockDim.x / tpr;
@@ -935,10 +937,10 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
 
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
-                         int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
-                         int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
-                         int32_t* table, int64_t cap, int table_block, int32_t* err,
-                         cudaStream_t stream) {
+                         int64_t bt_stride, const int32_t* ctx, const int32_t* q_start,
+                         int short_rows, int S, int max_blocks, int64_t num_blocks, int Hkv,
+                         int D, int bs, int dtype, int fmt, int32_t* table, int64_t cap,
+                         int table_block, int32_t* err, cudaStream_t stream) {
   if (S == 0 || max_blocks == 0) return 0;
   const dim3 grid(static_cast<unsigned>(S),
                   static_cast<unsigned>(max_blocks < 4096 ? max_blocks : 4096));
@@ -949,7 +951,8 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
                            piece_threads(Hkv * D / 8), 0, stream, static_cast<T*>(k_out),
                            static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
                            static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride,
-                           ctx, max_blocks, num_blocks, Hkv, D, bs, table, cap, table_block, err);
+                           ctx, q_start, short_rows, max_blocks, num_blocks, Hkv, D, bs, table,
+                           cap, table_block, err);
     });
   });
 }

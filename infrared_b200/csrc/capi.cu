@@ -643,10 +643,13 @@ int check_q8_rows(int64_t n, int hkv, int d, int bs, int64_t num_slots, int dtyp
 struct PrefillQ8Plan {
   int path;        // 1 rows as decode rows, 2 / 3 expansion + tensor cores, 4 fp32 tiles
   bool dense;      // the expansion lays the histories out sequence by sequence
+  bool split;      // sequences of up to kFewRows rows are decoded row by row beside it
   int64_t cap;     // rows of a sequence there
-  // workspace: K, V, table, or the rows path's tables and contexts
-  size_t pool, table_off, rows_table, rows_ctx, bytes;
+  // workspace: K, V, table; the decoded rows' tables, contexts and scratch
+  size_t pool, table_off, rows_off, rows_table, rows_ctx, bytes;
 };
+
+constexpr int kFewRows = 8;
 
 constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy per key tile
 
@@ -681,9 +684,9 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   const bool tc = rows_ok && s->max_blocks > 0 && (p->dense || in_place);
   if (g_prefill_path >= 2 && !(tc && (g_prefill_path == 2 || s->head_dim == 128)))
     return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but shape not eligible");
-  const int64_t most = half ? 8 : s->total_q <= 64 ? 16 : 2;  // rows per sequence
-  const bool few = s->num_heads / s->num_kv_heads <= 16 &&
-                   s->total_q <= most * static_cast<int64_t>(s->num_seqs);
+  const int64_t most = half ? kFewRows : s->total_q <= 64 ? 16 : 2;  // rows per sequence
+  const int group = s->num_heads / s->num_kv_heads;
+  const bool few = group <= 16 && s->total_q <= most * s->num_seqs;
   p->path = g_prefill_path >= 2 ? g_prefill_path
             : few               ? 1
             : tc && g_prefill_path == 0 ? 2
@@ -694,14 +697,24 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
     p->table_off = 2 * p->pool;
     p->bytes = p->table_off +
                (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
-  } else if (p->path == 1) {
+    // A step of many decode rows and a prompt or two: expanding the histories of
+    // the former would cost 2.5 ns a row, most of the call (64 single rows over
+    // 512-4096 keys beside 512 rows: 384 us, decoded beside 71; 32 over 100-500
+    // 72 and 52). Decoding none costs three launches over all rows (32 x 200 rows
+    // over 500 142 us, with them 196), hence the limits.
+    p->split = g_prefill_path == 0 && group <= 16 && s->total_q <= 4096 &&
+               s->total_q <= int64_t{64} * s->num_seqs &&
+               static_cast<int64_t>(s->num_seqs - 1) * s->max_blocks * bs >= 16384;
+  }
+  if (p->path == 1 || p->split) {
     ir_decode_shape d = rows_shape(s);
     Plan plan;
     rc = make_plan(&d, &plan, fmt);
     if (rc) return rc;
+    p->rows_off = p->bytes;
     p->rows_table = align256(static_cast<size_t>(s->total_q) * s->max_blocks * 4);
     p->rows_ctx = align256(static_cast<size_t>(s->total_q) * 4);
-    p->bytes = p->rows_table + p->rows_ctx + plan.bytes;
+    p->bytes += p->rows_table + p->rows_ctx + plan.bytes;
   }
   return IR_OK;
 }
@@ -1092,10 +1105,12 @@ size_t ir_paged_prefill_workspace_size(const ir_prefill_shape* shape) {
   return total;
 }
 
-int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v_pool,
-                     const int32_t* block_tables, const int32_t* context_lens,
-                     const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
-                     size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream) {
+// (sequences of at most short_rows rows are left out; 0: none)
+static int prefill_impl(void* out, const void* q, const void* k_pool, const void* v_pool,
+                        const int32_t* block_tables, const int32_t* context_lens,
+                        const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
+                        size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream,
+                        int short_rows) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
   if (s->num_seqs == 0 || s->total_q == 0) return IR_OK;
@@ -1134,6 +1149,7 @@ int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v
     a.num_blocks = s->num_slots / s->block_size;
     a.scale_log2 = s->scale * irb::kLog2e;
     a.err = err_flag;
+    a.short_rows = short_rows;
     CUtensorMap tmq, tmk, tmv;
     const int rows = s->block_size < 128 ? s->block_size : 128;
     // a CTA of a pair stages 64 keys of each K tile
@@ -1168,6 +1184,14 @@ int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v
   return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr, 0,
                      nullptr, row_bt, row_ctx, &d, ws + tb + cb, workspace_bytes - tb - cb,
                      err_flag, st);
+}
+
+int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v_pool,
+                     const int32_t* block_tables, const int32_t* context_lens,
+                     const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
+                     size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream) {
+  return prefill_impl(out, q, k_pool, v_pool, block_tables, context_lens, q_start, s, workspace,
+                      workspace_bytes, err_flag, stream, 0);
 }
 
 // ---------------------------------------------------------------- 8-bit cache
@@ -1302,20 +1326,23 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     p.path = 4;
   }
   int e;
-  if (p.path == 1) {
-    int32_t* row_bt = reinterpret_cast<int32_t*>(ws);
-    int32_t* row_ctx = reinterpret_cast<int32_t*>(ws + p.rows_table);
-    e = irb::launch_prefill_rows(block_tables, s->bt_stride, context_lens, q_start, s->num_seqs,
-                                 s->total_q, s->max_blocks, s->max_blocks * s->block_size, row_bt,
-                                 row_ctx, err_flag, st);
-    if (e) return cuda_status(e, "prefill row tables");
+  // rows as sequences of their own (only_short: those of sequences of few rows)
+  auto decode_rows = [&](int only_short) {
+    int32_t* row_bt = reinterpret_cast<int32_t*>(ws + p.rows_off);
+    int32_t* row_ctx = reinterpret_cast<int32_t*>(ws + p.rows_off + p.rows_table);
+    int rc = irb::launch_prefill_rows(block_tables, s->bt_stride, context_lens, q_start,
+                                      s->num_seqs, s->total_q, s->max_blocks,
+                                      s->max_blocks * s->block_size, row_bt, row_ctx, err_flag, st,
+                                      only_short);
+    if (rc) return cuda_status(rc, "prefill row tables");
     ir_decode_shape d = rows_shape(s);
-    const size_t off = p.rows_table + p.rows_ctx;
-    // (rows of no sequence have an empty context and stay as they are)
+    const size_t off = p.rows_off + p.rows_table + p.rows_ctx;
+    // (rows of an empty context, which no sequence or a longer one has, stay)
     return decode_impl(Mode::kFinal, out, nullptr, nullptr, q, k_pool, v_pool, nullptr, nullptr,
                        0, nullptr, row_bt, row_ctx, &d, ws + off, workspace_bytes - off, err_flag,
                        st, nullptr, nullptr, 0, kv_format, k_scale, v_scale, true);
-  }
+  };
+  if (p.path == 1) return decode_rows(0);
   irb::PrefillArgs a{};
   a.q = q;
   a.q_stride = s->q_stride;
@@ -1341,11 +1368,14 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, st);
     return cuda_status(e, "8-bit prefill launch");
   }
+  const int few = p.split ? kFewRows : 0;
+  if (few && (rc = decode_rows(few)) != IR_OK) return rc;
   int32_t* table = p.dense ? reinterpret_cast<int32_t*>(ws + p.table_off) : nullptr;
   e = irb::launch_expand_blocks(ws, ws + p.pool, k_pool, v_pool, k_scale, v_scale, block_tables,
-                                s->bt_stride, context_lens, s->num_seqs, s->max_blocks,
-                                a.num_blocks, s->num_kv_heads, s->head_dim, s->block_size,
-                                s->dtype, kv_format, table, p.cap, kDenseBlock, err_flag, st);
+                                s->bt_stride, context_lens, q_start, few, s->num_seqs,
+                                s->max_blocks, a.num_blocks, s->num_kv_heads, s->head_dim,
+                                s->block_size, s->dtype, kv_format, table, p.cap, kDenseBlock,
+                                err_flag, st);
   if (e) return cuda_status(e, "8-bit block expansion launch");
   ir_prefill_shape x = *s;
   if (p.dense) {
@@ -1354,8 +1384,8 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     x.bt_stride = x.max_blocks;
     x.num_slots = p.cap * s->num_seqs;
   }
-  return ir_paged_prefill(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
-                          q_start, &x, nullptr, 0, err_flag, stream);
+  return prefill_impl(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
+                      q_start, &x, nullptr, 0, err_flag, stream, few);
 }
 
 // ---------------------------------------------------------------- q/k norm + rotation

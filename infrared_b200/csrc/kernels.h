@@ -25,6 +25,7 @@ struct PrefillArgs {
   int64_t num_slots, num_blocks;
   float scale_log2;
   int32_t* err;
+  int short_rows;  // sequences of at most this many rows are left out (0: none)
 };
 
 // tcgen05 kernel: 16-bit dtypes, D in {64, 128}, block size a power of two
@@ -112,10 +113,10 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
 // not finite it becomes 0 and its K NaN.
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
-                         int64_t bt_stride, const int32_t* ctx, int S, int max_blocks,
-                         int64_t num_blocks, int Hkv, int D, int bs, int dtype, int fmt,
-                         int32_t* table, int64_t cap, int table_block, int32_t* err,
-                         cudaStream_t stream);
+                         int64_t bt_stride, const int32_t* ctx, const int32_t* q_start,
+                         int short_rows, int S, int max_blocks, int64_t num_blocks, int Hkv,
+                         int D, int bs, int dtype, int fmt, int32_t* table, int64_t cap,
+                         int table_block, int32_t* err, cudaStream_t stream);
 
 // prefill_q8.cu: packed rows over an 8-bit pool in fp32 on the CUDA cores
 // (args as in PrefillArgs)
@@ -168,7 +169,8 @@ int launch_build_decode_inputs(const int32_t* bt, int64_t bt_stride,
                                uint32_t min_bits, cudaStream_t stream);
 int launch_prefill_rows(const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
                         const int32_t* q_start, int S, int total_q, int max_blocks, int max_ctx,
-                        int32_t* row_bt, int32_t* row_ctx, int32_t* err, cudaStream_t stream);
+                        int32_t* row_bt, int32_t* row_ctx, int32_t* err, cudaStream_t stream,
+                        int only_short = 0);
 int launch_derive_varlen(const int64_t* gs, const void* mask, int64_t mask_stride,
                          int mask_elem_bytes, int Q, int64_t K, int bs, int max_blocks,
                          int32_t* bt, int32_t* ctx, int32_t* q_start, int32_t* nseq,

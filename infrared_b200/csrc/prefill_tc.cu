@@ -105,8 +105,10 @@ __device__ __forceinline__ void locate_tile(const PrefillArgs& a, int t, int lan
   for (int base = 0; base < a.S; base += 32) {
     const int sq = base + lane;
     int nt = 0;
-    if (sq < a.S) nt = (a.q_start[sq + 1] - a.q_start[sq] + TR - 1) / TR;
-    if (nt < 0) nt = 0;
+    if (sq < a.S) {
+      const int rows = a.q_start[sq + 1] - a.q_start[sq];
+      nt = rows <= a.short_rows ? 0 : (rows + TR - 1) / TR;
+    }
     int incl = nt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -573,6 +573,41 @@ def test_prefill_few_rows_and_forced_paths(dtype):
         ops.set_prefill_path(0)
 
 
+@pytest.mark.parametrize("dtype,fmt", [(torch.bfloat16, "e4m3"), (torch.float16, "int8")])
+def test_prefill_mixed_frame(dtype, fmt):
+    """Wide tables and both long and short sequences: those of up to 8 rows are
+    decoded from the codes, the others expanded; rows of neither stay."""
+    spans = [(300, 1), (0, 200), (500, 8), (100, 9), (20, 0), (64, 1)]
+    for bs in (16, 32):
+        check_prefill(28, 4, 128, bs, spans, dtype, fmt, 2, width=400, dirty=True)
+    check_prefill(8, 1, 64, 8, spans, dtype, fmt, 2, width=800, dirty=True)
+    f = wl.prefill_frame("t", 3, [s for s, _ in spans], [n for _, n in spans], 8, 2, 64, 16)
+    kc, ks = make_pool(np.random.default_rng(1), f.num_blocks, 16, 2, 64, fmt)
+    pool, sc = codes_to(kc, fmt), dev(ks.astype(np.float32))
+    q = dev(np.random.default_rng(2).normal(size=(250, 8, 64))).to(dtype)
+    out = torch.full_like(q, 7.0)
+    call = lambda q, **kw: irb.paged_prefill_q8(  # noqa: E731
+        q, pool, pool, sc, sc, dev(np.pad(f.block_tables, ((0, 0), (0, 400)))),
+        dev(f.context_lens), dev(f.q_start), f.scale, 16, **kw)
+    call(q, out=out)
+    assert (out[219:] == 7.0).all() and torch.equal(out[:219], call(q[:219]))
+    bad = f.context_lens.copy()
+    bad[0] = 0                                    # a short sequence, then a long one
+    bad[1] = 100
+    irb.paged_prefill_q8(q, pool, pool, sc, sc, dev(np.pad(f.block_tables, ((0, 0), (0, 400)))),
+                         dev(bad), dev(f.q_start), f.scale, 16, out=out.fill_(7.0))
+    with pytest.raises(irb.DeviceError, match="CONTEXT_LEN"):
+        irb.check_device_errors()
+    good = call(q[:219])
+    assert torch.equal(out[209:218], good[209:218])
+    # decoded rows are cut into pieces by the lengths of all of them: each result
+    # is within one output rounding (at most 2^-8), one of the weights (2^-11) and
+    # the scores' (72 * 2^-23 * 100 < 2^-10) of the same weighted mean of V
+    top = np.abs(q8.values(kc, ks, 16)).max()
+    rest = [*range(201, 209), 218]
+    assert (np.abs(host(out[rest]) - host(good[rest])) <= 2 * (2.0 ** -8 + 2.0 ** -9) * top).all()
+
+
 def test_prefill_unaligned_rows():
     rng = np.random.default_rng(4)
     n, h, d = 29, 8, 64
