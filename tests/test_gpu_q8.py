@@ -109,6 +109,16 @@ def test_write_many_tokens(n, hkv, d, bs, nb, order, fmt):
     _check_write(*case, bs, fmt, neg=(0, 17, n - 1))
 
 
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+@pytest.mark.parametrize("n,bs,nb", [(8193, 16, 600), (20000, 16, 1400), (32769, 16, 2100),
+                                     (20000, 1, 30000)])
+def test_write_links_of_long_calls(n, bs, nb, order):
+    """Calls whose rows are linked per block, over many CTAs and blocks."""
+    rng = np.random.default_rng(n)
+    case = _write_case(rng, n, 1, 64, bs, nb, "e4m3", torch.bfloat16, order)
+    _check_write(*case, bs, "e4m3", neg=(0, 17, n - 1))
+
+
 @pytest.mark.parametrize("n", [40, 1100])
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 def test_write_same_slot_twice_keeps_the_last_row(fmt, n):
