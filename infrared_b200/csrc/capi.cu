@@ -225,6 +225,7 @@ bool make_pool_map_q8(CUtensorMap* map, const void* pool, int64_t num_slots, int
 struct Plan {
   int path;     // 1 generic, 2 tma
   int G;        // CTAs per kv head
+  int per_seq;  // 8-bit TMA path: heads of a CTA that takes a whole sequence (0: shares)
   int dyn;      // dynamic tail units (TMA path, flag set)
   int inl;      // short rows merged in the decode kernel (TMA path, flag set)
   int64_t slots;  // partial slots per kv head
@@ -303,6 +304,15 @@ int make_plan(const ir_decode_shape* s, Plan* p, int fmt = 0) {
   if (e) return cuda_status(e, "cudaGetDevice");
   p->path = path;
   p->G = G;
+  p->per_seq = 0;
+  if (fmt && path == 2 && s->batch > 0) {
+    int sms = 1;
+    e = cached(-1, sm_count_now, 0, &sms);
+    if (e) return cuda_status(e, "device query");
+    p->per_seq = irb::q8_seq_heads(s->batch, s->num_kv_heads, s->num_heads / s->num_kv_heads,
+                                   static_cast<int64_t>(s->max_blocks) * s->block_size, sms);
+    if (p->per_seq) p->G = s->batch;  // (the workspace stays as large as for shares)
+  }
   const int64_t B = s->batch, H = s->num_heads, D = s->head_dim;
   const int groups = path == 2 ? s->num_kv_heads / head_group(s, fmt) : 0;
   const bool hdr = path == 2 && static_cast<size_t>(groups) * 8 <= kCtrBytes;
@@ -377,6 +387,8 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
       // count the workspace was sized for
       int G = 1;
       ctas_per_group(1, s, &G, fmt);
+      if (plan.per_seq) ctas_per_group(2, s, &plan.G, fmt);
+      plan.per_seq = 0;
       plan.G = G > plan.G ? plan.G : G;
     }
   }
@@ -430,7 +442,8 @@ int decode_impl(Mode mode, void* out, float* lse_o, float* lse_out,
   if (plan.path == 2 && fmt) {
     CUtensorMap tmk, tmv;
     const int rows = s->block_size == 8 ? 8 : 16;
-    const int hg = head_group(s, fmt);
+    const int hg = plan.per_seq ? plan.per_seq : head_group(s, fmt);
+    a.per_seq = plan.per_seq;
     if (!make_pool_map_q8(&tmk, k_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg) ||
         !make_pool_map_q8(&tmv, v_pool, s->num_slots, s->num_kv_heads, s->head_dim, rows, hg))
       return fail(IR_ERR_CUDA, "cuTensorMapEncodeTiled failed");

@@ -80,6 +80,7 @@ struct DecodeArgs {
   const float* k_scale;
   const float* v_scale;
   int keep_empty;  // 1: rows of empty contexts keep what `out` holds
+  int per_seq;     // > 0: a CTA per sequence and this many kv heads (no shares, no merge)
 };
 
 __device__ __forceinline__ int clamp_ctx(int c, const DecodeArgs& a) {

@@ -21,6 +21,8 @@
 // Without the arithmetic the same copies take 35.1 and a device copy of 100 MB
 // takes 35. Around the stream stand finding the share (1.3), the first tiles'
 // tables (2.4), the first bytes (4.8), the last flush (1.4) and the merge (2.5).
+// Short contexts (q8_seq_heads) have a CTA per sequence instead, without the
+// first and the last of these: one of 201 tokens, int8, 2 heads of 64, 5.5 us.
 //
 // Mathematics of a tile (16 tokens, one kv head, 8 query heads):
 //   S^T[16 x 8] = K[16 x D] . Q^T     (codes as fp16, q as fp16)
@@ -180,7 +182,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   // alone, 8 sequences a lane, without a block-wide scan (the merge kernel sums
   // the tile prefix itself then); the rows of empty sequences by the others.
   constexpr int kEach = 8;
-  if (a.B <= 32 * kEach) {
+  if (a.per_seq) {
+    if (warp == 0) {
+      const int c = a.context_lens[g], n = tiles_of(a, g);
+      if (lane == 0) {
+        if (clamp_ctx(c, a) != c) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
+        ri->start = 0;
+        ri->end = n;
+        ri->b_first = g;
+        ri->p_first = 0;
+      }
+      if (n == 0 && !a.keep_empty) {
+        T* o = reinterpret_cast<T*>(a.out) + g * a.out_stride +
+               static_cast<int64_t>(kv0) * a.n_rep * D;
+        for (int i = lane; i < HG * a.n_rep * D; i += 32) o[i] = DT<T>::from_f(0.f);
+      }
+      __syncwarp();
+    }
+  } else if (a.B <= 32 * kEach) {
     if (warp == 0) {
       int64_t sum = 0;
       int n[kEach];
@@ -938,7 +957,7 @@ int by_rows(const CallQ8* c) {
 }
 template <typename T, typename C, int D>
 int by_heads(const CallQ8* c) {
-  const int hg = q8_head_group(c->a->Hkv, c->a->n_rep);
+  const int hg = c->a->per_seq ? c->a->per_seq : q8_head_group(c->a->Hkv, c->a->n_rep);
   if (c->a->n_rep <= 8) {
     switch (hg) {
       case 1: return by_rows<T, C, D, 1, false>(c);
@@ -964,6 +983,19 @@ int by_code(int fmt, const CallQ8* c) {
 
 }  // namespace
 
+// Heads of a CTA that takes a whole sequence, 0: shares. Short contexts do without
+// the share search and the merge, with as few heads a CTA as leave all CTAs in one
+// wave. Against shares, 28 / 4 heads of 128 (contexts of the tables' width): 1 x 201
+// 6.6 us and 8.2, 64 x 201 7.7 and 13.8, 128 x 512 16.3 and 22.6, 64 x 1024 15.9 and
+// 20.9; but 1 x 1024 12.0 and 9.4, 128 x 1024 with 8 / 8 ragged 45 and 33.
+int q8_seq_heads(int batch, int num_kv_heads, int n_rep, int64_t max_ctx, int sms) {
+  for (int hg : {1, 2, 4, 8})
+    if (num_kv_heads % hg == 0 && (hg < 8 || n_rep <= 8) &&
+        static_cast<int64_t>(batch) * (num_kv_heads / hg) <= sms)
+      return max_ctx <= 512 || (max_ctx <= 1024 && batch >= 16 && hg <= 2) ? hg : 0;
+  return 0;
+}
+
 int q8_head_group(int num_kv_heads, int n_rep) {
   for (int hg : {8, 4, 2})
     if (num_kv_heads % hg == 0 && (hg < 8 || n_rep <= 8)) return hg;
@@ -977,7 +1009,7 @@ int launch_decode_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, const Decod
   const CallQ8 call{&tmk, &tmv, &a, q_bulk, stream};
   const bool bf16 = dtype == IR_DTYPE_BF16;
   const int e = bf16 ? by_code<__nv_bfloat16>(fmt, &call) : by_code<__half>(fmt, &call);
-  if (e) return e;
+  if (e || a.per_seq) return e;
   return bf16 ? launch_merge_q8<__nv_bfloat16>(a, stream) : launch_merge_q8<__half>(a, stream);
 }
 

@@ -92,7 +92,9 @@ int decode_generic_occupancy(int dtype, int D, int fmt);
 // bs % 16 == 0. One CTA (per SM) covers q8_head_group(Hkv, group) kv heads; the
 // maps view a pool as (D bytes, slots, Hkv) with boxes {D, min(bs, 16), head
 // group} and a swizzle as wide as the row. The merge of split rows is launched
-// behind.
+// behind, unless q8_seq_heads (sequences of at most max_ctx tokens) says that CTAs
+// take whole sequences.
+int q8_seq_heads(int batch, int num_kv_heads, int n_rep, int64_t max_ctx, int sms);
 int q8_head_group(int num_kv_heads, int n_rep);
 int launch_decode_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, const DecodeArgs& a,
                      int dtype, int fmt, cudaStream_t stream);

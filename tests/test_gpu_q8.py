@@ -265,13 +265,14 @@ def attend_tolerance(out, weighted, size, n, d, dtype, low_p):
     return 2 * e[:, None] * weighted + tail + half * np.abs(out) * (1 + 2.0 ** -6) + tiny
 
 
-def check_decode(w, fmt, dtype, path=None, seed=0, q=None, spread=1.0, out=None):
+def check_decode(w, fmt, dtype, path=None, seed=0, q=None, spread=1.0, out=None, width=0):
     rng = np.random.default_rng(seed)
     kc, ks = make_pool(rng, w.num_blocks, w.block_size, w.num_kv_heads, w.head_dim, fmt, spread)
     vc, vs = make_pool(rng, w.num_blocks, w.block_size, w.num_kv_heads, w.head_dim, fmt)
     if q is None:
         q = dev(rng.normal(size=(w.batch, w.num_heads, w.head_dim))).to(dtype)
-    bt, ctx = dev(w.block_tables), dev(w.context_lens)
+    cols = -(-width // w.block_size) - w.block_tables.shape[1]   # tables of `width` tokens
+    bt, ctx = dev(np.pad(w.block_tables, ((0, 0), (0, max(cols, 0))))), dev(w.context_lens)
     kp, vp = codes_to(kc, fmt), codes_to(vc, fmt)
     if path is not None:
         assert ops.decode_plan_q8(q, kp, bt, w.block_size)[0] == path
@@ -308,6 +309,45 @@ def test_decode_bf16(geom, fmt):
     check_decode(w, fmt, torch.bfloat16, path)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("geom", GEOM)
+def test_decode_wide_tables(geom, fmt):
+    """The same in equal shares of all tokens (tables wider than the contexts)."""
+    h, hkv, d, bs, path = geom
+    w = wl.custom(h + bs, 7, h, hkv, d, bs, 0, 150)
+    w.context_lens[:4] = [0, 1, 150, 17]
+    check_decode(w, fmt, torch.bfloat16, path, width=2000)
+
+
+@pytest.mark.parametrize("geom", GEOM[:14])
+def test_decode_whole_sequences(geom):
+    """A CTA per sequence: none of its results goes through the merge, so a row does
+    not depend on the others."""
+    h, hkv, d, bs, path = geom
+    w = _with_lengths(5, [500, 0, 1, 16, 17, 256, 257, 33, 129, 400], h, hkv, d, bs)
+    got = check_decode(w, "e4m3", torch.bfloat16, path)
+    rng = np.random.default_rng(0)
+    kc, ks = make_pool(rng, w.num_blocks, bs, hkv, d, "e4m3")
+    vc, vs = make_pool(rng, w.num_blocks, bs, hkv, d, "e4m3")
+    q = dev(rng.normal(size=(w.batch, h, d))).to(torch.bfloat16)
+    for i in (0, 1, 6):
+        one = irb.paged_decode_q8(q[i:i + 1], codes_to(kc, "e4m3"), codes_to(vc, "e4m3"),
+                                  dev(ks.astype(np.float32)), dev(vs.astype(np.float32)),
+                                  dev(w.block_tables[i:i + 1]), dev(w.context_lens[i:i + 1]),
+                                  w.scale, bs)
+        if 10 * hkv <= 148:   # (else ten sequences take more heads a CTA than one)
+            assert torch.equal(one[0], got[i])
+    bad = w.context_lens.copy()
+    bad[0], bad[3] = -1, w.block_tables.shape[1] * bs + 1   # read as none and as all
+    bt = w.block_tables.copy()
+    bt[5, 0] = w.num_blocks
+    irb.paged_decode_q8(q, codes_to(kc, "e4m3"), codes_to(vc, "e4m3"),
+                        dev(ks.astype(np.float32)), dev(vs.astype(np.float32)), dev(bt), dev(bad),
+                        w.scale, bs)
+    with pytest.raises(irb.DeviceError, match="CONTEXT_LEN"):
+        irb.check_device_errors()
+
+
 def _with_lengths(seed, lens, h, hkv, d, bs):
     """A workload of exactly these context lengths."""
     rng = np.random.default_rng(seed)
@@ -339,9 +379,18 @@ def test_decode_lengths(lens):
 
 @pytest.mark.parametrize("hkv", [1, 2, 4, 8])
 @pytest.mark.parametrize("rep", [1, 8, 9, 16])
-def test_decode_head_groups(hkv, rep):
+@pytest.mark.parametrize("width", [0, 2000])
+def test_decode_head_groups(hkv, rep, width):
     w = _with_lengths(hkv, [300, 1, 77, 200], hkv * rep, hkv, 128, 16)
-    check_decode(w, "int8", torch.bfloat16, 2)
+    check_decode(w, "int8", torch.bfloat16, 2, width=width)
+
+
+@pytest.mark.parametrize("batch", [30, 60, 140])
+def test_decode_whole_sequences_of_several_heads(batch):
+    """2, 4 and 8 heads a CTA: as many as leave the CTAs in one wave."""
+    rng = np.random.default_rng(batch)
+    w = _with_lengths(batch, rng.integers(0, 300, batch).tolist(), 16, 8, 64, 16)
+    check_decode(w, "e4m3", torch.bfloat16, 2)
 
 
 def test_decode_strided_and_unaligned_rows():
