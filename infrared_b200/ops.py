@@ -921,7 +921,7 @@ def cache_gather_q8(pool: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor
                                         (*slots.shape, pool.shape[1], pool.shape[2]),
                                         pool.shape, dtype_code(dtype), fmt))
     dev, fn, n, shape, (num_slots, hkv, d), code, fmt = plan
-    out = torch.empty(shape, dtype=dtype, device=pool.device)
+    out = pool.new_empty(shape, dtype=dtype)
     if n:
         slots = slots if slots.is_contiguous() else slots.contiguous()
         _issue(dev, fn, (out.data_ptr(), pool.data_ptr(), scale.data_ptr(), slots.data_ptr(), n,
