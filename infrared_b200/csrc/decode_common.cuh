@@ -226,8 +226,8 @@ __device__ __forceinline__ void tail_prefixes(const DecodeArgs& a, int64_t total
 // Find this CTA's share (its static unit under a dynamic plan). All NT
 // threads must call it. The CTA streams kv heads [kv0, kv0 + nkv). The first
 // CTA of kv head 0 publishes the tile prefix to the workspace for the merge
-// kernel; CTAs with g == 0 write the rows of sequences with no context (no
-// CTA streams them). With a.dyn, tailp / tailc (shared memory, kDynSeqs + 1
+// kernel; the rows of sequences with no context (no CTA streams them) are
+// dealt over all CTAs. With a.dyn, tailp / tailc (shared memory, kDynSeqs + 1
 // and kDynSeqs entries) receive the prefixes and context lengths of the
 // sequences the dynamic tiles lie in.
 template <int NT, typename T>
@@ -236,16 +236,19 @@ __device__ void find_share(const DecodeArgs& a, int g, int kv0, int nkv,
                            int* tailc = nullptr) {
   const int tid = threadIdx.x;
   const bool publish = (g == 0 && kv0 == 0);
-  auto empty_rows = [&](int b) {
-    // empty context: zero rows (and lse = -inf) of this CTA's heads
-    if (a.keep_empty) return;
-    for (int i = 0; i < nkv * a.n_rep * a.D; ++i) {
-      const int h = kv0 * a.n_rep + i / a.D, d = i % a.D;
-      if (a.lse_mode) {
-        a.lse_o[(static_cast<int64_t>(b) * a.H + h) * a.D + d] = 0.f;
-        if (d == 0) a.lse_out[static_cast<int64_t>(b) * a.H + h] = -INFINITY;
-      } else {
-        reinterpret_cast<T*>(a.out)[b * a.out_stride + h * a.D + d] = DT<T>::from_f(0.f);
+  // Empty contexts (lane's sequence b, if `empty`): zero rows (and lse = -inf) of
+  // this CTA's heads, a warp per row.
+  auto empty_rows = [&](int b, bool empty) {
+    for (unsigned m = __ballot_sync(0xffffffffu, empty); m != 0; m &= m - 1) {
+      const int64_t row = __shfl_sync(0xffffffffu, b, __ffs(m) - 1);
+      for (int i = tid & 31; i < nkv * a.n_rep * a.D; i += 32) {
+        const int h = kv0 * a.n_rep + i / a.D, d = i % a.D;
+        if (a.lse_mode) {
+          a.lse_o[(row * a.H + h) * a.D + d] = 0.f;
+          if (d == 0) a.lse_out[row * a.H + h] = -INFINITY;
+        } else {
+          reinterpret_cast<T*>(a.out)[row * a.out_stride + h * a.D + d] = DT<T>::from_f(0.f);
+        }
       }
     }
   };
@@ -278,8 +281,8 @@ __device__ void find_share(const DecodeArgs& a, int g, int kv0, int nkv,
         ri->b_first = b;
         ri->p_first = p;
       }
-      if (n == 0 && g == 0) empty_rows(b);
     }
+    if (!a.keep_empty) empty_rows(b, b < a.B && n == 0 && b % a.G == g);
     if (tid == 0) {
       ri->total = total;
       ri->start = start;
@@ -317,8 +320,8 @@ __device__ void find_share(const DecodeArgs& a, int g, int kv0, int nkv,
         ri->b_first = b;
         ri->p_first = p;
       }
-      if (n == 0 && g == 0) empty_rows(b);
     }
+    if (!a.keep_empty) empty_rows(b, b < a.B && n == 0 && b % a.G == g);
     running += chunk_total;
   }
   if (tid == 0) {

@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (lane == 0) ri->start = from, ri->end = to;
       __syncwarp();
-    } else if (g == 0 && !a.keep_empty) {
-      for (int sb = warp - 1; sb < a.B; sb += kConsumers) {
+    } else if (!a.keep_empty) {
+      for (int sb = (warp - 1) * a.G + g; sb < a.B; sb += kConsumers * a.G) {
         if (clamp_ctx(a.context_lens[sb], a) != 0) continue;
         T* o = reinterpret_cast<T*>(a.out) + sb * a.out_stride +
                static_cast<int64_t>(kv0) * a.n_rep * D;
