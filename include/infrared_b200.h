@@ -521,8 +521,9 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *     its whole head NaN in the rows that attend it. In frames of at most 64
  *     rows per sequence on average and long tables, sequences of up to 8 rows are
  *     decoded as in 1 beside it;
- *   1 at most 8 query rows per sequence on average (fp32: 2, or 16 up to 64
- *     rows): every row decoded as its own sequence (ir_paged_decode_q8);
+ *   1 at most 8 query rows per sequence on average (fp32: 2, or few rows in all:
+ *     320 over the kv heads and 2240 over the query heads): every row decoded as
+ *     its own sequence (ir_paged_decode_q8);
  *   4 everything else: fp32 tiles on the CUDA cores, codes read directly.
  * Rows of q that belong to no sequence leave theirs of out as they are.
  * Values of K or V at positions that a row does not attend change nothing in it,

@@ -677,7 +677,8 @@ constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy pe
 // 373, 64 x 8 209 against 379, 64 x 16 444 against 400; 1 x 8 over 4096 18 against
 // 42; 4 x 8 over 100 15 against 12. fp32, decoded against tiles: 64 single rows
 // over 300 keys 52 against 95, 64 x 4 over 50 49 against 31, but 4 x 16 over
-// 512-4096 174 against 275.
+// 512-4096 174 against 275, 3 x 41 over 900 with 6 / 2 heads 76 against 160 (too few
+// tiles for the SMs); 4 x 80 over 500 with 16 / 1 heads of 64 92 against 59.
 int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
@@ -697,16 +698,20 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   const bool tc = rows_ok && s->max_blocks > 0 && (p->dense || in_place);
   if (g_prefill_path >= 2 && !(tc && (g_prefill_path == 2 || s->head_dim == 128)))
     return fail(IR_ERR_UNSUPPORTED, "tensor-core prefill forced but shape not eligible");
-  const int64_t most = half ? kFewRows : s->total_q <= 64 ? 16 : 2;  // rows per sequence
   const int group = s->num_heads / s->num_kv_heads;
-  const bool few = group <= 16 && s->total_q <= most * s->num_seqs;
+  const int64_t S = s->num_seqs, rows = s->total_q;
+  // (fp32: also where the tiles would be too few for the SMs)
+  const bool few = group <= 16 &&
+                   (half ? rows <= kFewRows * S
+                         : rows <= 2 * S || (rows * s->num_kv_heads <= 320 &&
+                                             rows * s->num_heads <= 2240));
   p->path = g_prefill_path >= 2 ? g_prefill_path
             : few               ? 1
             : tc && g_prefill_path == 0 ? 2
                                 : 4;
   if (p->path == 2 || p->path == 3) {
-    const int64_t rows = p->dense ? dense_rows : s->num_slots;
-    p->pool = align256(static_cast<size_t>(rows) * row_bytes);
+    const int64_t held = p->dense ? dense_rows : s->num_slots;
+    p->pool = align256(static_cast<size_t>(held) * row_bytes);
     p->table_off = 2 * p->pool;
     p->bytes = p->table_off +
                (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);

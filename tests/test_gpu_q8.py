@@ -540,15 +540,16 @@ def test_decode_is_deterministic_and_replays():
 
 
 def check_prefill(h, hkv, d, bs, spans, dtype, fmt, path, q=None, out=None, width=0, spread=1.0,
-                  dirty=False):
+                  dirty=False, more=0):
     """Every row of a packed frame against 64 bits; `width`: extra table columns;
+    `more`: rows of no sequence behind the others (a frame of many rows);
     `dirty`: NaN in the workspace and in pool rows that no row attends."""
     rng = np.random.default_rng(h + d)
     f = wl.prefill_frame("t", 3, [s for s, _ in spans], [n for _, n in spans], h, hkv, d, bs)
     kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, fmt, spread)
     vc, vs = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
     if q is None:
-        q = dev(rng.normal(size=(f.total_q, h, d))).to(dtype)
+        q = dev(rng.normal(size=(f.total_q + more, h, d))).to(dtype)
     table = np.pad(f.block_tables, ((0, 0), (0, width)))
     kd, vd, ksd, vsd = kc.copy(), vc.copy(), ks.copy(), vs.copy()
     if dirty:
@@ -599,8 +600,13 @@ def check_prefill(h, hkv, d, bs, spans, dtype, fmt, path, q=None, out=None, widt
     (40, 2, 64, 16, [(0, 9), (70, 20)]),   # a group of 20
 ])
 def test_prefill(h, hkv, d, bs, spans, dtype, fmt):
-    path = 4 if dtype == torch.float32 else 2
-    check_prefill(h, hkv, d, bs, spans, dtype, fmt, path)
+    if dtype != torch.float32:
+        check_prefill(h, hkv, d, bs, spans, dtype, fmt, 2)
+        return
+    rows = sum(n for _, n in spans)
+    few = rows * max(7 * hkv, h) <= 2240 and h // hkv <= 16
+    check_prefill(h, hkv, d, bs, spans, dtype, fmt, 1 if few else 4)
+    check_prefill(h, hkv, d, bs, spans, dtype, fmt, 4, more=2300)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -610,8 +616,9 @@ def test_prefill_layouts(bs, width, dtype):
     nothing read that no row attends."""
     check_prefill(8, 2, 64, bs, [(0, 70), (33, 2), (0, 1), (260, 140)], dtype, "e4m3",
                   2 if dtype == torch.bfloat16 else 4, width=width, dirty=True)
+    more = 2300 if dtype == torch.float32 else 0
     check_prefill(8, 2, 64, bs, [(0, 70), (33, 20)], dtype, "int8",
-                  2 if dtype == torch.bfloat16 else 4, width=width)
+                  2 if dtype == torch.bfloat16 else 4, width=width, more=more)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -627,7 +634,8 @@ def test_prefill_few_rows_and_forced_paths(dtype):
     ops.set_prefill_path(1)
     try:
         check_prefill(28, 4, 128, 16, spans, dtype, "e4m3", 1)
-        check_prefill(28, 4, 128, 16, [(3, 70), (10, 9)], dtype, "int8", 4, spread=4.0)
+        check_prefill(28, 4, 128, 16, [(3, 70), (10, 9)], dtype, "int8", 4, spread=4.0,
+                      more=2300)
     finally:
         ops.set_prefill_path(0)
 
