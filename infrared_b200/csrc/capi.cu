@@ -1123,12 +1123,13 @@ size_t ir_paged_prefill_workspace_size(const ir_prefill_shape* shape) {
   return total;
 }
 
-// (sequences of at most short_rows rows are left out; 0: none)
+// (sequences of at most short_rows rows are left out, 0: none; contexts beyond
+// max_ctx are refused, -1: beyond the table of `s`)
 static int prefill_impl(void* out, const void* q, const void* k_pool, const void* v_pool,
                         const int32_t* block_tables, const int32_t* context_lens,
                         const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
                         size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream,
-                        int short_rows) {
+                        int short_rows, int max_ctx) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
   if (s->num_seqs == 0 || s->total_q == 0) return IR_OK;
@@ -1168,6 +1169,7 @@ static int prefill_impl(void* out, const void* q, const void* k_pool, const void
     a.scale_log2 = s->scale * irb::kLog2e;
     a.err = err_flag;
     a.short_rows = short_rows;
+    a.max_ctx = max_ctx >= 0 ? max_ctx : s->max_blocks * s->block_size;
     CUtensorMap tmq, tmk, tmv;
     const int rows = s->block_size < 128 ? s->block_size : 128;
     // a CTA of a pair stages 64 keys of each K tile
@@ -1209,7 +1211,7 @@ int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v
                      const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
                      size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream) {
   return prefill_impl(out, q, k_pool, v_pool, block_tables, context_lens, q_start, s, workspace,
-                      workspace_bytes, err_flag, stream, 0);
+                      workspace_bytes, err_flag, stream, 0, -1);
 }
 
 // ---------------------------------------------------------------- 8-bit cache
@@ -1382,6 +1384,7 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
   a.num_blocks = s->num_slots / s->block_size;
   a.scale_log2 = s->scale * irb::kLog2e;
   a.err = err_flag;
+  a.max_ctx = s->max_blocks * s->block_size;
   if (p.path == 4) {
     e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, st);
     return cuda_status(e, "8-bit prefill launch");
@@ -1403,7 +1406,7 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     x.num_slots = p.cap * s->num_seqs;
   }
   return prefill_impl(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
-                      q_start, &x, nullptr, 0, err_flag, stream, few);
+                      q_start, &x, nullptr, 0, err_flag, stream, few, a.max_ctx);
 }
 
 // ---------------------------------------------------------------- q/k norm + rotation

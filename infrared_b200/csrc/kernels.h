@@ -26,6 +26,7 @@ struct PrefillArgs {
   float scale_log2;
   int32_t* err;
   int short_rows;  // sequences of at most this many rows are left out (0: none)
+  int max_ctx;     // longest context the caller's block table holds
 };
 
 // tcgen05 kernel: 16-bit dtypes, D in {64, 128}, block size a power of two

@@ -89,8 +89,7 @@ __global__ void __launch_bounds__(kT, 2)
   const int tile = s_tiles - 1 - s_tile;
   const int q0 = a.q_start[sq];
   const int q_len = a.q_start[sq + 1] - q0, ctx = a.context_lens[sq];
-  if (ctx < q_len || ctx > static_cast<int64_t>(a.max_blocks) * a.bs ||
-      q0 + static_cast<int64_t>(q_len) > a.total_q) {
+  if (ctx < q_len || ctx > a.max_ctx || q0 + static_cast<int64_t>(q_len) > a.total_q) {
     if (tid == 0) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
     return;
   }

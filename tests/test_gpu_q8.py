@@ -1039,3 +1039,40 @@ def test_a_long_table_passes_32_bits_of_bytes():
     want, weighted, size = q8.attend(host(q[0]), host(kf), host(vf), d ** -0.5)
     assert (np.abs(host(out[0]) - want) <=
             attend_tolerance(want, weighted, size, n, d, torch.bfloat16, True)).all()
+
+
+# ---------------------------------------------------------------- contexts past the table
+
+
+@pytest.mark.parametrize("over", [1, 63, 64])
+@pytest.mark.parametrize("dtype,d,force", [
+    (torch.bfloat16, 64, 0), (torch.float16, 64, 0), (torch.float32, 64, 0),
+    (torch.bfloat16, 128, 2), (torch.bfloat16, 128, 3), (torch.bfloat16, 64, 1)])
+def test_prefill_context_past_the_table_leaves_its_rows_alone(dtype, d, force, over):
+    """A context that the table does not hold is flagged and its rows stay as they
+    were, on every path: nothing that the call's workspace held before comes out."""
+    rng = np.random.default_rng(2)
+    f = wl.prefill_frame("t", 3, [10, 0], [40, 30], 8, 2, d, 16)
+    kc, ks = make_pool(rng, f.num_blocks, 16, 2, d, "e4m3")
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    q = dev(rng.normal(size=(70, 8, d))).to(dtype)
+    bt, qs = dev(f.block_tables), dev(f.q_start)
+    held = 16 * f.block_tables.shape[1]
+    ops.set_prefill_path(force)
+    try:
+        _, nbytes = ops.prefill_plan_q8(q, pool, bt, qs, 16)
+        for first in (held + over, held):
+            ws = torch.full((max(nbytes, 256),), 0xff, dtype=torch.uint8, device=DEV)
+            out = torch.full_like(q, 7.0)
+            irb.paged_prefill_q8(q, pool, pool, sc, sc, bt, dev(np.array([first, 30], np.int32)),
+                                 qs, f.scale, 16, out=out, ws=ws)
+            if first > held:
+                with pytest.raises(irb.DeviceError, match="CONTEXT_LEN"):
+                    irb.check_device_errors()
+                assert (out[:40] == 7.0).all()
+                rest = out[40:].clone()
+    finally:
+        ops.set_prefill_path(0)
+    assert not (out[:40] == 7.0).all() and torch.isfinite(out).all()
+    if force != 1:   # (rows decoded one by one are cut by the lengths of all)
+        assert torch.equal(out[40:], rest)
