@@ -515,8 +515,11 @@ int ir_paged_decode_q8(void* out, const void* q, const void* k_pool, const void*
  *   2 (3: its CTA-pair form) 16-bit q with 16-byte aligned rows: the blocks of
  *     the sequences' histories are expanded once into rows of shape->dtype in
  *     the workspace, which the tensor-core kernel attends over: a block's
- *     conversion is paid once, not once per 128 query rows and head. Exact in
- *     bf16 for power-of-two scales. The workspace holds the histories (or one
+ *     conversion is paid once, not once per 128 query rows and head. Exact for
+ *     power-of-two scales; others round each value to shape->dtype. (In fp16 a
+ *     K or V beyond its range, and a K that is no multiple of its smallest value,
+ *     sends the rows that attend it to the tiles of 4; a V below its normal
+ *     range is off by up to 2^-25.) The workspace holds the histories (or one
  *     layer's pool) in shape->dtype and can serve every layer. A NaN in V makes
  *     its whole head NaN in the rows that attend it. In frames of at most 64
  *     rows per sequence on average and long tables, sequences of up to 8 rows are

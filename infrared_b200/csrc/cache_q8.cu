@@ -352,10 +352,11 @@ struct Q8Links {
 
 // (a kernel rather than a memset, so that the three grids can overlap their
 // starts: 32768 rows 29.2 us from 29.9)
-__global__ void zero_kernel(int* p, int n) {
+__global__ void fill_kernel(int* p, int n, int value) {
   let_next_grid_start();
   wait_prior_grid();
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x)
+    p[i] = value;
 }
 
 __global__ void __launch_bounds__(kQThreads)
@@ -749,6 +750,24 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Whether one of 8 values code * s is lost as a row of fp16: beyond its range
+// (where it would saturate), or, with `fine`, below its normal range and not a
+// multiple of its smallest value. NaN is not: it stays NaN.
+template <typename C>
+__device__ __forceinline__ bool lost_in_half(uint2 codes, float s, bool fine) {
+  bool lost = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 f = decode4<C>(i == 0 ? codes.x : codes.y);
+    const float v[4] = {f.x * s, f.y * s, f.z * s, f.w * s};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      lost = lost || fabsf(v[e]) > 65504.f ||
+             (fine && fabsf(v[e]) < 1.f && __half2float(__float2half_rn(v[e])) != v[e]);
+  }
+  return lost && finite(s);
+}
+
 // The blocks of the sequences' histories as rows of T: with `table` null, each
 // in its own place of a pool laid out as the codes are; else sequence by
 // sequence (cap rows each), with the block table of that order. The tensor
@@ -756,13 +775,29 @@ __global__ void __launch_bounds__(256)
 // that is not finite would reach rows that do not attend it. So it becomes 0,
 // and its head's K NaN instead: the score of a row that attends it is NaN, and
 // a masked score is never used.
+//
+// fp16 has fewer exponents than code * scale (bf16 has as many as fp32). Of the
+// values that it cannot hold, a small V is off by at most 2^-25, half of the
+// output's own smallest step; but a K or V beyond 65504 would saturate, and the
+// error of a small K is multiplied by q, whatever its size. exact_from (fp16
+// only) receives each sequence's first position with such a value, and behind
+// the S sequences the smallest of all: rows from there on are left to the fp32
+// kernel, which reads the codes. Powers of two in [2^-15, 2^7] (e4m3; int8
+// [2^-24, 2^9]) have none, so the codes are looked at only under other scales. (A
+// scale that is no power of two rounds a value to half a unit of T, as writing it
+// to a 16-bit pool would.)
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)
     expand_blocks_kernel(T* kout, T* vout, const uint8_t* kp, const uint8_t* vp, const float* ks,
                          const float* vs, const int32_t* bt, int64_t bt_stride, const int32_t* ctx,
                          const int32_t* q_start, int short_rows, int max_blocks,
                          int64_t num_blocks, int Hkv, int D, int bs, int32_t* table, int64_t cap,
-                         int table_block, int32_t* err) {
+                         int table_block, int32_t* exact_from, int32_t* err) {
+  constexpr bool kHalfRows = std::is_same<T, __half>::value;
+  constexpr bool kInt = std::is_same<C, int8_t>::value;
+  constexpr float kFinest = kInt ? 0x1p-24f : 0x1p-15f;
+  constexpr float kWidest = 65504.f / (kInt ? 127.f : 448.f);
+  int first = INT32_MAX;  // first position that fp16 rows cannot hold
   wait_prior_grid();
   const int sq = blockIdx.x;
   // (sequences of few rows are attended from the codes)
@@ -784,12 +819,17 @@ __global__ void __launch_bounds__(256)
     const int64_t to = table ? sq * cap + static_cast<int64_t>(j) * bs : id * bs;
     for (int c = threadIdx.x % tpr; c < pieces; c += tpr) {
       const float k = ok ? ks[id * Hkv + c * 8 / D] : 0.f, v = ok ? vs[id * Hkv + c * 8 / D] : 0.f;
+      const bool fine = fabsf(k) < kFinest;
+      const bool look = kHalfRows && (fine || fabsf(k) > kWidest || fabsf(v) > kWidest);
 #pragma unroll 4
       for (int r = threadIdx.x / tpr; r < bs; r += side) {
         const int64_t at = (id * bs + r) * pieces + c, dst = (to + r) * pieces + c;
         uint2 kc = reinterpret_cast<const uint2*>(kp)[at];
         uint2 vc = reinterpret_cast<const uint2*>(vp)[at];
         if (!ok) kc = vc = make_uint2(0u, 0u);
+        if (kHalfRows && look && j * bs + r < c0 &&
+            (lost_in_half<C>(kc, k, fine) || lost_in_half<C>(vc, v, false)))
+          first = min(first, j * bs + r);
         float kr = k, vr = v;
         if (!finite(v) || (std::is_same<C, e4m3_t>::value && (has_nan(vc.x) || has_nan(vc.y)))) {
           kr = __uint_as_float(0x7fc00000u);
@@ -804,6 +844,10 @@ __global__ void __launch_bounds__(256)
   if (table != nullptr && blockIdx.y == 0)
     for (int i = threadIdx.x; i < cap / table_block; i += blockDim.x)
       table[sq * (cap / table_block) + i] = static_cast<int32_t>(sq * (cap / table_block) + i);
+  if (kHalfRows && first != INT32_MAX) {
+    atomicMin(&exact_from[sq], first);
+    atomicMin(&exact_from[gridDim.x], first);
+  }
 }
 
 template <typename F>
@@ -875,8 +919,8 @@ int launch_cache_write_q8(const void* k, const void* v, int64_t k_stride, int64_
   l.next = reinterpret_cast<int*>(w + heads);
   l.owners = reinterpret_cast<int*>(w + heads + align256(static_cast<size_t>(n) * 4));
   const int words = static_cast<int>(num_blocks + 2);
-  int rc = launch_behind(zero_kernel, dim3(words < 65536 ? (words + 255) / 256 : 256), 256, 0,
-                         stream, l.count, words);
+  int rc = launch_behind(fill_kernel, dim3(words < 65536 ? (words + 255) / 256 : 256), 256, 0,
+                         stream, l.count, words, 0);
   if (rc) return rc;
   rc = launch_behind(link_runs_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0,
                          stream, slots, n, num_slots, bs, l, err);
@@ -940,8 +984,14 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
                          int64_t bt_stride, const int32_t* ctx, const int32_t* q_start,
                          int short_rows, int S, int max_blocks, int64_t num_blocks, int Hkv,
                          int D, int bs, int dtype, int fmt, int32_t* table, int64_t cap,
-                         int table_block, int32_t* err, cudaStream_t stream) {
+                         int table_block, int32_t* exact_from, int32_t* err,
+                         cudaStream_t stream) {
   if (S == 0 || max_blocks == 0) return 0;
+  if (exact_from) {
+    const int rc = launch_behind(fill_kernel, dim3(S < 65536 ? S / 256 + 1 : 256), 256, 0, stream,
+                                 exact_from, S + 1, INT32_MAX);
+    if (rc) return rc;
+  }
   const dim3 grid(static_cast<unsigned>(S),
                   static_cast<unsigned>(max_blocks < 4096 ? max_blocks : 4096));
   return by_type(dtype, [&](auto t) {
@@ -952,7 +1002,7 @@ int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const voi
                            static_cast<T*>(v_out), static_cast<const uint8_t*>(k_pool),
                            static_cast<const uint8_t*>(v_pool), k_scale, v_scale, bt, bt_stride,
                            ctx, q_start, short_rows, max_blocks, num_blocks, Hkv, D, bs, table,
-                           cap, table_block, err);
+                           cap, table_block, exact_from, err);
     });
   });
 }

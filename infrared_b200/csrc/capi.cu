@@ -658,8 +658,9 @@ struct PrefillQ8Plan {
   bool dense;      // the expansion lays the histories out sequence by sequence
   bool split;      // sequences of up to kFewRows rows are decoded row by row beside it
   int64_t cap;     // rows of a sequence there
-  // workspace: K, V, table; the decoded rows' tables, contexts and scratch
-  size_t pool, table_off, rows_off, rows_table, rows_ctx, bytes;
+  // workspace: K, V, table, exact_from (fp16); the decoded rows' tables, contexts
+  // and scratch
+  size_t pool, table_off, exact_off, rows_off, rows_table, rows_ctx, bytes;
 };
 
 constexpr int kFewRows = 8;
@@ -713,8 +714,10 @@ int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
     const int64_t held = p->dense ? dense_rows : s->num_slots;
     p->pool = align256(static_cast<size_t>(held) * row_bytes);
     p->table_off = 2 * p->pool;
-    p->bytes = p->table_off +
-               (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
+    p->exact_off = p->table_off +
+                   (p->dense ? align256(static_cast<size_t>(dense_rows / kDenseBlock) * 4) : 0);
+    p->bytes = p->exact_off;
+    if (s->dtype == IR_DTYPE_F16) p->bytes += align256((static_cast<size_t>(S) + 1) * 4);
     // A step of many decode rows and a prompt or two: expanding the histories of
     // the former would cost 2.5 ns a row, most of the call (64 single rows over
     // 512-4096 keys beside 512 rows: 384 us, decoded beside 71; 32 over 100-500
@@ -1124,12 +1127,12 @@ size_t ir_paged_prefill_workspace_size(const ir_prefill_shape* shape) {
 }
 
 // (sequences of at most short_rows rows are left out, 0: none; contexts beyond
-// max_ctx are refused, -1: beyond the table of `s`)
+// max_ctx are refused, -1: beyond the table of `s`; exact_from as in PrefillArgs)
 static int prefill_impl(void* out, const void* q, const void* k_pool, const void* v_pool,
                         const int32_t* block_tables, const int32_t* context_lens,
                         const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
                         size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream,
-                        int short_rows, int max_ctx) {
+                        int short_rows, int max_ctx, const int32_t* exact_from) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;
   if (s->num_seqs == 0 || s->total_q == 0) return IR_OK;
@@ -1170,6 +1173,7 @@ static int prefill_impl(void* out, const void* q, const void* k_pool, const void
     a.err = err_flag;
     a.short_rows = short_rows;
     a.max_ctx = max_ctx >= 0 ? max_ctx : s->max_blocks * s->block_size;
+    a.exact_from = exact_from;
     CUtensorMap tmq, tmk, tmv;
     const int rows = s->block_size < 128 ? s->block_size : 128;
     // a CTA of a pair stages 64 keys of each K tile
@@ -1211,7 +1215,7 @@ int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v
                      const int32_t* q_start, const ir_prefill_shape* s, void* workspace,
                      size_t workspace_bytes, int32_t* err_flag, ir_stream_t stream) {
   return prefill_impl(out, q, k_pool, v_pool, block_tables, context_lens, q_start, s, workspace,
-                      workspace_bytes, err_flag, stream, 0, -1);
+                      workspace_bytes, err_flag, stream, 0, -1, nullptr);
 }
 
 // ---------------------------------------------------------------- 8-bit cache
@@ -1392,12 +1396,19 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
   const int few = p.split ? kFewRows : 0;
   if (few && (rc = decode_rows(few)) != IR_OK) return rc;
   int32_t* table = p.dense ? reinterpret_cast<int32_t*>(ws + p.table_off) : nullptr;
+  int32_t* exact_from =
+      s->dtype == IR_DTYPE_F16 ? reinterpret_cast<int32_t*>(ws + p.exact_off) : nullptr;
   e = irb::launch_expand_blocks(ws, ws + p.pool, k_pool, v_pool, k_scale, v_scale, block_tables,
                                 s->bt_stride, context_lens, q_start, few, s->num_seqs,
                                 s->max_blocks, a.num_blocks, s->num_kv_heads, s->head_dim,
                                 s->block_size, s->dtype, kv_format, table, p.cap, kDenseBlock,
-                                err_flag, st);
+                                exact_from, err_flag, st);
   if (e) return cuda_status(e, "8-bit block expansion launch");
+  if (exact_from) {
+    a.exact_from = exact_from;
+    e = irb::launch_prefill_q8(a, k_pool, v_pool, k_scale, v_scale, s->dtype, kv_format, st);
+    if (e) return cuda_status(e, "8-bit prefill launch");
+  }
   ir_prefill_shape x = *s;
   if (p.dense) {
     x.block_size = kDenseBlock;
@@ -1406,7 +1417,7 @@ int ir_paged_prefill_q8(void* out, const void* q, const void* k_pool, const void
     x.num_slots = p.cap * s->num_seqs;
   }
   return prefill_impl(out, q, ws, ws + p.pool, p.dense ? table : block_tables, context_lens,
-                      q_start, &x, nullptr, 0, err_flag, stream, few, a.max_ctx);
+                      q_start, &x, nullptr, 0, err_flag, stream, few, a.max_ctx, exact_from);
 }
 
 // ---------------------------------------------------------------- q/k norm + rotation

@@ -27,6 +27,9 @@ struct PrefillArgs {
   int32_t* err;
   int short_rows;  // sequences of at most this many rows are left out (0: none)
   int max_ctx;     // longest context the caller's block table holds
+  // null, or per sequence the first position whose row is computed in fp32 from
+  // the codes (INT32_MAX: none), and behind them the smallest of all
+  const int32_t* exact_from;
 };
 
 // tcgen05 kernel: 16-bit dtypes, D in {64, 128}, block size a power of two
@@ -113,16 +116,18 @@ int launch_cache_gather_q8(void* out, const void* pool, const float* scale, cons
 // Every block that a sequence's history covers, as rows of dtype: at the same
 // place of the output pools (table null), or sequence by sequence, cap rows
 // each, with the block table [S, cap / table_block] of that order. Where a V is
-// not finite it becomes 0 and its K NaN.
+// not finite it becomes 0 and its K NaN. exact_from [S + 1] (fp16): see
+// PrefillArgs.
 int launch_expand_blocks(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
                          const float* k_scale, const float* v_scale, const int32_t* bt,
                          int64_t bt_stride, const int32_t* ctx, const int32_t* q_start,
                          int short_rows, int S, int max_blocks, int64_t num_blocks, int Hkv,
                          int D, int bs, int dtype, int fmt, int32_t* table, int64_t cap,
-                         int table_block, int32_t* err, cudaStream_t stream);
+                         int table_block, int32_t* exact_from, int32_t* err,
+                         cudaStream_t stream);
 
 // prefill_q8.cu: packed rows over an 8-bit pool in fp32 on the CUDA cores
-// (args as in PrefillArgs)
+// (args as in PrefillArgs; with exact_from only the rows from there on)
 int launch_prefill_q8(const PrefillArgs& a, const void* k_pool, const void* v_pool,
                       const float* k_scale, const float* v_scale, int dtype, int fmt,
                       cudaStream_t s);

@@ -1,6 +1,7 @@
 // Causal attention of packed query rows over an 8-bit pool in fp32 on the CUDA
-// cores: for q of 32 bits, and for 16-bit calls that the tensor-core path
-// cannot take (rows that are not 16-byte aligned, or asked for).
+// cores: for q of 32 bits, for 16-bit calls that the tensor-core path cannot
+// take (rows that are not 16-byte aligned, or asked for), and beside it for
+// fp16 rows that attend values beyond fp16 (PrefillArgs::exact_from).
 //
 // A CTA takes 64 rows of one kv head, a row being a (query token, head of the
 // group) pair, and walks the sequence's keys 64 at a time: the codes of a tile
@@ -77,6 +78,7 @@ __global__ void __launch_bounds__(kT, 2)
   __shared__ int s_seq, s_tile, s_tiles, s_nan;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int kvh = blockIdx.y;
+  if (a.exact_from != nullptr && a.exact_from[a.S] == INT32_MAX) return;  // mostly
   if (tid < 32) {
     int seq = -1, tile = 0, tiles = 0;
     if (!find_tile(a.q_start, a.S, a.total_q, a.n_rep, blockIdx.x, &seq, &tile, &tiles)) seq = -1;
@@ -95,15 +97,18 @@ __global__ void __launch_bounds__(kT, 2)
   }
   const int64_t m0 = static_cast<int64_t>(tile) * kM;
   const int64_t rows = static_cast<int64_t>(q_len) * a.n_rep;
+  const int from = a.exact_from != nullptr ? a.exact_from[sq] : 0;  // first position to compute
+  const int64_t last = (m0 + kM < rows ? m0 + kM : rows) - 1;
+  const int keys = ctx - q_len + static_cast<int>(last / a.n_rep) + 1;  // the tile's last row's
+  if (keys <= from) return;
   // this thread's rows: their position (-1: no row), and in the group
   int pos[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + ty * 4 + i;
     pos[i] = m < rows ? ctx - q_len + static_cast<int>(m / a.n_rep) : -1;
+    if (pos[i] < from) pos[i] = -1;
   }
-  const int64_t last = (m0 + kM < rows ? m0 + kM : rows) - 1;
-  const int keys = ctx - q_len + static_cast<int>(last / a.n_rep) + 1;  // the tile's last row's
 
   // q rows, scaled so that scores come in log2 units
   for (int i = tid; i < kM * D; i += kT) {

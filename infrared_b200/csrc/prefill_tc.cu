@@ -133,7 +133,8 @@ __device__ __forceinline__ void locate_tile(const PrefillArgs& a, int t, int lan
 // One work item: TR (128, or 256 for a CTA pair) query rows of one sequence
 // for one query head.
 struct Item {
-  int s;      // sequence; -1: past the last item; -2: invalid metadata (skipped)
+  int s;      // sequence; -1: past the last item; -2: invalid metadata, -3: no row
+              // of it is this kernel's (both skipped)
   int h, kvh;
   int r0;     // first packed query row
   int nrows;  // rows of the tile inside the sequence
@@ -164,6 +165,13 @@ __device__ __forceinline__ Item item_of(const PrefillArgs& a, int it, int lane) 
   x.r0 = qs + qt * TR;
   x.nrows = min(TR, ql - qt * TR);
   x.pos0 = ctx - ql + qt * TR;
+  if (a.exact_from != nullptr) {  // the fp32 kernel's rows
+    x.nrows = min(x.nrows, a.exact_from[sq] - x.pos0);
+    if (x.nrows <= 0) {
+      x.s = -3;
+      return x;
+    }
+  }
   x.n_kv = (x.pos0 + x.nrows - 1) / kKeys + 1;
   x.ctx = ctx;
   return x;
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item x = item_of<TR>(a, it, lane);
       if (x.s == -1) break;
       if (x.s < 0) {
-        if (threadIdx.x == 0) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
+        if (threadIdx.x == 0 && x.s == -2) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
         continue;
       }
       const int pos = x.pos0 + rbase + r;

@@ -1076,3 +1076,76 @@ def test_prefill_context_past_the_table_leaves_its_rows_alone(dtype, d, force, o
     assert not (out[:40] == 7.0).all() and torch.isfinite(out).all()
     if force != 1:   # (rows decoded one by one are cut by the lengths of all)
         assert torch.equal(out[40:], rest)
+
+
+# ---------------------------------------------------------------- fp16 rows, values beyond fp16
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("side", ["large k", "large v", "small k", "both"])
+@pytest.mark.parametrize("d,bs,width,force", [(64, 16, 0, 0), (128, 16, 4000, 0), (64, 12, 0, 0),
+                                              (128, 16, 0, 3)])
+def test_prefill_fp16_over_values_beyond_its_range(d, bs, width, force, side, fmt):
+    """A pool written from wider rows holds values that fp16 does not: the rows that
+    attend one are held to the fp32 kernel's bound (no rounding of weights or of
+    the history), those before keep their bits, as do other sequences; codes past
+    the context decide nothing."""
+    rng = np.random.default_rng(6)
+    h, hkv, n, head = 8, 2, 150, 31
+    f = wl.prefill_frame("t", 3, [head, 0, 5], [n, 20, 70], h, hkv, d, bs)
+    kc, ks0 = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    vc, vs0 = make_pool(rng, f.num_blocks, bs, hkv, d, fmt)
+    table = f.block_tables[0, :-(-(head + n) // bs)]
+    # the last block: small codes and then, past the context, one that fp16 cannot hold
+    past = (head + n) % bs
+    at = table[-1] * bs
+    vc[at:at + bs] = np.sign(vc[at:at + bs])
+    vs0[table[-1]] = 2.0 ** (8 if fmt == "e4m3" else 10)
+    vx = vc.copy()
+    vx[at + past:at + bs] = 448 if fmt == "e4m3" else 127
+    ks, vs, scale, qsize = ks0.copy(), vs0.copy(), f.scale, 1.0
+    blk = table[70 // bs]
+    if side in ("large v", "both"):        # up to 114688 or 130048
+        vs[blk] = 2.0 ** (8 if fmt == "e4m3" else 10)
+    if side in ("large k", "both"):
+        ks[blk, 1] = 2.0 ** (10 if fmt == "e4m3" else 12)
+        qsize = 2.0 ** -16
+    if side == "small k":                  # scores of usual size from large q and scale
+        ks[table] *= 2.0 ** -22 if fmt == "e4m3" else 2.0 ** -24
+        scale, qsize = scale * 2.0 ** 12, 2.0 ** 10
+    q = dev(rng.normal(size=(f.total_q, h, d)) * qsize).to(torch.float16)
+    bt = dev(np.pad(f.block_tables, ((0, 0), (0, width))))
+
+    def run(ks, vs, vc=vc):
+        return irb.paged_prefill_q8(q, codes_to(kc, fmt), codes_to(vc, fmt),
+                                    dev(ks.astype(np.float32)), dev(vs.astype(np.float32)), bt,
+                                    dev(f.context_lens), dev(f.q_start), scale, bs)
+
+    ops.set_prefill_path(force)
+    try:
+        assert ops.prefill_plan_q8(q, codes_to(kc, fmt), bt, dev(f.q_start), bs)[0] == (force or 2)
+        got, clean = run(ks, vs), run(ks0, vs0)
+        assert torch.equal(run(ks0, vs0, vx), clean)
+    finally:
+        ops.set_prefill_path(0)
+    kh = q8.history(q8.values(kc, ks, bs), f.block_tables[0], head + n, bs)
+    vh = q8.history(q8.values(vc, vs, bs), f.block_tables[0], head + n, bs)
+    lost = (np.abs(kh) > 65504) | (np.abs(vh) > 65504) | \
+        ((np.abs(kh) < 2.0 ** -14) & (np.clip(kh, -1, 1).astype(np.float16) != kh))
+    start = int(np.nonzero(lost.any(axis=(1, 2)))[0][0])
+    assert side == "small k" or 70 // bs * bs <= start < (70 // bs + 1) * bs
+    before = max(start - head, 0)          # rows of the first sequence that attend none of them
+    same = 0 if side == "small k" else 70 // bs * bs - head   # nor another row of their block
+    assert torch.equal(got[:same], clean[:same]) and torch.equal(got[n:], clean[n:])
+    g, qh = host(got), host(q)
+    for r in (*range(same, before), *range(before, n, 3)):
+        t = head + r + 1
+        want, weighted, size = q8.attend(qh[r], kh[:t], vh[:t], scale)
+        tol = attend_tolerance(want, weighted, size, t, d, torch.float16, False)
+        if r < before:                     # the tensor cores' rows, as in check_prefill
+            tol = tol + 2.0 ** -10 * weighted + t * 2.0 ** -25 * np.abs(vh[:t]).max() + 2.0 ** -24
+        # (an output that rounds beyond fp16 is infinite: 65520 is half way to 2^16)
+        over = np.abs(want) - tol > 65520
+        assert (g[r][over] == np.sign(want[over]) * np.inf).all()
+        sure = np.abs(want) + tol < 65520
+        assert (np.abs(g[r] - want)[sure] <= tol[sure]).all(), r
