@@ -792,13 +792,18 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 _err_ptrs: dict[int, int] = {}   # device -> address of its error word (allocated once)
 
 
+def _on_device(dev: int, fn, *args):
+    """A library call with device ``dev`` current: plans and workspace sizes
+    depend on it, and launches need it."""
+    if dev == _current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _issue(dev: int, fn, args) -> None:
     """One library call on device ``dev``; ``args`` end with its stream."""
-    if dev == _current_device():
-        rc = fn(*args)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args)
+    rc = _on_device(dev, fn, *args)
     if rc:
         check(rc)
 
@@ -974,14 +979,21 @@ def _scratch(ws: torch.Tensor | None, nbytes: int, q: torch.Tensor) -> torch.Ten
     return ws
 
 
+def _plan_device(q: torch.Tensor) -> int:
+    """Device whose plan is meant: q's, or the current one (q's shape may be all
+    there is)."""
+    return _dev_index(q) if q.is_cuda else _current_device()
+
+
 def decode_plan_q8(q, k_pool, block_tables, block_size, scale=1.0):
     """``(path, ctas_per_kv_head, workspace_bytes)`` of :func:`paged_decode_q8`."""
     s = _shape(q, k_pool, block_tables, block_size, scale, q.shape[1] * q.shape[2])
     fmt = kv_format(k_pool.dtype)
     lib = _lib.load()
+    dev = _plan_device(q)
     path, g = _lib.c_int(), _lib.c_int()
-    check(lib.ir_paged_decode_q8_plan(s, fmt, path, g))
-    return path.value, g.value, lib.ir_paged_decode_q8_workspace_size(s, fmt)
+    check(_on_device(dev, lib.ir_paged_decode_q8_plan, s, fmt, path, g))
+    return path.value, g.value, _on_device(dev, lib.ir_paged_decode_q8_workspace_size, s, fmt)
 
 
 def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1005,10 +1017,9 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                    row if out is None else _row_stride(out, row))
         s.q_stride, s.bt_stride = _row_stride(q, row), _row_stride(block_tables, s.max_blocks)
         lib = _lib.load()
-        with torch.cuda.device(dev):
-            nbytes = lib.ir_paged_decode_q8_workspace_size(s, fmt)
-            if nbytes == 0:
-                check(lib.ir_paged_decode_q8_plan(s, fmt, None, None))
+        nbytes = _on_device(dev, lib.ir_paged_decode_q8_workspace_size, s, fmt)
+        if nbytes == 0:
+            check(_on_device(dev, lib.ir_paged_decode_q8_plan, s, fmt, None, None))
         plan = _decode_q8_plans.keep(key, (dev, lib.ir_paged_decode_q8, s, fmt, nbytes))
     dev, fn, s, fmt, nbytes = plan
     if out is None:
@@ -1027,9 +1038,10 @@ def prefill_plan_q8(q, k_pool, block_tables, q_start, block_size, scale=1.0):
                        q.shape[1] * q.shape[2])
     fmt = kv_format(k_pool.dtype)
     lib = _lib.load()
+    dev = _plan_device(q)
     path = _lib.c_int()
-    check(lib.ir_paged_prefill_q8_plan(s, fmt, path))
-    return path.value, lib.ir_paged_prefill_q8_workspace_size(s, fmt)
+    check(_on_device(dev, lib.ir_paged_prefill_q8_plan, s, fmt, path))
+    return path.value, _on_device(dev, lib.ir_paged_prefill_q8_workspace_size, s, fmt)
 
 
 def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1062,10 +1074,9 @@ def paged_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     # (asked each time: it depends on the path chosen by set_prefill_path)
-    nbytes = lib.ir_paged_prefill_q8_workspace_size(s, fmt)
+    nbytes = _on_device(dev, lib.ir_paged_prefill_q8_workspace_size, s, fmt)
     if nbytes == 0:
-        with torch.cuda.device(dev):
-            check(lib.ir_paged_prefill_q8_plan(s, fmt, None))
+        check(_on_device(dev, lib.ir_paged_prefill_q8_plan, s, fmt, None))
     ws = _scratch(ws, max(nbytes, 256), q)
     _issue(dev, lib.ir_paged_prefill_q8,
            (out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),

@@ -143,3 +143,57 @@ def test_cpu_tensors_are_refused():
         irb.qk_norm_rope(k, k, None, None, k[:, 0], k[:, 0], 1e-6)
     with pytest.raises(irb.UnsupportedShape):
         ops.kv_format(torch.uint8)
+
+
+class _FakeLib:
+    """Entry points that record which device was current when they were called."""
+
+    def __init__(self, now):
+        self.now, self.seen = now, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.seen.append((name, self.now[-1]))
+            return 4096 if name.endswith("_workspace_size") else 0
+        return call
+
+
+def test_sizes_are_asked_of_the_tensors_device(monkeypatch):
+    """A call on device 1 while device 0 is current: plans, workspace sizes and
+    launches all see device 1 (sizes follow the device's SM count)."""
+    now = [0]
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            now.append(self.dev)
+
+        def __exit__(self, *exc):
+            now.pop()
+
+    lib = _FakeLib(now)
+    monkeypatch.setattr(ops, "_dev_index", lambda t: 1)
+    monkeypatch.setattr(ops, "_plan_device", lambda t: 1)
+    monkeypatch.setattr(ops, "_current_device", lambda: now[-1])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_err_ptr", lambda dev: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
+    for plans in ("_decode_q8_plans", "_prefill_q8_plans"):
+        monkeypatch.setattr(ops, plans, ops._Plans())
+    pool = torch.zeros(64, 2, 64, dtype=torch.int8)
+    sc, q = torch.zeros(4, 2), torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    bt, ctx = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    qs = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+    ops.decode_plan_q8(q, pool, bt, 16)
+    ops.prefill_plan_q8(q, pool, bt, qs, 16)
+    irb.paged_decode_q8(q, pool, pool, sc, sc, bt, ctx, 0.1, 16)
+    irb.paged_prefill_q8(q, pool, pool, sc, sc, bt, ctx, qs, 0.1, 16)
+    assert [name for name, _ in lib.seen] == [
+        "ir_paged_decode_q8_plan", "ir_paged_decode_q8_workspace_size",
+        "ir_paged_prefill_q8_plan", "ir_paged_prefill_q8_workspace_size",
+        "ir_paged_decode_q8_workspace_size", "ir_paged_decode_q8",
+        "ir_paged_prefill_q8_workspace_size", "ir_paged_prefill_q8"]
+    assert all(dev == 1 for _, dev in lib.seen) and now == [0]
