@@ -73,6 +73,20 @@ def prefill_frame(q: torch.Tensor, paged, mask: torch.Tensor, layer_idx: int,
     return out
 
 
+def decode_rows(q: torch.Tensor, pool, bt: torch.Tensor, ctx: torch.Tensor, layer_idx: int,
+                scale: float) -> torch.Tensor:
+    """Read path of a decode call ``q [B, 1, H, D]`` whose K/V are in the pool."""
+    b, _, h, d = q.shape
+    out = torch.empty((b, 1, h, d), dtype=q.dtype, device=q.device)
+    if isinstance(pool, PagedKVPoolQ8):
+        ops.paged_decode_q8(q.reshape(b, h, d), *pool.layer(layer_idx), bt, ctx, scale,
+                            pool.block_size, out=out.view(b, h, d))
+        return out
+    ops.paged_decode(q.reshape(b, h, d), pool.k[layer_idx], pool.v[layer_idx], bt, ctx, scale,
+                     pool.block_size, out=out.view(b, h, d))
+    return out
+
+
 def clear_metadata_cache() -> None:
     with _cache_lock:
         _cache.clear()
@@ -105,20 +119,11 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, paged,
                    paged.write_slots)
         return prefill_frame(q, paged, mask, layer_idx, scale)
     bt, ctx = block_metadata(paged, mask)
-    q3 = q.reshape(b, h, d)
-    out = torch.empty((b, 1, h, d), dtype=q.dtype, device=q.device)
-    if isinstance(pool, PagedKVPoolQ8):
-        pool.write(layer_idx, k.reshape(-1, hkv, d), v.reshape(-1, hkv, d),
-                   paged.write_slots)
-        ops.paged_decode_q8(q3, *pool.layer(layer_idx), bt, ctx, scale, pool.block_size,
-                            out=out.view(b, h, d))
-    elif paged.use_triton:
-        ops.paged_decode_write(q3, k.reshape(b, hkv, d), v.reshape(b, hkv, d),
+    if paged.use_triton and not isinstance(pool, PagedKVPoolQ8):
+        out = torch.empty((b, 1, h, d), dtype=q.dtype, device=q.device)
+        ops.paged_decode_write(q.reshape(b, h, d), k.reshape(b, hkv, d), v.reshape(b, hkv, d),
                                pool.k[layer_idx], pool.v[layer_idx], paged.write_slots,
                                bt, ctx, scale, pool.block_size, out=out.view(b, h, d))
-    else:
-        pool.write(layer_idx, k.reshape(-1, hkv, d), v.reshape(-1, hkv, d),
-                   paged.write_slots)
-        ops.paged_decode(q3, pool.k[layer_idx], pool.v[layer_idx], bt, ctx, scale,
-                         pool.block_size, out=out.view(b, h, d))
-    return out
+        return out
+    pool.write(layer_idx, k.reshape(-1, hkv, d), v.reshape(-1, hkv, d), paged.write_slots)
+    return decode_rows(q, pool, bt, ctx, layer_idx, scale)

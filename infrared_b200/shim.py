@@ -41,6 +41,11 @@ infrared:
   write in its epilogue: the new K/V rows go from the accumulator to their
   slots), then ``ir_paged_decode_rope`` attends with RoPE applied to q.
 
+A context whose pool is a ``PagedKVPoolQ8`` goes the same way: the pool's own
+``write`` quantises, decode calls read through ``ir_paged_decode_q8`` and packed
+frames through ``ir_paged_prefill_q8`` (the fused forwards keep infrared's own
+``Attention.forward`` for it, which ends in the same seam).
+
 The replacement read path trusts the engine's decode metadata: the mask is a
 prefix of zeros and ``gather_slots`` lists whole blocks; a call that breaks
 either is reported by the device error flag (``check_device_errors``).
@@ -54,7 +59,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
-from .attention import block_metadata, prefill_frame
+from .attention import block_metadata, decode_rows, prefill_frame
 
 _SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -76,15 +81,10 @@ def paged_attention_b200(q: torch.Tensor, paged, mask: torch.Tensor, layer_idx: 
                          scale: float, n_rep: int) -> torch.Tensor:
     """Read path with the signature of ``_paged_attention_triton``
     (triton_attention.py:310-318): the pool already holds this step's K/V."""
-    b, sq, h, d = q.shape
-    if sq != 1:
+    if q.shape[1] != 1:
         return prefill_frame(q, paged, mask, layer_idx, scale)
-    pool = paged.pool
     bt, ctx = block_metadata(paged, mask)
-    out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
-    ops.paged_decode(q.reshape(b, h, d), pool.k[layer_idx], pool.v[layer_idx], bt, ctx,
-                     scale, pool.block_size, out=out.view(b, h, d))
-    return out
+    return decode_rows(q, paged.pool, bt, ctx, layer_idx, scale)
 
 
 def _make_write(original):

@@ -187,6 +187,53 @@ def test_shim_routes_decode_to_b200(dtype):
         h.uninstall()
 
 
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")
+@pytest.mark.parametrize("kv", [torch.float8_e4m3fn, torch.int8])
+def test_installed_seam_serves_an_8bit_pool(kv):
+    """A packed frame, then decode steps, of a context with an 8-bit pool: what
+    ``paged_attention`` of this package gives on a pool of the same rows."""
+    import infrared_b200 as irb
+
+    ta, pk, calls = _stand_in_seam()
+    rng = np.random.default_rng(5)
+    nh, nkv, d, bs, dt = 14, 2, 64, 16, torch.bfloat16
+    bt = rng.permutation(12)[:8].reshape(2, 4).astype(np.int32)
+    qls = [20, 37]
+    fr = orc.varlen_frame(bt, [0, 0], qls, bs)
+
+    def dev(x):
+        return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+    def rows(b, s, heads):
+        return dev(rng.normal(size=(b, s, heads, d))).to(dt)
+
+    steps = [(*(rows(1, 57, n) for n in (nh, nkv, nkv)), dev(fr["write_slots"]),
+              dev(fr["gather_slots"]).reshape(1, -1),
+              dev(orc.varlen_mask(fr["q_seq_ids"], fr["q_pos"], fr["k_seq_ids"], fr["k_pos"])))]
+    for i in (1, 2):
+        ctx = np.array(qls, np.int32) + i
+        t = int(ctx.max())
+        steps.append((*(rows(2, 1, n) for n in (nh, nkv, nkv)), dev(wl.tail_slots(bt, ctx, bs)),
+                      dev(orc.gather_slots_from_tables(bt, ctx, bs, t)),
+                      dev(orc.decode_mask(ctx, t))))
+
+    def run(attend):
+        pool = irb.PagedKVPoolQ8(2, 12, bs, nkv, d, dt, kv)
+        return [attend(q, k, v, irb.PagedContext(pool, ws, gs), mask, 1, d ** -0.5, nh // nkv)
+                for q, k, v, ws, gs, mask in steps]
+
+    h = shim.install(ta, pk, graph_inputs=False, prefill=True)
+    try:
+        got = run(ta.paged_attention)
+    finally:
+        h.uninstall()
+    assert calls == {"b200": 3, "naive": 0}
+    for a, b in zip(got, run(irb.paged_attention)):
+        assert torch.equal(a, b)
+    irb.check_device_errors()
+
+
 # ---------------------------------------------------------------- RoPE-fused forward
 
 
