@@ -464,8 +464,9 @@ size_t ir_cache_write_q8_workspace_size(int64_t num_tokens, int64_t num_slots,
  * rows touch, with amax the largest finite magnitude of the rows,
  *   scale = max(scale, smallest power of two s >= 2^-126 with
  *                      amax <= 448 s (e4m3) or 127 s (int8)),
- * the codes of the block's other rows are rescaled if it grew, and the new
- * rows become round(x / scale), ties to even. A write that holds a block's
+ * the codes of the block's other rows are rescaled if it grew (int8: rounded
+ * again, so that such a row is off by less than one unit of the scale instead of
+ * half a unit), and the new rows become round(x / scale), ties to even. A write that holds a block's
  * first row (slot % block_size == 0) begins the block: its old scale does not
  * count and rows that the call does not write are no longer defined. So a
  * block filled in order, by one call or token by token, ends with the scale of

@@ -2,12 +2,19 @@
 //
 // A pool holds codes [num_slots, Hkv, D] and one fp32 scale per (block, kv
 // head); a row's value is code * scale. The scales the cache write makes are
-// powers of two: dividing by one is exact, so the only rounding of a stored
-// value is the code's own (half a unit of its last place: 2^-4 of the value in
-// e4m3, scale / 2 in int8), and raising a scale later moves an e4m3 code
-// without another rounding unless it becomes subnormal. For a floating-point
-// code a finer scale would gain nothing. Readers multiply by the scale in fp32
-// and take any value of it.
+// powers of two: dividing by one is exact, so the only rounding of a value
+// written under its block's final scale is the code's own (half a unit of its
+// last place: 2^-4 of the value in e4m3, scale / 2 in int8). Raising a scale
+// later moves an e4m3 code without another rounding unless it becomes
+// subnormal, but rounds an int8 code again: each scale s that it went through
+// adds up to s / 2, and every one is at most half of the next, so a value of a
+// block whose scale grew is off by less than one unit of the final scale (e4m3:
+// 2^-4 of the value and less than 2^-9 of the scale). For a floating-point code
+// a finer scale would gain nothing. An int8 one loses up to a bit against
+// amax / 127 (the largest code lies between 64 and 127); powers of two are kept
+// there too, since a scale then grows by doublings alone, so that not every
+// larger row rounds its block's codes again, and code * scale is exact in 16-bit
+// rows. Readers multiply by the scale in fp32 and take any value of it.
 #pragma once
 
 #include <cuda_fp8.h>

@@ -1149,3 +1149,39 @@ def test_prefill_fp16_over_values_beyond_its_range(d, bs, width, force, side, fm
         assert (g[r][over] == np.sign(want[over]) * np.inf).all()
         sure = np.abs(want) + tol < 65520
         assert (np.abs(g[r] - want)[sure] <= tol[sure]).all(), r
+
+
+# ---------------------------------------------------------------- blocks whose scale grows
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("seqs,hkv,d,bs", [(3, 2, 64, 16), (5, 1, 128, 32), (1100, 1, 64, 16),
+                                           (1030, 2, 64, 8)])
+def test_write_growing_blocks_stay_near_their_rows(seqs, hkv, d, bs, fmt):
+    """Blocks filled token by token (one call a step, on the short and the long path)
+    by rows that grow, so that most steps raise the scale: what is read back
+    against the rows themselves. A value goes through scales of which each is at
+    most half of the next: int8 is off by half a unit of each, less than one unit
+    of the last; e4m3 by 2^-4 of the value, and where it is subnormal by half of
+    2^-9 of each scale, less than 2^-9 of the last."""
+    rng = np.random.default_rng(bs + seqs)
+    size = 2.0 ** (rng.uniform(0.3, 1.0, size=(seqs, bs, 1, 1)).cumsum(axis=1) - 6)
+    x = dev(rng.normal(size=(seqs, bs, hkv, d)) * size).to(torch.bfloat16)
+    pools = [torch.zeros(seqs * bs, hkv, d, dtype=torch.int8, device=DEV).view(FMT[fmt])
+             for _ in range(2)]
+    scales = [torch.zeros(seqs, hkv, device=DEV) for _ in range(2)]
+    table = dev(rng.permutation(seqs))
+    raised = 0
+    for i in range(bs):
+        before = scales[0].clone()
+        row = x[:, i].contiguous()
+        irb.cache_write_q8(row, -row, *pools, *scales, table * bs + i, bs)
+        raised += int((scales[0] > before).sum())
+    assert raised > seqs * hkv * bs // 3
+    slots = (table[:, None] * bs + torch.arange(bs, device=DEV)).reshape(-1)
+    want = x.reshape(seqs * bs, hkv, d).double()
+    for pool, scale, sign in zip(pools, scales, (1, -1)):
+        back = irb.cache_gather_q8(pool, scale, slots, bs, torch.float32).double() * sign
+        last = scale[table].double().repeat_interleave(bs, dim=0)[..., None]
+        tol = last if fmt == "int8" else 2.0 ** -4 * want.abs() + 2.0 ** -9 * last
+        assert ((back - want).abs() < tol).all()
