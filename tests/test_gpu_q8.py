@@ -1185,3 +1185,36 @@ def test_write_growing_blocks_stay_near_their_rows(seqs, hkv, d, bs, fmt):
         last = scale[table].double().repeat_interleave(bs, dim=0)[..., None]
         tol = last if fmt == "int8" else 2.0 ** -4 * want.abs() + 2.0 ** -9 * last
         assert ((back - want).abs() < tol).all()
+
+
+def test_write_one_block_of_two_runs_in_a_long_call():
+    """A long call in order but for one block, whose rows come in two runs."""
+    rng = np.random.default_rng(3)
+    n, bs, nb = 3000, 16, 200
+    for fmt in ("e4m3", "int8"):
+        codes, scale, rows, slots = _write_case(rng, n, 2, 64, bs, nb, fmt, torch.bfloat16, "runs")
+        at = np.nonzero(slots // bs == slots[1500] // bs)[0]   # one row of it to the front
+        order = np.concatenate([at[1:2], np.delete(np.arange(n), at[1])])
+        _check_write(codes, scale, [x[dev(order)] for x in rows], slots[order], bs, fmt)
+
+
+# ---------------------------------------------------------------- frames of a serving step
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("chunk,path", [(150, 1), (400, 2)])
+def test_prefill_many_single_rows_and_a_chunk(chunk, path, dtype):
+    """A step of many decode rows and a chunk of a prompt: with few rows on average
+    all are decoded, the chunk's too; else the single rows are, beside it."""
+    spans = [(7 * i, 1) for i in range(25)] + [(130, chunk)] + [(50, 1)] * 5
+    check_prefill(14, 2, 64, 16, spans, dtype, "e4m3", path, width=60)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_prefill_many_sequences_under_a_wide_table(dtype):
+    """Tables far wider than any context (as a packed frame's seam makes them), where
+    the history is expanded in the blocks' own places."""
+    spans = [(5 * i, 1) for i in range(30)] + [(40, 333)]
+    check_prefill(8, 2, 64, 16, spans, dtype, "int8", 4 if dtype == torch.float32 else 2,
+                  width=9400, dirty=True)
+    check_prefill(8, 2, 64, 16, spans[:30], dtype, "e4m3", 1, width=9400)
