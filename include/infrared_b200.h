@@ -417,8 +417,9 @@ size_t ir_paged_prefill_workspace_size(const ir_prefill_shape* shape);
 
 /* out[t, h, :] for every packed query row t. context_lens and q_start are
  * int32 device arrays; a sequence with context_lens < q_len (or past the
- * block table) sets IR_DEVERR_CONTEXT_LEN and its rows are not valid output;
- * bad block ids read zeros and set IR_DEVERR_BLOCK_ID. */
+ * block table), or with rows outside [0, total_q) on the tensor-core paths,
+ * sets IR_DEVERR_CONTEXT_LEN and its rows are not valid output (nothing outside
+ * of out is written); bad block ids read zeros and set IR_DEVERR_BLOCK_ID. */
 int ir_paged_prefill(void* out, const void* q, const void* k_pool, const void* v_pool,
                      const int32_t* block_tables, const int32_t* context_lens,
                      const int32_t* q_start, const ir_prefill_shape* shape, void* workspace,

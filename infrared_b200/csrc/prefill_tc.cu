@@ -158,7 +158,8 @@ __device__ __forceinline__ Item item_of(const PrefillArgs& a, int it, int lane) 
   const int ql = a.q_start[sq + 1] - qs;
   const int qt = (ql + TR - 1) / TR - 1 - t;
   const int ctx = a.context_lens[sq];
-  if (ctx < ql || ctx > a.max_ctx) {
+  // (rows outside the packed ones would be written outside of out)
+  if (ctx < ql || ctx > a.max_ctx || qs < 0 || ql > a.total_q - qs) {
     x.s = -2;
     return x;
   }

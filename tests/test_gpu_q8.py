@@ -1218,3 +1218,48 @@ def test_prefill_many_sequences_under_a_wide_table(dtype):
     check_prefill(8, 2, 64, 16, spans, dtype, "int8", 4 if dtype == torch.float32 else 2,
                   width=9400, dirty=True)
     check_prefill(8, 2, 64, 16, spans[:30], dtype, "e4m3", 1, width=9400)
+
+
+# ---------------------------------------------------------------- rows outside the frame
+
+
+@pytest.mark.parametrize("pool8", [True, False])
+@pytest.mark.parametrize("dtype,force", [(torch.bfloat16, 2), (torch.float16, 2), (torch.bfloat16, 3),
+                                         (torch.float32, 0), (torch.bfloat16, 1)])
+@pytest.mark.parametrize("q_start", [[0, 40, 300], [-60, 40, 70], [0, 40, 2 ** 31 - 1],
+                                     [-2 ** 31, 40, 70]])
+def test_prefill_rows_outside_the_frame_write_nothing(q_start, dtype, force, pool8):
+    """q_start that reaches past the packed rows, or before them: the sequence's rows
+    outside are not written (here they lie in the same buffer, before and behind)."""
+    rng = np.random.default_rng(2)
+    n, h, hkv, d, bs = 70, 8, 2, 128, 16
+    f = wl.prefill_frame("t", 3, [300, 300], [40, 30], h, hkv, d, bs)
+    kc, ks = make_pool(rng, f.num_blocks, bs, hkv, d, "e4m3")
+    pool, sc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32))
+    rows = dev(q8.values(kc, ks, bs).astype(np.float32)).to(dtype)
+    q = dev(rng.normal(size=(n, h, d))).to(dtype)
+    bt, ctx = dev(f.block_tables), dev(f.context_lens)
+    good = q_start[0] == 0   # the first sequence is sound, else the second
+
+    def run(start):
+        room = torch.full((512 + n + 512, h, d), 7.0, dtype=dtype, device=DEV)
+        out = room[512:512 + n]
+        starts = dev(np.array(start, np.int32))
+        if pool8:
+            irb.paged_prefill_q8(q, pool, pool, sc, sc, bt, ctx, starts, f.scale, bs, out=out)
+        else:
+            irb.paged_prefill(q, rows, rows, bt, ctx, starts, f.scale, bs, out=out)
+        return room, out
+
+    ops.set_prefill_path(force)
+    try:
+        _, want = run([0, 40, 70])
+        room, out = run(q_start)
+    finally:
+        ops.set_prefill_path(0)
+    torch.cuda.synchronize()
+    ops.error_flag().zero_()   # (the tensor-core and tile kernels flag it, decoded rows do not)
+    assert (room[:512] == 7.0).all() and (room[512 + n:] == 7.0).all()
+    if force >= 2:
+        assert torch.equal(out[:40] if good else out[40:], want[:40] if good else want[40:])
+        assert (out[40:] == 7.0).all() if good else (out[:40] == 7.0).all()
