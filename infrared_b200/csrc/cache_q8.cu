@@ -15,8 +15,11 @@
 // and the codes; rows of a larger block, or with a value that is not finite, are
 // read again for the codes.
 //
-// Bound by HBM where calls are large: 32768 rows of 4 heads of 128, bf16, move
-// 101 MB in 24.4 us. Small calls are one launch (64 rows 3.3 us, 777 int8 5.6).
+// Large calls wait for their reads: 32768 rows of 4 heads of 128, bf16, move 101 MB
+// in 24.4 us (15.6 at the copy rate), 23 without the stores, HBM 39 % busy; 5-6 of
+// them are the two small grids that group the rows. Blocks of more than 2048
+// elements a head have no streamed form (8192 rows in blocks of 64: 13.4 us,
+// 8.8 in blocks of 16). Small calls are one launch (64 rows 3.3 us, 777 int8 5.6).
 #include "kernels.h"
 #include "quant.cuh"
 
@@ -488,7 +491,7 @@ __device__ __noinline__ void quantise_apart(const Q8WriteArgs& a, int64_t blk, i
 // while the current one is computed, so that a warp's reads never pause; every
 // lane copies and reads its own pieces. Two CTAs fill an SM's registers (32768
 // rows of 4 heads of 128, bf16, the three grids together: 24.4 us = 4.1 TB/s, against 29.2
-// with the rows in registers; a device copy of as many bytes takes 35).
+// with the rows in registers).
 template <typename T, typename C>
 __global__ void __launch_bounds__(kQThreads, 2) write_stream_kernel(const Q8WriteArgs a,
                                                                     const Q8Links l) {
@@ -710,7 +713,9 @@ inline int piece_threads(int pieces) { return pieces >= 256 ? 256 : 256 / pieces
 
 // Rows by slot; a thread reads the same piece of kRows rows at once (with more
 // CTAs in flight one does best: both sides of 32768 rows of 4 heads of 128 to
-// bf16, 101 MB, 23.7 us = 4.3 TB/s; 2 and 4 rows 24.2 and 25.5). Bound by HBM.
+// bf16, 101 MB, 23.7 us = 4.3 TB/s; 2 and 4 rows 24.2 and 25.5). Bound by the
+// chain slot, then scale and codes, of one load a thread (HBM 14 % busy, the
+// written rows stay in L2).
 constexpr int kRows = 1;
 template <typename T, typename C>
 __global__ void __launch_bounds__(256)

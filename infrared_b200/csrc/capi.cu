@@ -680,6 +680,10 @@ constexpr int kDenseBlock = 128;  // block size of the dense layout: one copy pe
 // over 300 keys 52 against 95, 64 x 4 over 50 49 against 31, but 4 x 16 over
 // 512-4096 174 against 275, 3 x 41 over 900 with 6 / 2 heads 76 against 160 (too few
 // tiles for the SMs); 4 x 80 over 500 with 16 / 1 heads of 64 92 against 59.
+// The rules go by the frame's averages and the table's width, all that the host
+// knows, and miss where sequences differ much: beside 64 single rows over
+// 512-4096, 256 rows behind 4096 keys are decoded too (174 us), 512 are not (109);
+// 16 single rows are decoded beside 1060 rows (107) but expanded beside 1100 (188).
 int plan_prefill_q8(const ir_prefill_shape* s, int fmt, PrefillQ8Plan* p) {
   int rc = check_prefill_shape(s);
   if (rc) return rc;

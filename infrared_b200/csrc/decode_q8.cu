@@ -18,9 +18,11 @@
 //
 // Bound by HBM and by fixed costs: 64 sequences of 512-4096 tokens, 28 / 4 heads
 // of 128, e4m3 (163 MB): 38.1 us = 4.3 TB/s; 4 of 32768, int8 (134 MB): 31.3 us.
-// Without the arithmetic the same copies take 35.1 and a device copy of 100 MB
-// takes 35. Around the stream stand finding the share (1.3), the first tiles'
-// tables (2.4), the first bytes (4.8), the last flush (1.4) and the merge (2.5).
+// Without the arithmetic the same copies take 35.1; at the copy rate the bytes
+// alone would take 25.5 and 20.8. Around the stream stand finding the share (1.3),
+// the first tiles' tables (2.4), the first bytes (4.8), the CTAs' different ends
+// (half of them have ended at 28, the last at 34), the last flush (1.4) and the
+// merge (2.5).
 // Short contexts (q8_seq_heads) have a CTA per sequence instead, without the
 // first and the last of these: one of 201 tokens, int8, 2 heads of 64, 5.5 us.
 //
