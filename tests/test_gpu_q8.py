@@ -1263,3 +1263,38 @@ def test_prefill_rows_outside_the_frame_write_nothing(q_start, dtype, force, poo
     if force >= 2:
         assert torch.equal(out[:40] if good else out[40:], want[:40] if good else want[40:])
         assert (out[40:] == 7.0).all() if good else (out[:40] == 7.0).all()
+
+
+def test_prefill_fp16_graph_follows_the_scales():
+    """A captured fp16 prefill whose pool's scales change between replays: which rows
+    leave the tensor cores is found anew each time, on another stream too."""
+    rng = np.random.default_rng(8)
+    f = wl.prefill_frame("t", 3, [40, 0], [100, 60], 8, 2, 64, 16)
+    kc, ks = make_pool(rng, f.num_blocks, 16, 2, 64, "e4m3")
+    pool, sc, vsc = codes_to(kc, "e4m3"), dev(ks.astype(np.float32)), dev(ks.astype(np.float32))
+    q = dev(rng.normal(size=(160, 8, 64))).to(torch.float16)
+    bt, ctx, qs = dev(f.block_tables), dev(f.context_lens), dev(f.q_start)
+    call = lambda **kw: irb.paged_prefill_q8(q, pool, pool, sc, vsc, bt, ctx, qs, f.scale, 16,  # noqa: E731
+                                             **kw)
+    large = vsc.clone()
+    large[int(f.block_tables[0, 4])] = 2.0 ** 8
+    small = vsc.clone()
+    vsc.copy_(large)
+    want_large = call()
+    vsc.copy_(small)
+    want = call()
+    assert not torch.equal(want, want_large)
+    out = torch.empty_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out=out)
+    side = torch.cuda.Stream()
+    for scales, expect in ((small, want), (large, want_large), (small, want), (large, want_large)):
+        vsc.copy_(scales)
+        g.replay()
+        assert torch.equal(out, expect)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = call()
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(other, expect)
