@@ -145,7 +145,8 @@ struct Item {
 
 // Item `it` of the list (q tile major, head minor; the q tiles of a sequence
 // from the last, longest one down). Warp-collective: every lane gets the same.
-template <int TR = kRows>
+// EXACT: a.exact_from may be given (fp16).
+template <int TR, bool EXACT>
 __device__ __forceinline__ Item item_of(const PrefillArgs& a, int it, int lane) {
   Item x;
   x.h = it % a.H;
@@ -166,7 +167,7 @@ __device__ __forceinline__ Item item_of(const PrefillArgs& a, int it, int lane) 
   x.r0 = qs + qt * TR;
   x.nrows = min(TR, ql - qt * TR);
   x.pos0 = ctx - ql + qt * TR;
-  if (a.exact_from != nullptr) {  // the fp32 kernel's rows
+  if (EXACT && a.exact_from != nullptr) {  // the fp32 kernel's rows
     x.nrows = min(x.nrows, a.exact_from[sq] - x.pos0);
     if (x.nrows <= 0) {
       x.s = -3;
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NS = L::NS;
   constexpr int TR = PAIR ? 2 * kRows : kRows;  // query rows of a work item
   constexpr bool kBf16 = DT<T>::code == IR_DTYPE_BF16;
+  constexpr bool kExact = !kBf16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0, ii = 0;
     int g_prev = -1;  // the previous item's last tile
     for (int it = unit; it < n_items && ok; it += units) {
-      const Item x = item_of<TR>(a, it, lane);
+      const Item x = item_of<TR, kExact>(a, it, lane);
       if (x.s == -1) break;
       if (x.s < 0) continue;
       // Q of this item, once the previous item's last Q.K^T has completed
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int g = 0, ii = 0;
     for (int it = unit; it < n_items && lead; it += units) {
-      const Item x = item_of<TR>(a, it, lane);
+      const Item x = item_of<TR, kExact>(a, it, lane);
       if (x.s == -1) break;
       if (x.s < 0) continue;
       if (lane == 0 && is_qk) {
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     int g = 0, ii = 0;
     for (int it = unit; it < n_items; it += units) {
-      const Item x = item_of<TR>(a, it, lane);
+      const Item x = item_of<TR, kExact>(a, it, lane);
       if (x.s == -1) break;
       if (x.s < 0) {
         if (threadIdx.x == 0 && x.s == -2) set_err(a.err, IR_DEVERR_CONTEXT_LEN);
